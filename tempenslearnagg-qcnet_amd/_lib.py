@@ -123,6 +123,17 @@ def _declare(lib) -> None:
     lib.qcn_coalesce_fill.argtypes = [P, P, c_int64, c_int64, P, P, P, P]
     lib.qcn_nms_select_f32.restype = c_int
     lib.qcn_nms_select_f32.argtypes = [P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, c_float, P, P, P]
+    I, L = c_int, c_int64
+    lib.qcn_rotary_embed.restype = I
+    lib.qcn_rotary_embed.argtypes = [P, L, L, I, P, L, L, I, L, I, I, P, I, I, P, POINTER(ctypes.c_int32), I, I, P, P, P]
+    lib.qcn_attn_window.restype = I
+    lib.qcn_attn_window.argtypes = [P, L, L, P, L, L, P, L, L, P, P, P, L, L, L, I, I, I, I, L, L, c_float, P, P]
+    lib.qcn_window_cache_append.restype = I
+    lib.qcn_window_cache_append.argtypes = [P, L, L, P, L, L, P, P, P, L, L, I, I, I, L, L, P, P, P, P]
+    lib.qcn_attn_window_step_workspace_bytes.restype = c_size_t
+    lib.qcn_attn_window_step_workspace_bytes.argtypes = [L, I, I, I, L, L]
+    lib.qcn_attn_window_step.restype = I
+    lib.qcn_attn_window_step.argtypes = [P, L, L, P, L, L, P, L, L, P, P, L, I, I, I, I, L, L, c_float, P, P, P, P, P, c_size_t, P]
 
 
 EXPORTED_SYMBOLS = (
@@ -133,6 +144,7 @@ EXPORTED_SYMBOLS = (
     'qcn_attn_modes_store_f32', 'qcn_attn_modes_store_bf16', 'qcn_attn_modes_cached_f32', 'qcn_attn_modes_table_slots', 'qcn_stream_copy', 'qcn_gru_blocked_rows', 'qcn_fourier_gru_input_f32', 'qcn_gru_blocked_f32',
     'qcn_motion_metrics_f32', 'qcn_to_agent_frame_f32', 'qcn_to_world_frame_f32', 'qcn_nms_select_f32',
     'qcn_csr_static_max_edges', 'qcn_csr_build_static',
+    'qcn_rotary_embed', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step_workspace_bytes', 'qcn_attn_window_step',
     'qcn_mask_pairs_count', 'qcn_mask_pairs_fill', 'qcn_coalesce_workspace_bytes', 'qcn_coalesce_count', 'qcn_coalesce_fill',
 )
 

@@ -1,0 +1,197 @@
+// Rotary positions over several axes: feature pair i of every head is turned by t = pos[token, axis(i)] * freqs[i],
+//   a' = a cos t - b sin t,   b' = a sin t + b cos t   (inverse: -t, which is also the gradient's rotation).
+// Pairs are (x[i], x[i + pairs]) or, interleaved, (x[2 i], x[2 i + 1]); features behind 2 * pairs pass through.
+//
+// HBM-bound: every element is read and written once.  The angle is formed and reduced to a fraction of a turn in fp64 (a
+// position of 10^6 times a frequency near 1 has no correct fraction in fp32: its ulp there is 0.06 rad), once per (token,
+// pair) and not per head: a block builds the (cos, sin) table of its tokens in LDS, then streams the rows past it.
+#include "sequence.hip.h"
+
+namespace {
+
+using namespace qcn_seq;
+
+constexpr int kThreads = 256;
+constexpr int kTable = 2048;      // (cos, sin) pairs a block can hold: 16 KiB
+constexpr int kMaxAxes = 8;
+
+struct Axes {
+    int first[kMaxAxes + 1];      // pair range of each axis
+};
+
+template <class T, int N> struct alignas(sizeof(T) * N) Vec { T e[N]; };
+
+struct Args {
+    const void *in[2];
+    void *out[2];
+    Rows rows[2];                 // input strides; outputs are contiguous
+    int heads[2];
+    int64_t n_tokens;
+    int dim, pairs, n_axes, tokens_per_block, heads_per_block;
+    const void *pos;
+    const float *freqs;
+    Axes axes;
+    int inverse;
+};
+
+template <class P>
+__device__ __forceinline__ float2 turn(const Args &a, int64_t token, int pair)
+{
+    int axis = 0;
+    while (axis + 1 < a.n_axes && pair >= a.axes.first[axis + 1]) ++axis;
+    const double x = (double)reinterpret_cast<const P *>(a.pos)[token * a.n_axes + axis];
+    const double rev = x * (double)a.freqs[pair] * 0.15915494309189533577;   // 1 / (2 pi)
+    const float frac = (float)(rev - rint(rev));
+    float s, c;
+    sincospif(2.f * frac, &s, &c);
+    return make_float2(c, a.inverse ? -s : s);
+}
+
+// VE elements per access.  A unit is VE pairs (two accesses) or, interleaved, VE elements; units behind the pairs copy.
+template <class T, class P, int VE, bool INTERLEAVED>
+__global__ __launch_bounds__(kThreads) void rotary_kernel(Args a)
+{
+    __shared__ float2 table[kTable];
+    const int64_t tok0 = (int64_t)blockIdx.x * a.tokens_per_block;
+    const int ntok = (int)((a.n_tokens - tok0) < a.tokens_per_block ? (a.n_tokens - tok0) : a.tokens_per_block);
+    for (int i = threadIdx.x; i < ntok * a.pairs; i += kThreads) table[i] = turn<P>(a, tok0 + i / a.pairs, i % a.pairs);
+    __syncthreads();
+
+    const int all_heads = a.heads[0] + a.heads[1];
+    const int head0 = (int)blockIdx.y * a.heads_per_block;
+    const int nheads = (all_heads - head0) < a.heads_per_block ? (all_heads - head0) : a.heads_per_block;
+    const int pair_units = INTERLEAVED ? a.dim / VE : a.pairs / VE;
+    const int units = INTERLEAVED ? pair_units : pair_units + (a.dim - 2 * a.pairs) / VE;
+    const int total = ntok * nheads * units;
+    using V = Vec<T, VE>;
+    for (int i = threadIdx.x; i < total; i += kThreads) {
+        const int u = i % units, th = i / units;
+        const int t = th / nheads;
+        int h = head0 + th % nheads;
+        const int which = h >= a.heads[0];
+        h -= which ? a.heads[0] : 0;
+        const T *src = reinterpret_cast<const T *>(a.in[which]) + (tok0 + t) * a.rows[which].tok + h * a.rows[which].head;
+        T *dst = reinterpret_cast<T *>(a.out[which]) + ((tok0 + t) * a.heads[which] + h) * (int64_t)a.dim;
+        const float2 *cs = table + t * a.pairs;
+        if (INTERLEAVED) {
+            V x = *reinterpret_cast<const V *>(src + u * VE);
+#pragma unroll
+            for (int e = 0; e + 1 < VE; e += 2) {
+                const int pair = (u * VE + e) / 2;
+                if (pair < a.pairs) {
+                    const float2 r = cs[pair];
+                    const float p = to_f32(x.e[e]), q = to_f32(x.e[e + 1]);
+                    x.e[e] = from_f32<T>(p * r.x - q * r.y);
+                    x.e[e + 1] = from_f32<T>(p * r.y + q * r.x);
+                }
+            }
+            *reinterpret_cast<V *>(dst + u * VE) = x;
+        } else if (u < pair_units) {
+            V x = *reinterpret_cast<const V *>(src + u * VE), y = *reinterpret_cast<const V *>(src + a.pairs + u * VE);
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+                const float2 r = cs[u * VE + e];
+                const float p = to_f32(x.e[e]), q = to_f32(y.e[e]);
+                x.e[e] = from_f32<T>(p * r.x - q * r.y);
+                y.e[e] = from_f32<T>(p * r.y + q * r.x);
+            }
+            *reinterpret_cast<V *>(dst + u * VE) = x;
+            *reinterpret_cast<V *>(dst + a.pairs + u * VE) = y;
+        } else {
+            const int at = 2 * a.pairs + (u - pair_units) * VE;
+            *reinterpret_cast<V *>(dst + at) = *reinterpret_cast<const V *>(src + at);
+        }
+    }
+}
+
+template <class T, class P, int VE>
+void launch_ve(const Args &a, bool interleaved, dim3 grid, hipStream_t s)
+{
+    if (interleaved)
+        hipLaunchKernelGGL((rotary_kernel<T, P, VE < 2 ? 2 : VE, true>), grid, dim3(kThreads), 0, s, a);
+    else
+        hipLaunchKernelGGL((rotary_kernel<T, P, VE, false>), grid, dim3(kThreads), 0, s, a);
+}
+
+template <class T, class P>
+void launch(const Args &a, int ve, bool interleaved, dim3 grid, hipStream_t s)
+{
+    constexpr int kMost = 16 / (int)sizeof(T);
+    if (ve >= 8 && kMost >= 8) launch_ve<T, P, kMost>(a, interleaved, grid, s);
+    else if (ve >= 4) launch_ve<T, P, 4>(a, interleaved, grid, s);
+    else if (ve >= 2) launch_ve<T, P, 2>(a, interleaved, grid, s);
+    else launch_ve<T, P, 1>(a, interleaved, grid, s);
+}
+
+template <class T>
+int launch_pos(const Args &a, int pos_type, int ve, bool interleaved, dim3 grid, hipStream_t s)
+{
+    switch (pos_type) {
+    case QCN_POS_F32: launch<T, float>(a, ve, interleaved, grid, s); break;
+    case QCN_POS_I32: launch<T, int32_t>(a, ve, interleaved, grid, s); break;
+    case QCN_POS_I64: launch<T, int64_t>(a, ve, interleaved, grid, s); break;
+    default: return QCN_ERR_INVALID_ARGUMENT;
+    }
+    QCN_CHECK_LAUNCH();
+    return QCN_OK;
+}
+
+}  // namespace
+
+extern "C" int qcn_rotary_embed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int n_q_heads, const void *k,
+                                int64_t k_tok_stride, int64_t k_head_stride, int n_k_heads, int64_t n_tokens, int dim, int dtype,
+                                const void *pos, int pos_type, int n_axes, const float *freqs, const int32_t *sections_host,
+                                int interleaved, int inverse, void *q_out, void *k_out, void *stream)
+{
+    if (n_tokens < 0 || n_q_heads < 0 || n_k_heads < 0 || dim < 2 || (dim & 1) || n_axes < 1 || n_axes > kMaxAxes || !sections_host ||
+        !dtype_known(dtype) || pos_type < QCN_POS_F32 || pos_type > QCN_POS_I64)
+        return QCN_ERR_INVALID_ARGUMENT;
+    Args a = {};
+    for (int i = 0; i < n_axes; ++i) {
+        if (sections_host[i] < 0 || sections_host[i] > dim / 2) return QCN_ERR_INVALID_ARGUMENT;
+        a.axes.first[i + 1] = a.axes.first[i] + sections_host[i];
+    }
+    a.pairs = a.axes.first[n_axes];
+    if (a.pairs < 1 || 2 * a.pairs > dim) return QCN_ERR_INVALID_ARGUMENT;
+    const int heads = n_q_heads + n_k_heads;
+    if (n_tokens == 0 || heads == 0) return QCN_OK;
+    if ((k == nullptr) != (n_k_heads == 0) || !pos || !freqs || (n_q_heads && (!q || !q_out)) || (n_k_heads && (!k || !k_out))) return QCN_ERR_INVALID_ARGUMENT;
+    if (dim > 256 || heads > 65535 || n_tokens >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    a.in[0] = q; a.in[1] = k; a.out[0] = q_out; a.out[1] = k_out;
+    a.rows[0] = {q_tok_stride, q_head_stride}; a.rows[1] = {k_tok_stride, k_head_stride};
+    a.heads[0] = n_q_heads; a.heads[1] = n_k_heads;
+    a.n_tokens = n_tokens; a.dim = dim; a.n_axes = n_axes; a.pos = pos; a.freqs = freqs; a.inverse = inverse != 0;
+
+    // widest access that every row, the pairs' second half and the passed-through features are aligned to
+    const int es = (int)dtype_bytes(dtype);
+    int ve = 16 / es;
+    const auto fits = [&](int n) {
+        if (dim % n || (!interleaved && a.pairs % n)) return false;
+        for (int i = 0; i < 2; ++i) {
+            if (!a.heads[i]) continue;
+            if (a.rows[i].tok % n || a.rows[i].head % n) return false;
+            if (((uintptr_t)a.in[i] | (uintptr_t)a.out[i]) & (uintptr_t)(n * es - 1)) return false;
+        }
+        return true;
+    };
+    while (ve > 1 && !fits(ve)) ve /= 2;
+    if (interleaved && ve < 2) return QCN_ERR_INVALID_ARGUMENT;   // a pair straddles its alignment
+
+    // 32 KiB of rows per block while that leaves blocks for the card; few tokens: the heads are spread over blocks as well
+    const int64_t row_bytes = (int64_t)heads * dim * es;
+    int tpb = (int)((32 * 1024 + row_bytes - 1) / row_bytes);
+    if (tpb > kTable / a.pairs) tpb = kTable / a.pairs;
+    const int64_t cus = qcn_num_cus();
+    while (tpb > 1 && (n_tokens + tpb - 1) / tpb < 4 * cus) tpb /= 2;
+    int hpb = heads;
+    while (hpb > 4 && (n_tokens + tpb - 1) / tpb * ((heads + hpb - 1) / hpb) < 2 * cus) hpb = (hpb + 1) / 2;
+    a.tokens_per_block = tpb;
+    a.heads_per_block = hpb;
+    const dim3 grid((unsigned)((n_tokens + tpb - 1) / tpb), (unsigned)((heads + hpb - 1) / hpb));
+    hipStream_t s = qcn_stream(stream);
+    switch (dtype) {
+    case QCN_DTYPE_F32: return launch_pos<float>(a, pos_type, ve, interleaved, grid, s);
+    case QCN_DTYPE_F16: return launch_pos<_Float16>(a, pos_type, ve, interleaved, grid, s);
+    default: return launch_pos<__bf16>(a, pos_type, ve, interleaved, grid, s);
+    }
+}

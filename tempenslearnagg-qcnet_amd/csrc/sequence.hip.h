@@ -1,0 +1,104 @@
+// Shared pieces of the sequence operators (rotary.hip, attn_window.hip, attn_window_step.hip): element types, ragged
+// sequences, the window + sinks rule.
+#pragma once
+#include "common.hip.h"
+
+namespace qcn_seq {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+
+constexpr int kMaxDim = 128;
+
+template <class T> struct Elem;
+template <> struct Elem<float> { static constexpr int kDtype = QCN_DTYPE_F32; };
+template <> struct Elem<_Float16> { static constexpr int kDtype = QCN_DTYPE_F16; };
+template <> struct Elem<__bf16> { static constexpr int kDtype = QCN_DTYPE_BF16; };
+
+template <class T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
+// one rounding to nearest even at the store; everything before it is fp32
+template <class T> __device__ __forceinline__ T from_f32(float x) { return (T)x; }
+
+static inline size_t dtype_bytes(int dtype) { return dtype == QCN_DTYPE_F32 ? 4 : 2; }
+static inline bool dtype_known(int dtype) { return dtype == QCN_DTYPE_F32 || dtype == QCN_DTYPE_F16 || dtype == QCN_DTYPE_BF16; }
+
+// a strided row tensor [tokens, heads, dim]: the features of a head are contiguous
+struct Rows {
+    int64_t tok, head;   // strides in elements
+};
+
+// rows are loaded in 16-byte pieces
+static inline bool rows_aligned(const void *p, int64_t tok, int64_t head, int dtype)
+{
+    const int64_t piece = 16 / (int64_t)dtype_bytes(dtype);
+    return ((uintptr_t)p & 15) == 0 && tok % piece == 0 && head % piece == 0;
+}
+
+__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+// Boundaries of sequence b, forced into [0, n]: a boundary tensor that is wrong on the device gives wrong rows but no access
+// outside the token tensors.
+__device__ __forceinline__ void seq_range(const int64_t *__restrict__ cu, int64_t b, int64_t n, int64_t &beg, int64_t &end)
+{
+    beg = clamp64(cu[b], 0, n);
+    end = clamp64(cu[b + 1], beg, n);
+}
+
+// Ragged tiles without a host round trip: sequence b owns the tile numbers  start(b) .. start(b + 1) - 1  with
+// start(b) = (cu[b] * rows >> shift) + b, tiles of 2^shift rows.  That is at least ceil(len * rows / tile) numbers for every sequence (the floor of a sum
+// is at least the sum of the floors), at most one too many, and start() needs no prefix sum.  The whole wave searches:
+// 64 probes per step, so 4096 sequences take two dependent loads.  Returns the last b in [0, n_seq] with start(b) <= tile;
+// n_seq itself stands for the rows behind the last sequence.
+__device__ __forceinline__ int64_t find_seq(const int64_t *__restrict__ cu, int64_t n_seq, int64_t n, int64_t rows, int shift,
+                                            int64_t tile, int lane)
+{
+    int64_t lo = 0, count = n_seq + 1;   // candidates lo .. lo + count - 1; lo always satisfies start(lo) <= tile
+    while (count > 1) {
+        const int64_t step = (count + 63) / 64;
+        const int64_t b = lo + (int64_t)lane * step;
+        const bool in = (int64_t)lane * step < count;
+        const bool ok = in && (clamp64(cu[in ? b : lo], 0, n) * rows >> shift) + b <= tile;
+        const uint64_t hits = __ballot(ok) | 1ull;
+        const int last = 63 - __builtin_clzll(hits);
+        const int64_t next = lo + (int64_t)last * step;
+        const int64_t left = lo + count - next;
+        lo = next;
+        count = left < step ? left : step;
+    }
+    return lo;
+}
+
+// slot of position p in a cache of `sinks` first tokens and a ring of `window`
+__device__ __forceinline__ int64_t cache_slot(int64_t p, int64_t sinks, int64_t window)
+{
+    return p < sinks ? p : sinks + (p - sinks) % window;
+}
+
+__device__ __forceinline__ float wave_sum(float v)
+{
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+// Streaming softmax of one row held by a whole wave: lane owns features lane and lane + 64.  -inf scores of an empty
+// prefix are kept out of the exponent, so a row that sees nothing ends with l = 0.
+struct WaveRow {
+    float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
+    __device__ __forceinline__ void add(float score, float v0, float v1)
+    {
+        const float mn = fmaxf(m, score);
+        const float base = mn == -INFINITY ? 0.f : mn;
+        const float alpha = expf(m - base), p = expf(score - base);
+        l = fmaf(l, alpha, p);
+        acc[0] = fmaf(p, v0, acc[0] * alpha);
+        acc[1] = fmaf(p, v1, acc[1] * alpha);
+        m = mn;
+    }
+    __device__ __forceinline__ float result(int i) const { return l == 0.f ? 0.f : acc[i] / l; }
+};
+
+}  // namespace qcn_seq

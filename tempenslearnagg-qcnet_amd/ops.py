@@ -26,9 +26,9 @@ _LIBRARY = torch.library.Library('qcnet_hip', 'DEF')
 OP_NAMES: List[str] = []
 
 
-def _register(name: str, schema: str, fake=None):
+def _register(name: str, schema: str, fake=None, names: List[str] = OP_NAMES):
     """Decorator: define ``qcnet_hip::<name><schema>``, register the decorated function for the CUDA key, a refusing CPU
-    kernel, and ``fake`` as the meta implementation."""
+    kernel, and ``fake`` as the meta implementation; ``names`` is the list it is entered in."""
     def deco(fn):
         _LIBRARY.define(name + schema)
         _LIBRARY.impl(name, fn, 'CUDA')
@@ -39,7 +39,7 @@ def _register(name: str, schema: str, fake=None):
         _LIBRARY.impl(name, refuse, 'CPU')
         if fake is not None:
             torch.library.register_fake('qcnet_hip::' + name, fake, lib=_LIBRARY)
-        OP_NAMES.append(name)
+        names.append(name)
         return fn
     return deco
 
@@ -1497,3 +1497,10 @@ def _coalesce_max(edge_index, edge_attr, num_nodes):
         _lib.check(lib.qcn_coalesce_fill(_ptr(ws), _ptr(offset), e, int(num_nodes), _ptr(out_index[0]), _ptr(out_index[1]),
                                          _ptr(out_attr), st), 'qcn_coalesce_fill')
     return [out_index] + ([out_attr] if out_attr is not None else [])
+
+
+# ------------------------------------------------------------------------------------------------
+# token sequences (sequence_ops.py, which needs the helpers above)
+# ------------------------------------------------------------------------------------------------
+from .sequence_ops import (SEQUENCE_OP_NAMES, attn_window, attn_window_step, rotary_embed,  # noqa: E402,F401
+                           window_cache_append)

@@ -1,0 +1,510 @@
+"""GPU: the sequence operators (rotary_embed, attn_window, window_cache_append, attn_window_step) against float64 forms
+(oracle/sequence_oracle.py, which also derives the bounds used here)."""
+import pytest
+import torch
+
+from helpers import ROOT  # noqa: F401  (puts the repository's root in sys.path)
+from oracle import sequence_oracle as ref
+
+from tempenslearnagg_qcnet_amd import _lib, ops
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda:0'
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _rand(g, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(dtype)
+
+
+def _cu(lens):
+    return torch.tensor([0] + torch.tensor(lens, dtype=torch.int64).cumsum(0).tolist())
+
+
+def _check(got, r, dtype, dim, v, what=''):
+    o, mag, reach, count = r
+    got = got.cpu().double()
+    assert got.shape == o.shape
+    assert bool(torch.isfinite(got).all()), what
+    tol = ref.tolerance(dtype, dim, o, mag, reach, count, float(v.double().abs().max()) if v.numel() else 0.0)
+    ratio = ((got - o).abs() / tol)
+    assert o.numel() == 0 or float(ratio.max()) <= 1.0, (what, float(ratio.max()), int(ratio.argmax()))
+    empty = count == 0
+    assert bool((got[empty] == 0).all()), what
+
+
+# ------------------------------------------------------------------------------------------------
+# rotary
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('n,hq,hk,dim,sections,interleaved', [
+    (1, 1, 1, 2, [1], False), (1, 8, 8, 16, [3, 3, 2], False), (61, 8, 8, 16, [3, 3, 2], False), (5, 3, 1, 128, [64], False),
+    (130, 7, 1, 80, [13, 13, 13], False), (33, 4, 2, 96, [10, 6, 5], False), (700, 2, 1, 64, [16, 8, 8], True),
+    (9, 3, 2, 30, [7], True), (9, 3, 2, 30, [7], False), (17, 1, 0, 256, [128], False), (17, 2, 1, 256, [100, 28], True),
+    (40, 5, 5, 24, [0, 4, 8], False),
+])
+def test_rotary(n, hq, hk, dim, sections, interleaved, dtype):
+    g = _gen(n + dim)
+    x = _rand(g, n, hq + hk + 1, dim, dtype=dtype, scale=2.0)
+    qk = x.to(DEV)
+    q, k = qk[:, :hq], (qk[:, hq:hq + hk] if hk else None)
+    pairs = sum(sections)
+    freqs = torch.rand(pairs, generator=g) ** 3
+    for pos in (torch.randn(n, len(sections), generator=g) * 300, torch.randint(-5, 1_000_000, (n, len(sections)), generator=g),
+                torch.randint(0, 5000, (n, len(sections)), generator=g, dtype=torch.int32)):
+        for inverse in (False, True):
+            got = ops.rotary_embed(q, k, pos.to(DEV), freqs.to(DEV), sections, interleaved, inverse)
+            for part, a, b in ((got[0], 0, hq), (got[1], hq, hq + hk)):
+                if a == b:
+                    assert part is None
+                    continue
+                want = ref.rotary(x[:, a:b], pos, freqs, sections, interleaved, inverse)
+                tol = ref.rotary_tolerance(dtype, x[:, a:b], want, pairs, interleaved)
+                assert part.is_contiguous() and part.dtype == dtype
+                assert bool(((part.cpu().double() - want).abs() <= tol).all())
+                if not interleaved:
+                    assert torch.equal(part[..., 2 * pairs:].cpu(), x[:, a:b, 2 * pairs:])     # passed through, bit for bit
+                else:
+                    assert torch.equal(part[..., 2 * pairs:].cpu(), x[:, a:b, 2 * pairs:])
+
+
+def test_rotary_passes_non_finite_features_through_and_keeps_them_in_their_pair():
+    x = torch.randn(3, 2, 16, generator=_gen(1))
+    x[1, 0, 14], x[1, 1, 3] = float('nan'), float('inf')
+    for interleaved in (False, True):
+        got, _ = ops.rotary_embed(x.to(DEV), None, torch.arange(3).view(3, 1).to(DEV), torch.ones(5, device=DEV), [5], interleaved)
+        want = ref.rotary(x, torch.arange(3).view(3, 1), torch.ones(5), [5], interleaved)
+        assert torch.equal(torch.isfinite(got.cpu()), torch.isfinite(want))
+
+
+def test_rotary_of_strided_and_odd_inputs_and_its_inverse():
+    g = _gen(2)
+    wide = _rand(g, 50, 4, 41)
+    x = wide[:, :, 1:33]                                      # odd row stride, rows 4 bytes off
+    pos, freqs = torch.randint(0, 100, (50, 2), generator=g), torch.rand(16, generator=g)
+    got, _ = ops.rotary_embed(wide.to(DEV)[:, :, 1:33], None, pos.to(DEV), freqs.to(DEV), [10, 6])
+    want = ref.rotary(x, pos, freqs, [10, 6])
+    assert bool(((got.cpu().double() - want).abs() <= ref.rotary_tolerance(torch.float32, x, want, 16, False)).all())
+    turned = x.transpose(0, 1).contiguous().transpose(0, 1).to(DEV)   # head-major memory
+    again, _ = ops.rotary_embed(turned, None, pos.to(DEV), freqs.to(DEV), [10, 6])
+    assert torch.equal(again, got)
+    back, _ = ops.rotary_embed(got, None, pos.to(DEV), freqs.to(DEV), [10, 6], inverse=True)
+    # two rotations: twice the bound of one, on rows whose pairs keep their length (|a| + |b| grows by at most sqrt 2)
+    tol = 2 * 1.5 * ref.rotary_tolerance(torch.float32, x, x.double().abs() + 1, 16, False)
+    assert bool(((back.cpu().double() - x.double()).abs() <= tol).all())
+    empty = ops.rotary_embed(torch.empty(0, 2, 8, device=DEV), torch.empty(0, 1, 8, device=DEV), torch.empty(0, 1, device=DEV),
+                             torch.ones(4, device=DEV), [4])
+    assert empty[0].shape == (0, 2, 8) and empty[1].shape == (0, 1, 8)
+
+
+def test_rotary_inverse_is_the_gradient():
+    """<g, R x> = <R^T g, x>, against differences in float64 of the definition."""
+    g = _gen(3)
+    x, up = _rand(g, 6, 2, 16), _rand(g, 6, 2, 16)
+    pos, freqs = torch.randn(6, 3, generator=g) * 20, torch.rand(8, generator=g)
+    grad, _ = ops.rotary_embed(up.to(DEV), None, pos.to(DEV), freqs.to(DEV), [3, 3, 2], inverse=True)
+    h = 1e-3
+    for n, hd, i in ((0, 0, 0), (3, 1, 9), (5, 0, 15)):
+        e = torch.zeros_like(x, dtype=torch.float64)
+        e[n, hd, i] = h
+        f = lambda t: float((ref.rotary(t, pos, freqs, [3, 3, 2]) * up.double()).sum())
+        slope = (f(x.double() + e) - f(x.double() - e)) / (2 * h)          # linear in x: exact up to float64 rounding
+        assert abs(slope - float(grad[n, hd, i])) < 1e-5
+
+
+# ------------------------------------------------------------------------------------------------
+# window attention
+# ------------------------------------------------------------------------------------------------
+CASES = [
+    # lens, extra keys per sequence, hq, hk, dim, window, sinks, masked
+    ([1], None, 1, 1, 8, 1, 0, False),
+    ([59, 59, 59], None, 8, 8, 16, 10, 1, True),
+    ([3, 0, 17, 1, 64, 65], None, 4, 2, 16, 5, 2, False),
+    ([33, 1, 100], None, 6, 2, 32, 7, 0, True),
+    ([130, 31], None, 7, 1, 64, 50, 3, False),
+    ([257], None, 4, 4, 64, 64, 16, True),
+    ([200, 5], None, 2, 1, 80, 33, 4, False),
+    ([150], None, 3, 3, 96, 1, 0, False),
+    ([97, 140], None, 4, 1, 128, 70, 5, True),
+    ([300], None, 2, 2, 128, 1000, 4, False),
+    ([1, 2, 9], [70, 3, 128], 8, 2, 64, 40, 4, False),
+    ([40, 16], [100, 0], 5, 1, 128, 64, 1, True),
+    ([20, 30], [-7, -30], 2, 1, 32, 6, 2, False),          # fewer keys than queries: the first rows stand before the first key
+    ([70], [200], 2, 1, 48, 1 << 50, 1 << 50, False),
+    ([66, 66], None, 1, 1, 24, 2, 65, False),
+]
+
+
+def _case(lens, extra, hq, hk, dim, dtype, masked, seed=0, share=0.8):
+    g = _gen(seed + dim + sum(lens))
+    lens_k = lens if extra is None else [a + b for a, b in zip(lens, extra)]
+    nq, nk = sum(lens), sum(lens_k)
+    q, k, v = _rand(g, nq, hq, dim, dtype=dtype, scale=1.5), _rand(g, nk, hk, dim, dtype=dtype), _rand(g, nk, hk, dim, dtype=dtype)
+    mask = torch.rand(nk, generator=g) < share if masked else None
+    return q, k, v, _cu(lens), (None if extra is None else _cu(lens_k)), mask
+
+
+def _dev(*ts):
+    return [None if t is None else t.to(DEV) for t in ts]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('case', range(len(CASES)))
+def test_window(case, dtype):
+    lens, extra, hq, hk, dim, win, sinks, masked = CASES[case]
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hk, dim, dtype, masked)
+    dq, dk, dv, dcq, dck, dm = _dev(q, k, v, cu_q, cu_k, mask)
+    got = ops.attn_window(dq, dk, dv, dcq, win, sinks, cu_k=dck, key_mask=dm)
+    _check(got, ref.window(q, k, v, cu_q, win, sinks, cu_k, mask), dtype, dim, v)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [16, 64, 128])
+def test_window_views_scale_and_rows_behind_the_last_sequence(dim, dtype):
+    g = _gen(dim)
+    lens, hq, hk = [37, 90], 4, 2
+    n, behind = sum(lens), 11
+    qkv = _rand(g, n + behind, hq + 2 * hk, dim, dtype=dtype)
+    cu = _cu(lens)
+    d = qkv.to(DEV)
+    got = ops.attn_window(d[:, :hq], d[:, hq:hq + hk], d[:, hq + hk:], cu.to(DEV), 20, 2, scale=0.37)
+    q, k, v = qkv[:n, :hq], qkv[:n, hq:hq + hk], qkv[:n, hq + hk:]
+    _check(got[:n], ref.window(q, k, v, cu, 20, 2, scale=0.37), dtype, dim, v)
+    assert bool((got[n:] == 0).all())
+    odd = _rand(g, n, hq, dim + 1, dtype=dtype)                          # rows that are not 16-byte aligned: copied
+    dk, dv = k.contiguous().to(DEV), v.contiguous().to(DEV)
+    a = ops.attn_window(odd.to(DEV)[..., :dim], dk, dv, cu.to(DEV), 20, 2)
+    _check(a, ref.window(odd[..., :dim], k, v, cu, 20, 2), dtype, dim, v)
+    flat = ops.attn_window(odd.to(DEV)[..., :dim], dk, dv, cu.to(DEV), 20, 2, scale=0.0)      # scale 0: the plain mean
+    _check(flat, ref.window(odd[..., :dim], k, v, cu, 20, 2, scale=0.0), dtype, dim, v)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim,hq,hk', [(16, 8, 8), (64, 4, 2), (128, 4, 1)])
+def test_window_ignores_what_masked_and_unseen_places_hold(dim, hq, hk, dtype):
+    """NaN and infinities in keys and values that a row does not see change nothing for it: masked ones for all rows, later and
+    older ones for the rows that do not reach them."""
+    lens = [150, 70]
+    q, k, v, cu, _, mask = _case(lens, None, hq, hk, dim, dtype, True, seed=5)
+    want = ref.window(q, k, v, cu, 40, 2, None, mask)
+    for fill in (float('nan'), float('inf'), -float('inf')):
+        kk, vv = k.clone(), v.clone()
+        kk[~mask], vv[~mask] = fill, fill
+        _check(ops.attn_window(*_dev(q, kk, vv, cu), 40, 2, key_mask=mask.to(DEV)), want, dtype, dim, v, fill)
+        # one visible key's value is not finite: only the rows that see it (positions 30 .. 69 of the first sequence) follow
+        mask2 = mask.clone()
+        mask2[30] = True
+        vv[30] = fill
+        got = ops.attn_window(*_dev(q, kk if mask[30] else torch.where(torch.arange(220)[:, None, None] == 30, k, kk), vv, cu), 40, 2,
+                              key_mask=mask2.to(DEV)).cpu()
+        sees = torch.zeros(220, dtype=torch.bool)
+        sees[30:70] = True
+        assert not bool(torch.isfinite(got[sees]).any())
+        w2 = ref.window(q, k, v, cu, 40, 2, None, mask)
+        if bool(mask[30]):
+            keep = ~sees
+            tol = ref.tolerance(dtype, dim, *w2, float(v.double().abs().max()))
+            assert bool(((got.double() - w2[0]).abs() <= tol)[keep].all())
+        else:
+            assert bool(torch.isfinite(got[~sees]).all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_window_all_masked_and_large_scores(dtype):
+    q, k, v, cu, _, _ = _case([45, 30], None, 4, 2, 32, dtype, False, seed=6)
+    none = torch.zeros(75, dtype=torch.bool)
+    assert bool((ops.attn_window(*_dev(q, k, v, cu), 9, 1, key_mask=none.to(DEV)) == 0).all())
+    # scores of several thousands: the running maximum moves by far more than any exponent range
+    q2, k2 = q * 40, k * 40
+    q2, k2 = q2.to(dtype), k2.to(dtype)
+    r = ref.window(q2, k2, v, cu, 30, 1)
+    got = ops.attn_window(*_dev(q2, k2, v, cu), 30, 1).cpu().double()
+    assert bool(torch.isfinite(got).all())
+    tol = ref.tolerance(dtype, 32, *r, float(v.double().abs().max()))
+    assert bool(((got - r[0]).abs() <= tol).all())
+
+
+def test_window_bad_boundaries_stay_inside():
+    """Boundaries that are wrong on the device give wrong rows, not wild accesses; the right sequences of a next call are right."""
+    q, k, v, cu, _, _ = _case([45, 30], None, 4, 2, 64, torch.bfloat16, False, seed=7)
+    dq, dk, dv = _dev(q, k, v)
+    for bad in ([0, 100, 50], [0, 40, 1 << 40], [0, -5, 75], [75, 0, 75]):
+        out = ops.attn_window(dq, dk, dv, torch.tensor(bad, device=DEV), 9, 1)
+        assert out.shape == q.shape
+    torch.cuda.synchronize()
+    _check(ops.attn_window(dq, dk, dv, cu.to(DEV), 9, 1), ref.window(q, k, v, cu, 9, 1), torch.bfloat16, 64, v)
+
+
+def test_window_of_nothing():
+    e = lambda *s: torch.empty(*s, device=DEV)
+    z = torch.zeros(1, dtype=torch.int64, device=DEV)
+    assert ops.attn_window(e(0, 2, 16), e(0, 2, 16), e(0, 2, 16), z, 4).shape == (0, 2, 16)
+    # queries without any key are rows that see nothing; no sequence at all: rows behind the last one
+    got = ops.attn_window(torch.ones(5, 2, 16, device=DEV), e(0, 2, 16), e(0, 2, 16), torch.tensor([0, 5], device=DEV), 4,
+                          cu_k=torch.tensor([0, 0], device=DEV))
+    assert bool((got == 0).all())
+    assert bool((ops.attn_window(*[torch.ones(5, 2, 16, device=DEV)] * 3, z, 4) == 0).all())
+
+
+# ------------------------------------------------------------------------------------------------
+# cache
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lens,ages,hk,dim,win,sinks,masked', [
+    ([1], [0], 1, 8, 1, 0, False), ([5, 0, 40, 1], [0, 7, 3, 100], 2, 16, 6, 2, True), ([59] * 5, [0] * 5, 8, 16, 50, 1, True),
+    ([100, 33, 17], [0, 1 << 40, 15], 3, 128, 20, 4, False), ([70, 9], [2, -1], 2, 80, 64, 3, True),
+    ([16, 16, 32], [1, 2, 3], 1, 64, 3, 16, False),
+])
+def test_append(lens, ages, hk, dim, win, sinks, masked, dtype):
+    g = _gen(sum(lens))
+    n, b, slots = sum(lens), len(lens), win + sinks
+    behind = 3
+    k, v = _rand(g, n + behind, hk, dim, dtype=dtype), _rand(g, n + behind, hk, dim, dtype=dtype)
+    kc, vc = _rand(g, b, hk, slots, dim, dtype=dtype), _rand(g, b, hk, slots, dim, dtype=dtype)
+    mc = torch.rand(b, slots, generator=g) < 0.5 if masked else None
+    km = torch.rand(n + behind, generator=g) < 0.5 if masked else None
+    cu, lengths = _cu(lens), torch.tensor(ages)
+    dk, dv, dcu, dl, dkc, dvc, dkm, dmc = _dev(k, v, cu, lengths, kc, vc, km, mc)
+    ops.window_cache_append(dk, dv, dcu, dl, dkc, dvc, sinks, key_mask=dkm, mask_cache=dmc)
+    ref.append(k, v, cu, lengths, kc, vc, sinks, km, mc)
+    assert torch.equal(dkc.cpu(), kc) and torch.equal(dvc.cpu(), vc) and torch.equal(dl.cpu(), lengths)
+    assert mc is None or torch.equal(dmc.cpu(), mc)
+
+
+STEPS = [
+    # batch ages, hq, hk, dim, window, sinks, masked
+    ([0], 1, 1, 8, 1, 0, False),
+    ([0, 1, 5, 49, 50, 51, 300, -1], 8, 8, 16, 50, 1, True),
+    ([3, 700, 0], 4, 2, 32, 100, 4, False),
+    ([20000, 15, 257], 7, 1, 64, 260, 3, True),
+    ([1000, 1 << 41], 16, 1, 80, 65, 0, False),
+    ([129, 64, 5000], 20, 1, 96, 130, 16, True),
+    ([4103, 0, 4200, -7, 2000], 8, 2, 128, 1500, 4, False),
+    ([6000], 4, 1, 128, 4096, 4, False),
+    ([9000, 8000], 40, 2, 64, 2500, 0, True),
+]
+
+
+def _step_case(ages, hq, hk, dim, win, sinks, masked, dtype, seed=0):
+    g = _gen(seed + dim + win)
+    b, slots = len(ages), win + sinks
+    q, k, v = _rand(g, b, hq, dim, dtype=dtype, scale=1.5), _rand(g, b, hk, dim, dtype=dtype), _rand(g, b, hk, dim, dtype=dtype)
+    kc, vc = _rand(g, b, hk, slots, dim, dtype=dtype), _rand(g, b, hk, slots, dim, dtype=dtype)
+    mc = torch.rand(b, slots, generator=g) < 0.8 if masked else None
+    km = torch.rand(b, generator=g) < 0.6 if masked else None
+    return q, k, v, torch.tensor(ages), kc, vc, km, mc
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('case', range(len(STEPS)))
+def test_step(case, dtype):
+    ages, hq, hk, dim, win, sinks, masked = STEPS[case]
+    q, k, v, lengths, kc, vc, km, mc = _step_case(ages, hq, hk, dim, win, sinks, masked, dtype)
+    # slots that no position has filled hold what they hold
+    for b, age in enumerate(ages):
+        if 0 <= age < win + sinks - 1:
+            kc[b, :, age + 1:], vc[b, :, age + 1:] = float('nan'), float('nan')
+    dq, dk, dv, dl, dkc, dvc, dkm, dmc = _dev(q, k, v, lengths, kc, vc, km, mc)
+    got = ops.attn_window_step(dq, dk, dv, dl, dkc, dvc, sinks, key_mask=dkm, mask_cache=dmc)
+    r = ref.step(q, k, v, lengths, kc, vc, sinks, km, mc)
+    _check(got, r, dtype, dim, torch.cat([torch.nan_to_num(vc.double()).abs().amax().view(1)]))
+    same = lambda a, b: torch.equal(torch.nan_to_num(a.cpu(), 7.0), torch.nan_to_num(b, 7.0))
+    assert same(dkc, kc) and same(dvc, vc) and torch.equal(dl.cpu(), lengths)
+    assert mc is None or torch.equal(dmc.cpu(), mc)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_step_ignores_what_masked_slots_hold(dtype):
+    q, k, v, lengths, kc, vc, km, mc = _step_case([500, 40, 7], 8, 2, 64, 300, 4, True, dtype, seed=3)
+    for fill in (float('nan'), float('inf')):
+        a, b = kc.clone(), vc.clone()
+        a.masked_fill_(~mc[:, None, :, None], fill)
+        b.masked_fill_(~mc[:, None, :, None], fill)
+        dkc, dvc, dmc = _dev(a, b, mc)
+        got = ops.attn_window_step(*_dev(q, k, v, lengths), dkc, dvc, 4, key_mask=km.to(DEV), mask_cache=dmc)
+        _check(got, ref.step(q, k, v, lengths, kc.clone(), vc.clone(), 4, km, mc.clone()), dtype, 64, vc, fill)
+    gone = torch.zeros_like(mc).to(DEV)
+    got = ops.attn_window_step(*_dev(q, k, v, lengths, kc, vc), 4, key_mask=torch.zeros(3, dtype=torch.bool, device=DEV), mask_cache=gone)
+    assert bool((got == 0).all())
+
+
+# ------------------------------------------------------------------------------------------------
+# together
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('hq,hk,dim,win,sinks', [(8, 8, 16, 10, 1), (8, 2, 64, 24, 4)])
+def test_prefill_append_and_steps_are_the_whole_sequence(hq, hk, dim, win, sinks, dtype):
+    """Rotate, attend and cache a ragged prefix, then rotate + step token by token (one row leaves the batch on the way): every
+    step's output is the row that one pass over the whole sequence gives."""
+    g = _gen(11)
+    prefix, more = [31, 5, 0], 9
+    lens = [p + more for p in prefix]
+    n = sum(lens)
+    qkv = _rand(g, n, hq + 2 * hk, dim, dtype=dtype).to(DEV)
+    mask = (torch.rand(n, generator=g) < 0.8).to(DEV)
+    cu = _cu(lens).to(DEV)
+    pos = torch.cat([torch.arange(m) for m in lens]).view(n, 1).to(DEV)
+    freqs = torch.rand(dim // 2, generator=g).to(DEV)
+    q, k = ops.rotary_embed(qkv[:, :hq], qkv[:, hq:hq + hk], pos, freqs, [dim // 2])
+    v = qkv[:, hq + hk:]
+    want = ref.window(q.cpu(), k.cpu(), v.cpu(), cu.cpu(), win, sinks, key_mask=mask.cpu())
+    _check(ops.attn_window(q, k, v, cu, win, sinks, key_mask=mask), want, dtype, dim, v)
+    starts = cu[:-1].tolist()
+    rows = torch.cat([torch.arange(s, s + m) for s, m in zip(starts, prefix)]).to(DEV)
+    b = len(lens)
+    kc, vc = torch.zeros(b, hk, win + sinks, dim, dtype=dtype, device=DEV), torch.zeros(b, hk, win + sinks, dim, dtype=dtype, device=DEV)
+    mc = torch.zeros(b, win + sinks, dtype=torch.bool, device=DEV)
+    lengths = torch.zeros(b, dtype=torch.int64, device=DEV)
+    ops.window_cache_append(k[rows], v[rows], _cu(prefix).to(DEV), lengths, kc, vc, sinks, key_mask=mask[rows], mask_cache=mc)
+    lengths += torch.tensor(prefix, device=DEV)
+    tol = ref.tolerance(dtype, dim, *want, float(v.double().abs().max()))
+    for t in range(more):
+        at = torch.tensor([s + p + t for s, p in zip(starts, prefix)], device=DEV)
+        used = lengths.clone()
+        if t >= 5:
+            used[1] = -1
+        qt, kt = ops.rotary_embed(qkv[at, :hq], qkv[at, hq:hq + hk], pos[at], freqs, [dim // 2])
+        got = ops.attn_window_step(qt, kt, v[at], used, kc, vc, sinks, key_mask=mask[at], mask_cache=mc).cpu().double()
+        for r in range(b):
+            if r == 1 and t >= 5:
+                assert bool((got[r] == 0).all())
+            else:
+                assert bool(((got[r] - want[0][at[r]]).abs() <= tol[at[r]]).all()), (t, r)
+        lengths += 1
+
+
+def test_steps_in_a_graph_on_another_stream():
+    """A captured decoding step (rotate, step, advance the lengths), replayed with eager work in between, equals the eager run."""
+    g = _gen(12)
+    b, hq, hk, dim, win, sinks = 3, 8, 2, 128, 600, 4
+    dtype = torch.bfloat16
+    freqs = torch.rand(64, generator=g).to(DEV)
+    kc0, vc0 = _rand(g, b, hk, win + sinks, dim, dtype=dtype).to(DEV), _rand(g, b, hk, win + sinks, dim, dtype=dtype).to(DEV)
+    tokens = _rand(g, 5, b, hq + 2 * hk, dim, dtype=dtype).to(DEV)
+    start = torch.tensor([0, 590, 3000], device=DEV)
+
+    def one(x, lengths, kc, vc):
+        q, k = ops.rotary_embed(x[:, :hq], x[:, hq:hq + hk], lengths.view(b, 1), freqs, [64])
+        out = ops.attn_window_step(q, k, x[:, hq + hk:], lengths, kc, vc, sinks)
+        lengths += 1
+        return out
+
+    kc, vc, lengths = kc0.clone(), vc0.clone(), start.clone()
+    eager = [one(tokens[i], lengths, kc, vc).clone() for i in range(5)]
+    gk, gv, gl, x = kc0.clone(), vc0.clone(), start.clone(), tokens[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(x, gl, gk, gv)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one(x, gl, gk, gv)
+    gk.copy_(kc0), gv.copy_(vc0), gl.copy_(start)
+    for i in range(5):
+        x.copy_(tokens[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[i]), i
+        ops.attn_window_step(tokens[0, :, :hq], tokens[0, :, hq:hq + hk], tokens[0, :, hq + hk:], start, kc0.clone(), vc0.clone(), sinks)
+    assert torch.equal(gk, kc) and torch.equal(gv, vc) and torch.equal(gl, lengths)
+
+
+def test_window_on_two_streams_is_the_same_every_time():
+    q, k, v, cu, _, mask = _case([300, 45, 170], None, 8, 2, 64, torch.bfloat16, True, seed=9)
+    dq, dk, dv, dcu, dm = _dev(q, k, v, cu, mask)
+    first = ops.attn_window(dq, dk, dv, dcu, 60, 2, key_mask=dm)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs += [ops.attn_window(dq, dk, dv, dcu, 60, 2, key_mask=dm) for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, first) for o in outs)
+
+
+# ------------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------------
+def test_refusals():
+    f = lambda *s, **kw: torch.zeros(*s, device=DEV, **kw)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int64, device=DEV)
+    cu = torch.tensor([0, 4], device=DEV)
+    q, kv = f(4, 4, 16), f(4, 2, 16)
+    with pytest.raises(ValueError):
+        ops.attn_window(q, kv, f(4, 2, 24), cu, 4)
+    with pytest.raises(ValueError):
+        ops.attn_window(f(4, 3, 16), kv, kv, cu, 4)
+    with pytest.raises(ValueError):
+        ops.attn_window(q, kv, kv, cu, 0)
+    with pytest.raises(ValueError):
+        ops.attn_window(q, kv, kv, cu, 4, -1)
+    with pytest.raises(ValueError):
+        ops.attn_window(q, f(5, 2, 16), f(5, 2, 16), cu, 4)
+    with pytest.raises(TypeError):
+        ops.attn_window(q, kv, kv, cu.int(), 4)
+    with pytest.raises(TypeError):
+        ops.attn_window(q, kv.half(), kv.half(), cu, 4)
+    with pytest.raises(TypeError):
+        ops.attn_window(q.double(), kv.double(), kv.double(), cu, 4)
+    with pytest.raises(_lib.QcnError):
+        ops.attn_window(f(4, 4, 20), f(4, 2, 20), f(4, 2, 20), cu, 4)
+    with pytest.raises(_lib.QcnError):
+        ops.attn_window(f(4, 4, 136), f(4, 2, 136), f(4, 2, 136), cu, 4)
+    for bad in (float('nan'), float('inf'), -1.0):
+        with pytest.raises(ValueError):
+            ops.attn_window(q, kv, kv, cu, 4, scale=bad)
+    with pytest.raises(ValueError):
+        ops.attn_window(q, kv, kv, cu, 4, key_mask=f(3, dtype=torch.bool))
+    with pytest.raises(_lib.QcnError):
+        ops.attn_window(q.cpu(), kv.cpu(), kv.cpu(), cu.cpu(), 4)
+    cache = lambda: f(4, 2, 6, 16)
+    one = cache()
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(4), cache(), cache(), 6)                       # no slot left for the window
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(3), cache(), cache(), 1)
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(4), one, one, 1)
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(4), f(4, 2, 16, 6).transpose(2, 3), cache(), 1)    # not contiguous
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(4), cache(), cache(), 1, key_mask=f(4, dtype=torch.bool))
+    with pytest.raises(ValueError):
+        ops.attn_window_step(q, kv, kv, i(4), cache(), cache(), 1, mask_cache=f(6, 4, dtype=torch.bool).t())
+    with pytest.raises(TypeError):
+        ops.attn_window_step(q, kv, kv, i(4).int(), cache(), cache(), 1)
+    with pytest.raises(ValueError):
+        ops.window_cache_append(kv, kv, cu, i(2), f(1, 2, 6, 16), f(1, 2, 6, 16), 1)
+    with pytest.raises(TypeError):
+        ops.window_cache_append(kv, kv, cu, i(1), f(1, 2, 6, 16).half(), f(1, 2, 6, 16).half(), 1)
+    pos = i(4, 2)
+    with pytest.raises(ValueError):
+        ops.rotary_embed(q, None, pos, f(9), [5, 4])
+    with pytest.raises(ValueError):
+        ops.rotary_embed(q, None, pos, f(8), [8])
+    with pytest.raises(TypeError):
+        ops.rotary_embed(q, None, pos.double(), f(8), [4, 4])
+    with pytest.raises(ValueError):
+        ops.rotary_embed(q, f(4, 2, 24), pos, f(8), [4, 4])
+    with pytest.raises(_lib.QcnError):
+        ops.rotary_embed(f(4, 2, 15), None, pos, f(4), [2, 2])
+    with pytest.raises(ValueError):
+        ops.rotary_embed(q, None, pos, f(0), [0, 0])
+
+
+def test_sequence_ops_trace_under_fake_tensors():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(40, 12, 64, device=DEV, dtype=torch.bfloat16)
+        q, k = ops.rotary_embed(x[:, :8], x[:, 8:10], torch.empty(40, 1, device=DEV), torch.empty(32, device=DEV), [32])
+        assert q.shape == (40, 8, 64) and k.shape == (40, 2, 64) and q.dtype == torch.bfloat16
+        o = ops.attn_window(q, k, x[:, 10:], torch.empty(3, dtype=torch.int64, device=DEV), 8, 1)
+        assert o.shape == (40, 8, 64) and o.dtype == torch.bfloat16
+        c = torch.empty(40, 2, 9, 64, device=DEV, dtype=torch.bfloat16)
+        assert ops.attn_window_step(q, k, k, torch.empty(40, dtype=torch.int64, device=DEV), c, c.clone(), 1).shape == (40, 8, 64)
