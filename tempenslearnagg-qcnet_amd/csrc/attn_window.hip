@@ -18,7 +18,7 @@ struct Args {
     int64_t n_seq, nq, nk;
     int hq, hk, group, dim;
     int64_t window, sinks;
-    float scale;
+    float scale, c2;      // c2: scale in base 2
     void *out;            // [nq, hq, dim] contiguous
 };
 
@@ -46,40 +46,532 @@ __device__ __forceinline__ void row_by_wave(const Args &a, int64_t k_beg, int64_
     if (has1) o[lane + 64] = from_f32<T>(r.result(1));
 }
 
+// Rows behind the last sequence (and of sequences that see nothing): zero.
 template <class T>
-__global__ __launch_bounds__(256) void attn_window_rows_kernel(Args a)
+__device__ __forceinline__ void zero_row(const Args &a, int64_t row, int head, int lane, int lanes)
 {
-    const int lane = threadIdx.x & 63;
+    T *o = reinterpret_cast<T *>(a.out) + (row * a.hq + head) * (int64_t)a.dim;
+    for (int d = lane; d < a.dim; d += lanes) o[d] = from_f32<T>(0.f);
+}
+
+// A tile is 2^SHIFT consecutive ROWS of one sequence and one key head; a row is a (query, query head of the group) pair, heads
+// fastest: shared keys are read once for the whole group, and a short chunk of queries still fills the tile.
+struct Tile {
+    int64_t q_beg, k_beg;   // first token of the sequence
+    int64_t rows, row0;     // rows of the sequence; first row of the tile
+    int lk, shift;          // keys of the sequence; position of query i = i + shift
+    bool behind;            // rows behind the last sequence
+};
+
+__device__ __forceinline__ Tile find_tile(const Args &a, int64_t tile, int shift, int lane)
+{
+    Tile t;
+    const int64_t b = find_seq(a.cu_q, a.n_seq, a.nq, a.group, shift, tile, lane);
+    t.behind = b == a.n_seq;
+    int64_t q_end, k_end;
+    if (t.behind) {
+        t.q_beg = clamp64(a.cu_q[b], 0, a.nq);
+        q_end = a.nq;
+        t.k_beg = k_end = 0;
+    } else {
+        seq_range(a.cu_q, b, a.nq, t.q_beg, q_end);
+        seq_range(a.cu_k, b, a.nk, t.k_beg, k_end);
+    }
+    t.rows = (q_end - t.q_beg) * a.group;
+    t.row0 = (tile - ((t.q_beg * a.group >> shift) + b)) << shift;
+    t.lk = (int)(k_end - t.k_beg);
+    t.shift = t.lk - (int)(q_end - t.q_beg);
+    return t;
+}
+
+// The keys that the positions p0 .. p1 see, as one index range 0 .. total - 1: the sinks in front of the window, then the window.
+struct Keys {
+    int sinks, start, total;
+    __device__ __forceinline__ int key(int j) const { return j < sinks ? j : j - sinks + start; }
+};
+
+__device__ __forceinline__ int window_start(const Args &a, int p) { return a.window > (int64_t)p ? 0 : (int)(p + 1 - a.window); }
+
+__device__ __forceinline__ Keys key_range(const Args &a, int p0, int p1)
+{
+    Keys k;
+    k.start = p0 < 0 ? 0 : window_start(a, p0);
+    k.sinks = a.sinks < k.start ? (int)a.sinks : k.start;
+    k.total = p1 < 0 ? 0 : k.sinks + p1 + 1 - k.start;
+    return k;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// 16 rows per wave, keys straight from memory (float32 of every width; 16-bit types up to 16 features)
+// ---------------------------------------------------------------------------------------------------------------------
+// A wave is on its own: no LDS, no barrier.  For short windows (the agents' 10 steps) every key tile is used by two or three row
+// tiles at most, so staging would cost more than the cache hits it saves; the four waves of a block take neighbouring key heads
+// of the same tokens, whose rows share cache lines.
+//
+// v_mfma_f32_16x16x4_f32: contraction index = lane >> 4.  A lane loads 4 neighbouring features (16 bytes) of its key and feeds
+// them to 4 products, so product e of piece c contracts features 16 c + 4 g + e.  V^T tile (sb, e) holds features
+// sb SB + VW m + e (m = 0 .. 15): a lane loads VW neighbouring features of a key and ends with 4 VW neighbouring features of
+// its query.
+template <class T, int DP> struct Direct {
+    static constexpr int VW = DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1);
+    static constexpr int SB = 16 * VW, NSB = DP / SB, NT = DP / 16;
+};
+
+template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
+
+template <class T, int DP>
+__global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t n_tiles)
+{
+    using L = Direct<T, DP>;
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int NU = 2;                                  // 16-key tiles per step
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int64_t tile = item / a.hq;
-    const int head = (int)(item % a.hq);
-    if (tile > a.nq + a.n_seq) return;
-    const int64_t b = find_seq(a.cu_q, a.n_seq, a.nq, 1, 0, tile, lane);
-    if (b == a.n_seq) {
-        const int64_t row = clamp64(a.cu_q[b], 0, a.nq) + tile - (clamp64(a.cu_q[b], 0, a.nq) + b);
-        if (row >= a.nq) return;
-        T *o = reinterpret_cast<T *>(a.out) + (row * a.hq + head) * (int64_t)a.dim;
-        for (int d = lane; d < a.dim; d += 64) o[d] = from_f32<T>(0.f);
+    const int64_t item = (int64_t)qcn_xcd_remap(blockIdx.x, gridDim.x) * 4 + wave;
+    const int64_t tile = item / a.hk;
+    const int kvh = (int)(item % a.hk);
+    if (tile >= n_tiles) return;
+    const Tile t = find_tile(a, tile, 4, lane);
+    if (t.row0 < 0 || t.row0 >= t.rows) return;
+    const int last = (int)((t.rows - 1 - t.row0) < 15 ? (t.rows - 1 - t.row0) : 15);
+    const int64_t row = t.row0 + (n < last ? n : last);    // lanes past the end repeat the last row and do not store
+    const int64_t qi = row / a.group;
+    const int head = kvh * a.group + (int)(row % a.group);
+    if (t.behind) {
+        if (n <= last) zero_row<T>(a, t.q_beg + qi, head, g, 4);
         return;
     }
-    int64_t q_beg, q_end, k_beg, k_end;
-    seq_range(a.cu_q, b, a.nq, q_beg, q_end);
-    seq_range(a.cu_k, b, a.nk, k_beg, k_end);
-    const int64_t i = tile - (q_beg + b);
-    if (i >= q_end - q_beg) return;
-    row_by_wave<T>(a, k_beg, i + (k_end - k_beg) - (q_end - q_beg), q_beg + i, head, lane);
+    const int p = (int)qi + t.shift;
+    const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
+    const Keys keys = key_range(a, p0, p1);
+    const int lo = p < 0 ? 0 : window_start(a, p);
+    const int lo1 = p1 < 0 ? 0 : window_start(a, p1);
+
+    const T *q = reinterpret_cast<const T *>(a.q) + (t.q_beg + qi) * a.qr.tok + head * a.qr.head;
+    const T *kb = reinterpret_cast<const T *>(a.k) + t.k_beg * a.kr.tok + kvh * a.kr.head;
+    const T *vb = reinterpret_cast<const T *>(a.v) + t.k_beg * a.vr.tok + kvh * a.vr.head;
+    const uint8_t *mask = a.key_mask ? a.key_mask + t.k_beg : nullptr;
+
+    using P4 = Pack<T, 4>;
+    using PV = Pack<T, L::VW>;
+    P4 qf[DP / 16];
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+        const int d = 16 * c + 4 * g;
+        qf[c] = *reinterpret_cast<const P4 *>(q + (d < a.dim ? d : 0));
+        if (d >= a.dim) qf[c] = P4{};
+    }
+    f32x4 o[L::NT];
+#pragma unroll
+    for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float c2 = a.c2;
+
+    for (int j0 = 0; j0 < keys.total; j0 += 16 * NU) {
+        f32x4 s[NU];
+        unsigned seen[NU];                                 // bit per key of the tile: inside the range and not masked
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int j = j0 + 16 * u + n;
+            const bool in = j < keys.total;
+            const int key = keys.key(in ? j : keys.total - 1);
+            const bool ok = in && (!mask || mask[key] != 0);
+            seen[u] = (unsigned)__ballot(ok) & 0xffffu;
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            const T *kr = kb + key * a.kr.tok;
+            P4 kf[DP / 16];
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                const int d = 16 * c + 4 * g;
+                kf[c] = *reinterpret_cast<const P4 *>(kr + (d < a.dim ? d : 0));
+                if (d >= a.dim) kf[c] = P4{};
+            }
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) {
+                if constexpr (F32) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].e[e], qf[c].e[e], s[u], 0, 0, 0);
+                } else {
+                    using V4 = typename Mat<T>::V4;
+                    s[u] = Mat<T>::mul16(__builtin_bit_cast(V4, kf[c]), __builtin_bit_cast(V4, qf[c]), s[u]);
+                }
+            }
+        }
+        // a tile whose keys every row sees needs no mask: inside the range, unmasked, up to the first row's position, inside
+        // the last row's window
+        const int jz = j0 + 16 * NU - 1;
+        const bool full = !mask && j0 >= keys.sinks && jz < keys.total && keys.key(jz) <= p0 && keys.key(j0) >= lo1;
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (!full) {
+                    const int key = keys.key(j0 + 16 * u + 4 * g + r);
+                    if (!(((seen[u] >> (4 * g + r)) & 1) && key <= p && (key >= lo || key < a.sinks))) s[u][r] = -INFINITY;
+                }
+                top = fmaxf(top, s[u][r]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+        const float scaled = top * c2;
+        if (__ballot(scaled > m + 8.f)) {
+            const float mn = scaled > m ? scaled : m;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < L::NT; ++i) o[i] *= alpha;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
+                l += s[u][r];
+            }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            int64_t at[4];
+            bool ok[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = j0 + 16 * u + 4 * g + r;
+                ok[r] = (seen[u] >> (4 * g + r)) & 1;
+                at[r] = keys.key(j < keys.total ? j : keys.total - 1) * a.vr.tok;
+            }
+#pragma unroll
+            for (int sb = 0; sb < L::NSB; ++sb) {
+                const int d = sb * L::SB + L::VW * n;
+                PV v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = *reinterpret_cast<const PV *>(vb + at[r] + (d < a.dim ? d : 0));
+                    if (!ok[r]) v[r] = PV{};               // 0 times what a masked key holds must stay 0
+                }
+#pragma unroll
+                for (int e = 0; e < L::VW; ++e) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
+                    } else {
+                        typename Mat<T>::V4 va, pb;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
+                        o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                    }
+                }
+            }
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bool bad = false;
+    T *out = reinterpret_cast<T *>(a.out) + ((t.q_beg + qi) * a.hq + head) * (int64_t)a.dim;
+#pragma unroll
+    for (int i = 0; i < L::NT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            o[i][r] *= inv;
+            bad |= !(fabsf(o[i][r]) < INFINITY);
+        }
+    unsigned repair = 0;
+    {
+        const uint64_t b = __ballot(bad && n <= last);
+        repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
+    }
+    if (n <= last && !((repair >> n) & 1)) {
+#pragma unroll
+        for (int sb = 0; sb < L::NSB; ++sb) {
+            const int d = sb * L::SB + 4 * L::VW * g;
+#pragma unroll
+            for (int part = 0; part < L::VW; ++part) {     // 4 features each
+                if (d + 4 * part >= a.dim) break;
+                P4 w;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int f = 4 * part + x;            // feature f of the lane's 4 VW: r = f / VW, e = f % VW
+                    w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW]);
+                }
+                *reinterpret_cast<P4 *>(out + d + 4 * part) = w;
+            }
+        }
+    }
+    // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
+    // Rows that came out not finite are formed again key by key.
+    for (; repair; repair &= repair - 1) {
+        const int64_t r = t.row0 + __builtin_ctz(repair);
+        row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// 128 rows per block, keys through LDS (16-bit types)
+// ---------------------------------------------------------------------------------------------------------------------
+// Four waves of 32 rows share tiles of 64 keys, double-buffered in LDS; the next tile's loads are in flight while the matrix
+// units work on this one, one barrier per tile.  v_mfma_f32_32x32x16: A = 32 keys (S^T) or 32 features (O^T), B = 32 rows.
+// With the accumulator's row order, k-step t of key half-tile u contracts keys  32 u + 16 t + {4 h .. 4 h + 3, 8 + 4 h ..}  in lane
+// half h: V^T is fetched in that order by two transposing LDS reads, P^T is the S^T registers rounded to 16 bits.
+//
+// LDS rows are swizzled in 16-byte pieces so that 16 neighbouring keys' pieces (K) and the 4 x 64 bytes of a transposing read
+// (V) cover all 64 banks.
+template <int DP> __device__ __forceinline__ int k_piece(int row, int piece)
+{
+    return piece ^ (DP == 128 ? row & 15 : DP == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
+}
+template <int DP> __device__ __forceinline__ int v_piece(int row, int piece)
+{
+    return piece ^ (DP == 128 ? (row & 3) << 2 : DP == 64 ? ((row >> 1) & 1) << 2 : 0);
+}
+
+constexpr int kRowShift = 7, kKeys = 64;
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_t n_tiles)
+{
+    constexpr int PIECES = DP / 8, PER = kKeys * PIECES / 256, NK = DP / 16, ND = DP / 32;
+    using V8 = typename Mat<T>::V8;
+    __shared__ T lds[2][2][kKeys * DP];                    // [buffer][K, V]
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t item = qcn_xcd_remap(blockIdx.x, gridDim.x);
+    const int64_t tile = item % n_tiles;
+    const int kvh = (int)(item / n_tiles);
+    const Tile t = find_tile(a, tile, kRowShift, lane);
+    if (t.row0 < 0 || t.row0 >= t.rows) return;
+    const int64_t left = t.rows - 1 - t.row0;
+    const int last = (int)(left < 127 ? left : 127);       // last row of the tile
+    if (t.behind) {
+        for (int r = wave; r <= last; r += 4)
+            zero_row<T>(a, t.q_beg + (t.row0 + r) / a.group, kvh * a.group + (int)((t.row0 + r) % a.group), lane, 64);
+        return;
+    }
+    const int r_local = wave * 32 + n;
+    const bool real = r_local <= last;
+    const int64_t row = t.row0 + (real ? r_local : last);
+    const int64_t qi = row / a.group;
+    const int head = kvh * a.group + (int)(row % a.group);
+    const int p = (int)qi + t.shift, lo = p < 0 ? 0 : window_start(a, p);
+    const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
+    const Keys keys = key_range(a, p0, p1);
+    // the wave's own rows
+    const int wa = wave * 32 < last ? wave * 32 : last, wz = wave * 32 + 31 < last ? wave * 32 + 31 : last;
+    const int wp0 = (int)((t.row0 + wa) / a.group) + t.shift, wp1 = (int)((t.row0 + wz) / a.group) + t.shift;
+    const int wlo0 = wp0 < 0 ? 0 : window_start(a, wp0), wlo1 = wp1 < 0 ? 0 : window_start(a, wp1);
+
+    const T *q = reinterpret_cast<const T *>(a.q) + (t.q_beg + qi) * a.qr.tok + head * a.qr.head;
+    const T *kb = reinterpret_cast<const T *>(a.k) + t.k_beg * a.kr.tok + kvh * a.kr.head;
+    const T *vb = reinterpret_cast<const T *>(a.v) + t.k_beg * a.vr.tok + kvh * a.vr.head;
+    const uint8_t *mask = a.key_mask ? a.key_mask + t.k_beg : nullptr;
+
+    V8 qf[NK];
+#pragma unroll
+    for (int c = 0; c < NK; ++c) {
+        const int d = 16 * c + 8 * h;
+        u32x4 x = *reinterpret_cast<const u32x4 *>(q + (d < a.dim ? d : 0));
+        if (d >= a.dim) x = u32x4{0, 0, 0, 0};
+        qf[c] = __builtin_bit_cast(V8, x);
+    }
+    f32x16 o[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float c2 = a.c2;
+    const int n_steps = (keys.total + kKeys - 1) / kKeys;
+
+    u32x4 kreg[PER], vreg[PER];
+    const auto load = [&](int j0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int x = tid + 256 * i, j = j0 + x / PIECES, d = x % PIECES * 8;
+            const bool in = j < keys.total;
+            const int key = keys.key(in ? j : keys.total - 1);
+            const int at = d < a.dim ? d : 0;
+            kreg[i] = *reinterpret_cast<const u32x4 *>(kb + key * a.kr.tok + at);
+            vreg[i] = *reinterpret_cast<const u32x4 *>(vb + key * a.vr.tok + at);
+            if (d >= a.dim) kreg[i] = u32x4{0, 0, 0, 0};
+            if (!in || (mask && !mask[key])) vreg[i] = u32x4{0, 0, 0, 0};   // 0 times what a masked key holds must stay 0
+        }
+    };
+    const auto store = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int x = tid + 256 * i, r = x / PIECES, c = x % PIECES;
+            *reinterpret_cast<u32x4 *>(&lds[buf][0][r * DP + 8 * k_piece<DP>(r, c)]) = kreg[i];
+            *reinterpret_cast<u32x4 *>(&lds[buf][1][r * DP + 8 * v_piece<DP>(r, c)]) = vreg[i];
+        }
+    };
+    if (n_steps > 0) {
+        load(0);
+        store(0);
+    }
+    __syncthreads();
+    for (int step = 0; step < n_steps; ++step) {
+        const int j0 = step * kKeys, jz = j0 + kKeys - 1;
+        if (step + 1 < n_steps) load(j0 + kKeys);
+        const T *lk = lds[step & 1][0], *lv = lds[step & 1][1];
+        const int kmin = keys.key(j0), kmax = keys.key(jz < keys.total ? jz : keys.total - 1);
+        const bool window_only = j0 >= keys.sinks;
+        const bool none = wp1 < 0 || (window_only && (kmin > wp1 || (kmax < wlo0 && kmin >= a.sinks)));
+        if (!none) {
+            f32x16 s[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NK; ++c) {
+                    const int kr = 32 * u + n;
+                    const V8 kf = *reinterpret_cast<const V8 *>(&lk[kr * DP + 8 * k_piece<DP>(kr, 2 * c + h)]);
+                    s[u] = Mat<T>::mul32(kf, qf[c], s[u]);
+                }
+            }
+            const bool full = !mask && window_only && jz < keys.total && kmax <= wp0 && kmin >= wlo1;
+            if (!full) {
+                const int j = j0 + lane;
+                const bool in = j < keys.total;
+                const uint64_t seen = __ballot(in && (!mask || mask[keys.key(in ? j : keys.total - 1)] != 0));
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int i = 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h;
+                        const int key = keys.key(j0 + i);
+                        if (!(((seen >> i) & 1) && key <= p && (key >= lo || key < a.sinks))) s[u][r] = -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+            top = fmaxf(top, other_half(top));
+            // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+            const float scaled = top * c2;
+            if (__ballot(scaled > m + 8.f)) {
+                const float mn = scaled > m ? scaled : m;
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < ND; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+                m = mn;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    V8 pb;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        l += s[u][8 * ks + i];
+                        pb[i] = from_f32<T>(s[u][8 * ks + i]);
+                    }
+                    const int i16 = lane & 15, vr = 32 * u + 16 * ks + 4 * h + (i16 >> 2);
+#pragma unroll
+                    for (int dt = 0; dt < ND; ++dt) {
+                        const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+                        const uint2 x = lds_read_transposed(&lv[vr * DP + 8 * v_piece<DP>(vr, d >> 3) + (d & 7)]);
+                        const uint2 y = lds_read_transposed(&lv[(vr + 8) * DP + 8 * v_piece<DP>(vr + 8, d >> 3) + (d & 7)]);
+                        o[dt] = Mat<T>::mul32(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
+                    }
+                }
+            }
+        }
+        if (step + 1 < n_steps) store((step + 1) & 1);
+        __syncthreads();
+    }
+    l += other_half(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[i][r] *= inv;
+            bad |= !(fabsf(o[i][r]) < INFINITY);
+        }
+    unsigned repair;
+    {
+        const uint64_t b = __ballot(bad && real);
+        repair = (unsigned)(b | (b >> 32));
+    }
+    T *out = reinterpret_cast<T *>(a.out) + ((t.q_beg + qi) * a.hq + head) * (int64_t)a.dim;
+    const bool keep = real && !((repair >> n) & 1);
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {                      // 16 features: halves hold {0-3, 8-11} and {4-7, 12-15}
+            unsigned w[2][2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const int r = 8 * x + 4 * y + 2 * z;
+                    Pack<T, 2> two = {{from_f32<T>(o[i][r]), from_f32<T>(o[i][r + 1])}};
+                    w[y][z] = __builtin_bit_cast(unsigned, two);
+                }
+            const auto s0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            const int d = 32 * i + 16 * x + 8 * h;         // after the exchange a lane holds 8 neighbouring features
+            if (keep && d < a.dim) *reinterpret_cast<u32x4 *>(out + d) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+        }
+    // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
+    // Rows that came out not finite are formed again key by key.
+    for (; repair; repair &= repair - 1) {
+        const int64_t r = t.row0 + wave * 32 + __builtin_ctz(repair);
+        row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+    }
+}
+
+template <class T, int DP>
+int launch_direct(const Args &a, hipStream_t s)
+{
+    const int64_t tiles = (a.nq * a.group >> 4) + a.n_seq + 1, blocks = (tiles * a.hk + 3) / 4;
+    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((attn_window_direct_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles);
+    QCN_CHECK_LAUNCH();
+    return QCN_OK;
+}
+
+template <class T, int DP>
+int launch_tile(const Args &a, hipStream_t s)
+{
+    const int64_t tiles = (a.nq * a.group >> kRowShift) + a.n_seq + 1, blocks = tiles * a.hk;
+    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL((attn_window_tile_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles);
+    QCN_CHECK_LAUNCH();
+    return QCN_OK;
 }
 
 template <class T>
 int launch(const Args &a, hipStream_t s)
 {
-    const int64_t items = (a.nq + a.n_seq + 1) * a.hq;
-    const int64_t blocks = (items + 3) / 4;
-    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_window_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    QCN_CHECK_LAUNCH();
-    return QCN_OK;
+    if constexpr (sizeof(T) == 4) {
+        if (a.dim <= 16) return launch_direct<T, 16>(a, s);
+        if (a.dim <= 32) return launch_direct<T, 32>(a, s);
+        if (a.dim <= 64) return launch_direct<T, 64>(a, s);
+        if (a.dim <= 96) return launch_direct<T, 96>(a, s);
+        return launch_direct<T, 128>(a, s);
+    } else {
+        if (a.dim <= 16) return launch_direct<T, 16>(a, s);
+        if (a.dim <= 32) return launch_tile<T, 32>(a, s);
+        if (a.dim <= 64) return launch_tile<T, 64>(a, s);
+        if (a.dim <= 96) return launch_tile<T, 96>(a, s);
+        return launch_tile<T, 128>(a, s);
+    }
 }
 
 }  // namespace
@@ -96,14 +588,16 @@ extern "C" int qcn_attn_window(const void *q, int64_t q_tok_stride, int64_t q_he
     if (dim < 8 || dim > kMaxDim || dim % 8) return QCN_ERR_UNSUPPORTED;
     if (n_q_tokens == 0) return QCN_OK;
     if (!q || !out || !cu_q || !cu_k || (n_k_tokens && (!k || !v))) return QCN_ERR_INVALID_ARGUMENT;
-    if (n_q_tokens >= ((int64_t)1 << 40) || n_k_tokens >= ((int64_t)1 << 40) || n_seq >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (n_q_tokens >= ((int64_t)1 << 31) || n_k_tokens >= ((int64_t)1 << 31) || n_seq >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
     if (!rows_aligned(q, q_tok_stride, q_head_stride, dtype) || !rows_aligned(out, 0, 0, dtype) ||
         (n_k_tokens && (!rows_aligned(k, k_tok_stride, k_head_stride, dtype) || !rows_aligned(v, v_tok_stride, v_head_stride, dtype))))
         return QCN_ERR_INVALID_ARGUMENT;
-    const int64_t reach = (int64_t)1 << 42;   // positions are below 2^40: larger windows and sinks mean the same
+    const int64_t reach = ((int64_t)1 << 31) - 1;   // positions are below: larger windows and sinks mean the same
     const Args a = {q, k, v, {q_tok_stride, q_head_stride}, {k_tok_stride, k_head_stride}, {v_tok_stride, v_head_stride}, cu_q, cu_k,
                     key_mask, n_seq, n_q_tokens, n_k_tokens, n_q_heads, n_kv_heads, n_q_heads / n_kv_heads, dim,
-                    window < reach ? window : reach, sinks < reach ? sinks : reach, scale, out};
+                    window < reach ? window : reach, sinks < reach ? sinks : reach, scale,
+                    // an unseen key's score is -inf and has to stay so: scale 0 becomes one that no score outgrows
+                    fmaxf(scale * kLog2e, 1e-37f), out};
     hipStream_t s = qcn_stream(stream);
     switch (dtype) {
     case QCN_DTYPE_F32: return launch<float>(a, s);

@@ -101,4 +101,50 @@ struct WaveRow {
     __device__ __forceinline__ float result(int i) const { return l == 0.f ? 0.f : acc[i] / l; }
 };
 
+// ---------------------------------------------------------------------------------------------------------------------
+// matrix operands
+// ---------------------------------------------------------------------------------------------------------------------
+// Both attention kernels form S^T = K Q^T and O^T = V^T P^T.  A lane of the accumulator then holds ONE query (column) and some
+// keys (rows), so softmax statistics are per lane plus one or two lane exchanges, and the accumulator of S^T is, register for
+// register, the B operand of the second product: the order of the contraction index is free as long as V^T follows it.
+//   32 x 32 accumulator:  column = lane & 31, row = (r & 3) + 8 (r >> 2) + 4 (lane >> 5)
+//   16 x 16 accumulator:  column = lane & 15, row = r + 4 (lane >> 4)
+template <class T> struct Mat;
+template <> struct Mat<_Float16> {
+    using V8 = f16x8;
+    using V4 = __attribute__((ext_vector_type(4))) _Float16;
+    static __device__ __forceinline__ f32x16 mul32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul16(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul16(V4 a, V4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Mat<__bf16> {
+    using V8 = bf16x8;
+    using V4 = __attribute__((ext_vector_type(4))) __bf16;
+    using S4 = __attribute__((ext_vector_type(4))) short;
+    static __device__ __forceinline__ f32x16 mul32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul16(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mul16(V4 a, V4 b, f32x4 c)
+    {
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(S4, a), __builtin_bit_cast(S4, b), c, 0, 0, 0);
+    }
+};
+
+// ds_read_b64_tr_b16: the 16 lanes of a group read 8 bytes each, taken as 4 rows (lanes 4 j .. 4 j + 3) of 16 elements; lane l
+// gets column l: element j from row j.  (Checked lane by lane on the card.)
+__device__ __forceinline__ uint2 lds_read_transposed(const void *p)
+{
+    using S4 = __attribute__((ext_vector_type(4))) short;
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4 *)p));
+}
+
+// value of the lane in the other half of the wave
+__device__ __forceinline__ float other_half(float v)
+{
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    // r[0] = {own low half, low half again}: lanes below 32 need r[1], the others r[0]
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
 }  // namespace qcn_seq
