@@ -66,66 +66,365 @@ struct StepArgs {
     int64_t batch;
     int hq, hk, group, dim;
     int64_t window, sinks, slots;
-    float scale;
+    float c2;                     // scale in base 2
     void *k_cache, *v_cache;
     uint8_t *mask_cache;
     void *out;                    // [batch, hq, dim] contiguous
 };
 
-// One wave per row and query head, slot by slot.  The new token is read from the inputs, never from its slot: the slot is being
-// written by another wave of this launch.
-template <class T>
-__global__ __launch_bounds__(256) void attn_window_step_rows_kernel(StepArgs a)
+// A task is a cache row, a key head, up to 16 of the query heads that share it, and a part of the filled slots.  Its waves take
+// chunks of 32 slots in turn:  S^T (slots x heads) = K Q^T, O^T (features x heads) = V^T P^T with 16 x 16 accumulators, so that a
+// shared key head is read once for its whole group.
+//
+// HBM-bound: every filled slot is read once.  K goes straight into registers as the A operand (a lane reads 16 bytes of a slot,
+// four lanes 64).  V has to be transposed: 16-bit rows pass through LDS that belongs to the wave alone (no barrier) and come
+// back by transposing reads; float32 needs no transposition, a lane reads the features it multiplies.
+// The new token is read from the inputs, never from its slot, which another block of this launch is writing.
+template <class T, int DP> struct Step {
+    static constexpr bool F32 = sizeof(T) == 4;
+    static constexpr int CHUNK = 32, NT = DP / 16;
+    static constexpr int VW = !F32 ? 1 : (DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1));   // float32: features of a lane's V load
+    static constexpr int SB = 16 * VW, NSB = DP / SB;
+    static constexpr int PIECES = DP / 8;                 // 16-bit: 16-byte pieces of a row
+    static constexpr int O_STRIDE = DP + 4;               // floats: a row's pad keeps 16 heads off one bank
+    static constexpr int WAVE_BYTES = 64 * O_STRIDE;      // 32 rows of V, then 16 rows of O
+};
+
+// 8 rows x 32 bytes of a transposing read (half a wave) cover all banks
+template <int DP> __device__ __forceinline__ int v_piece(int row, int piece)
 {
-    const int lane = threadIdx.x & 63;
+    return piece ^ (DP == 128 ? (row & 7) << 1 : DP == 64 ? ((row >> 1) & 3) << 1 : DP == 16 ? 0 : ((row >> 2) & 1) << 1);
+}
+
+template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
+
+struct Part {
+    int heads, head0, kvh;    // query heads of the task
+    int64_t b, p, slot, n;    // cache row, position of the new token and its slot, filled slots
+    int64_t c0, c1;           // slots of this task
+};
+
+template <class T, int DP>
+__device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, int wave, int waves, int lane, char *lds,
+                                             f32x4 (&o)[DP / 16], float &m, float &l)
+{
+    using L = Step<T, DP>;
+    const int n = lane & 15, g = lane >> 4;
+    const int head = t.head0 + (n < t.heads ? n : t.heads - 1);
+    const T *q = reinterpret_cast<const T *>(a.q) + t.b * a.qr.tok + head * a.qr.head;
+    const T *kn = reinterpret_cast<const T *>(a.k) + t.b * a.kr.tok + t.kvh * a.kr.head;
+    const T *vn = reinterpret_cast<const T *>(a.v) + t.b * a.vr.tok + t.kvh * a.vr.head;
+    const int64_t base = (t.b * a.hk + t.kvh) * a.slots * a.dim;
+    const T *kc = reinterpret_cast<const T *>(a.k_cache) + base, *vc = reinterpret_cast<const T *>(a.v_cache) + base;
+    const uint8_t *mask = a.mask_cache ? a.mask_cache + t.b * a.slots : nullptr;
+    const bool new_seen = !mask || !a.key_mask || a.key_mask[t.b] != 0;
+
+    constexpr int NQ = L::F32 ? DP / 16 : (DP + 31) / 32;
+    u32x4 qf[NQ];
+    const auto piece = [&](const T *row, int d) {          // 16 bytes of a row's features, zero past its end
+        u32x4 x = *reinterpret_cast<const u32x4 *>(row + (d < a.dim ? d : 0));
+        if (d >= a.dim) x = u32x4{0, 0, 0, 0};
+        return x;
+    };
+#pragma unroll
+    for (int c = 0; c < NQ; ++c) qf[c] = piece(q, L::F32 ? 16 * c + 4 * g : 32 * c + 8 * g);
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY;
+    l = 0.f;
+
+    for (int64_t j0 = t.c0 + L::CHUNK * wave; j0 < t.c1; j0 += L::CHUNK * waves) {
+        const auto row_of = [&](const T *cache, const T *fresh, int r) {
+            int64_t c = j0 + r;
+            c = c < t.c1 ? c : t.c1 - 1;
+            return c == t.slot ? fresh : cache + c * a.dim;
+        };
+        u32x4 kf[2][NQ];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const T *row = row_of(kc, kn, 16 * u + n);
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) kf[u][c] = piece(row, L::F32 ? 16 * c + 4 * g : 32 * c + 8 * g);
+        }
+        const int64_t cl = j0 + (lane & 31);
+        const bool in = cl < t.c1;
+        const bool ok = in && (cl == t.slot ? new_seen : (!mask || mask[in ? cl : t.c1 - 1] != 0));
+        const unsigned seen = (unsigned)__ballot(ok);
+        constexpr int NV = L::F32 ? 1 : (32 * L::PIECES + 63) / 64;
+        u32x4 vf[NV];
+        if constexpr (!L::F32) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int x = lane + 64 * i, r = x / L::PIECES;
+                vf[i] = piece(row_of(vc, vn, r), x % L::PIECES * 8);
+            }
+        }
+        f32x4 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NQ; ++c) {
+                if constexpr (L::F32) {
+                    const f32x4 kk = __builtin_bit_cast(f32x4, kf[u][c]), qq = __builtin_bit_cast(f32x4, qf[c]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qq[e], s[u], 0, 0, 0);
+                } else {
+                    using V8 = typename Mat<T>::V8;
+                    s[u] = Mat<T>::mul16(__builtin_bit_cast(V8, kf[u][c]), __builtin_bit_cast(V8, qf[c]), s[u]);
+                }
+            }
+        }
+        if constexpr (!L::F32) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int x = lane + 64 * i, r = x / L::PIECES;
+                // 0 times what a masked slot holds must stay 0
+                const u32x4 v = (seen >> r) & 1 ? vf[i] : u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4 *>(lds + (r * L::PIECES + v_piece<DP>(r, x % L::PIECES)) * 16) = v;
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (!((seen >> (16 * u + 4 * g + r)) & 1)) s[u][r] = -INFINITY;
+                top = fmaxf(top, s[u][r]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+        const float scaled = top * a.c2;
+        if (__ballot(scaled > m + 8.f)) {
+            const float mn = scaled > m ? scaled : m;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) o[i] *= alpha;
+            m = mn;
+        }
+        const float at = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.c2, -at));
+                l += s[u][r];
+            }
+        if constexpr (L::F32) {
+            using PV = Pack<float, L::VW>;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int sb = 0; sb < L::NSB; ++sb) {
+                    const int d = sb * L::SB + L::VW * n;
+                    PV v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int c = 16 * u + 4 * g + r;
+                        v[r] = *reinterpret_cast<const PV *>(row_of(vc, vn, c) + (d < a.dim ? d : 0));
+                        if (!((seen >> c) & 1)) v[r] = PV{};
+                    }
+#pragma unroll
+                    for (int e = 0; e < L::VW; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
+                }
+        } else {
+            using V8 = typename Mat<T>::V8;
+            V8 pb;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) pb[i] = from_f32<T>(s[i >> 2][i & 3]);
+            // the wave's own LDS: its writes above are done in order before these reads; only the compiler is to keep them apart
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const int i16 = lane & 15, r = 4 * g + (i16 >> 2);
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
+                const uint2 x = lds_read_transposed(lds + (r * L::PIECES + v_piece<DP>(r, c)) * 16 + byte);
+                const uint2 y = lds_read_transposed(lds + ((r + 16) * L::PIECES + v_piece<DP>(r + 16, c)) * 16 + byte);
+                o[dt] = Mat<T>::mul16(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+}
+
+// features of accumulator element (tile i, register r) of lane group g
+template <class T, int DP> __device__ __forceinline__ int o_feature(int i, int g, int r)
+{
+    using L = Step<T, DP>;
+    return (i / L::VW) * L::SB + L::VW * (4 * g + r) + i % L::VW;
+}
+
+// WAVES per task: 4 share a task's slots and join through LDS; 1: a wave has a task of its own, four tasks to a block.
+template <class T, int DP, int WAVES>
+__global__ __launch_bounds__(256) void attn_window_step_kernel(StepArgs a, int head_tiles, int splits, float *part_o, float *part_ml)
+{
+    using L = Step<T, DP>;
+    __shared__ __attribute__((aligned(16))) char lds[4 * L::WAVE_BYTES];
+    __shared__ float ml[4][16][2];
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = (int64_t)blockIdx.x * 4 + wave;
-    const int64_t b = item / a.hq;
-    const int head = (int)(item % a.hq);
-    if (b >= a.batch) return;
-    const int kvh = head / a.group;
-    const bool has0 = lane < a.dim, has1 = lane + 64 < a.dim;
-    T *o = reinterpret_cast<T *>(a.out) + (b * a.hq + head) * (int64_t)a.dim;
-    const int64_t p = a.lengths[b];
-    if (p < 0) {                                            // a row that is not in use
-        if (has0) o[lane] = from_f32<T>(0.f);
-        if (has1) o[lane + 64] = from_f32<T>(0.f);
-        return;
+    const int64_t task = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int split = (int)(task % splits);
+    const int64_t r0 = task / splits, r1 = r0 / head_tiles;
+    const int ht = (int)(r0 % head_tiles);
+    Part t;
+    t.kvh = (int)(r1 % a.hk);
+    t.b = r1 / a.hk;
+    if (t.b >= a.batch) return;
+    t.heads = a.group - 16 * ht < 16 ? a.group - 16 * ht : 16;
+    t.head0 = t.kvh * a.group + 16 * ht;
+    t.p = a.lengths[t.b];
+    t.n = t.p < 0 ? 0 : (t.p < a.slots ? t.p + 1 : a.slots);
+    t.slot = t.p < 0 ? -1 : cache_slot(t.p, a.sinks, a.window);
+    // equal parts of what is filled, in whole block strides
+    const int64_t stride = L::CHUNK * WAVES, per = ((t.n + splits - 1) / splits + stride - 1) / stride * stride;
+    t.c0 = split * per;
+    t.c1 = t.c0 + per < t.n ? t.c0 + per : t.n;
+
+    f32x4 o[DP / 16];
+    float m, l;
+    attend_slots<T, DP>(a, t, WAVES == 4 ? wave : 0, WAVES, lane, lds + wave * L::WAVE_BYTES, o, m, l);
+
+    T *out = reinterpret_cast<T *>(a.out) + t.b * (int64_t)a.hq * a.dim;
+    if constexpr (WAVES == 1) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        if (n < t.heads) {
+#pragma unroll
+            for (int sb = 0; sb < L::NSB; ++sb)
+#pragma unroll
+                for (int part = 0; part < L::VW; ++part) {
+                    const int d = sb * L::SB + 4 * L::VW * g + 4 * part;
+                    Pack<T, 4> w;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int f = 4 * part + x;
+                        w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW] * inv);
+                    }
+                    if (d < a.dim) *reinterpret_cast<Pack<T, 4> *>(out + (t.head0 + n) * (int64_t)a.dim + d) = w;
+                }
+        }
+    } else {
+        float *mine = reinterpret_cast<float *>(lds + wave * L::WAVE_BYTES);
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mine[n * L::O_STRIDE + o_feature<T, DP>(i, g, r)] = o[i][r];
+        if (g == 0) { ml[wave][n][0] = m; ml[wave][n][1] = l; }
+        __syncthreads();
+        for (int i = threadIdx.x; i < t.heads * a.dim; i += 256) {
+            const int hd = i / a.dim, d = i % a.dim;
+            float top = -INFINITY, sum = 0.f, acc = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = fmaxf(top, ml[w][hd][0]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float mw = ml[w][hd][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
+                sum = fmaf(f, ml[w][hd][1], sum);
+                if (mw != -INFINITY) acc = fmaf(f, reinterpret_cast<float *>(lds + w * L::WAVE_BYTES)[hd * L::O_STRIDE + d], acc);
+            }
+            const int64_t row = t.b * a.hq + t.head0 + hd;
+            if (splits == 1) {
+                out[(t.head0 + hd) * (int64_t)a.dim + d] = from_f32<T>(sum == 0.f ? 0.f : acc / sum);
+            } else {
+                part_o[(row * splits + split) * a.dim + d] = acc;
+                if (d == 0) { part_ml[2 * (row * splits + split)] = top; part_ml[2 * (row * splits + split) + 1] = sum; }
+            }
+        }
     }
-    const T *q = reinterpret_cast<const T *>(a.q) + b * a.qr.tok + head * a.qr.head;
-    const T *kn = reinterpret_cast<const T *>(a.k) + b * a.kr.tok + kvh * a.kr.head;
-    const T *vn = reinterpret_cast<const T *>(a.v) + b * a.vr.tok + kvh * a.vr.head;
-    const int64_t base = (b * a.hk + kvh) * a.slots * a.dim;
-    T *kc = reinterpret_cast<T *>(a.k_cache) + base, *vc = reinterpret_cast<T *>(a.v_cache) + base;
-    const int64_t slot = cache_slot(p, a.sinks, a.window);
-    const int64_t n = p + 1 < a.slots ? p + 1 : a.slots;
-    const bool new_seen = !a.mask_cache || !a.key_mask || a.key_mask[b] != 0;
-    const float q0 = has0 ? to_f32(q[lane]) : 0.f, q1 = has1 ? to_f32(q[lane + 64]) : 0.f;
-    WaveRow r;
-    for (int64_t c = 0; c < n; ++c) {
-        const bool fresh = c == slot;
-        if (fresh ? !new_seen : (a.mask_cache && !a.mask_cache[b * a.slots + c])) continue;
-        const T *kj = fresh ? kn : kc + c * a.dim, *vj = fresh ? vn : vc + c * a.dim;
-        const float dot = (has0 ? q0 * to_f32(kj[lane]) : 0.f) + (has1 ? q1 * to_f32(kj[lane + 64]) : 0.f);
-        r.add(wave_sum(dot) * a.scale, has0 ? to_f32(vj[lane]) : 0.f, has1 ? to_f32(vj[lane + 64]) : 0.f);
-    }
-    if (has0) o[lane] = from_f32<T>(r.result(0));
-    if (has1) o[lane + 64] = from_f32<T>(r.result(1));
-    if (head % a.group == 0) {
-        if (has0) { kc[slot * a.dim + lane] = kn[lane]; vc[slot * a.dim + lane] = vn[lane]; }
-        if (has1) { kc[slot * a.dim + lane + 64] = kn[lane + 64]; vc[slot * a.dim + lane + 64] = vn[lane + 64]; }
-        if (head == 0 && lane == 0 && a.mask_cache) a.mask_cache[b * a.slots + slot] = new_seen;
+    // one wave stores the new token
+    if (split == 0 && ht == 0 && t.p >= 0 && (WAVES == 1 || wave == 0)) {
+        const T *kn = reinterpret_cast<const T *>(a.k) + t.b * a.kr.tok + t.kvh * a.kr.head;
+        const T *vn = reinterpret_cast<const T *>(a.v) + t.b * a.vr.tok + t.kvh * a.vr.head;
+        const int64_t to = ((t.b * a.hk + t.kvh) * a.slots + t.slot) * a.dim;
+        for (int d = lane; d < a.dim; d += 64) {
+            reinterpret_cast<T *>(a.k_cache)[to + d] = kn[d];
+            reinterpret_cast<T *>(a.v_cache)[to + d] = vn[d];
+        }
+        if (t.kvh == 0 && lane == 0 && a.mask_cache) a.mask_cache[t.b * a.slots + t.slot] = !a.key_mask || a.key_mask[t.b] != 0;
     }
 }
 
+// Joins the parts of a row: a wave per (cache row, query head).
 template <class T>
-int launch_step(const StepArgs &a, hipStream_t s)
+__global__ __launch_bounds__(256) void attn_window_step_join_kernel(StepArgs a, int splits, const float *__restrict__ part_o,
+                                                                    const float *__restrict__ part_ml)
 {
-    const int64_t blocks = (a.batch * a.hq + 3) / 4;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.batch * a.hq) return;
+    float top = -INFINITY;
+    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[2 * (row * splits + s)]);
+    float sum = 0.f, acc0 = 0.f, acc1 = 0.f;
+    const bool has0 = lane < a.dim, has1 = lane + 64 < a.dim;
+    for (int s = 0; s < splits; ++s) {
+        const float ms = part_ml[2 * (row * splits + s)];
+        if (ms == -INFINITY) continue;
+        const float f = __builtin_amdgcn_exp2f(ms - top);
+        const float *po = part_o + (row * splits + s) * a.dim;
+        sum = fmaf(f, part_ml[2 * (row * splits + s) + 1], sum);
+        if (has0) acc0 = fmaf(f, po[lane], acc0);
+        if (has1) acc1 = fmaf(f, po[lane + 64], acc1);
+    }
+    T *out = reinterpret_cast<T *>(a.out) + row * a.dim;
+    if (has0) out[lane] = from_f32<T>(sum == 0.f ? 0.f : acc0 / sum);
+    if (has1) out[lane + 64] = from_f32<T>(sum == 0.f ? 0.f : acc1 / sum);
+}
+
+struct Plan {
+    int waves, head_tiles, splits;
+};
+
+// A cache of up to 128 slots is four chunks: a wave of its own is enough, and four of them need not wait for each other.  Above, a
+// block per task; with few tasks the slots are split further until the card has four blocks per CU, down to 128 slots (one
+// chunk per wave).  The plan depends on sizes only, never on the lengths, which are on the device.
+Plan plan_step(int64_t batch, int hk, int group, int64_t slots)
+{
+    Plan p = {slots <= 128 ? 1 : 4, (group + 15) / 16, 1};
+    if (p.waves == 4) {
+        const int64_t tasks = batch * hk * p.head_tiles, want = 4 * (int64_t)qcn_num_cus();
+        int64_t s = tasks > 0 ? (want + tasks - 1) / tasks : 1;
+        if (s > (slots + 127) / 128) s = (slots + 127) / 128;
+        if (s > 64) s = 64;
+        p.splits = (int)(s < 1 ? 1 : s);
+    }
+    return p;
+}
+
+template <class T, int DP>
+int launch_step_dim(const StepArgs &a, const Plan &p, float *ws, hipStream_t s)
+{
+    const int64_t tasks = a.batch * a.hk * p.head_tiles * p.splits, blocks = p.waves == 4 ? tasks : (tasks + 3) / 4;
     if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL(attn_window_step_rows_kernel<T>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    const int64_t rows = a.batch * a.hq * p.splits;
+    float *part_o = ws, *part_ml = ws ? ws + rows * a.dim : nullptr;
+    if (p.waves == 4)
+        hipLaunchKernelGGL((attn_window_step_kernel<T, DP, 4>), dim3((unsigned)blocks), dim3(256), 0, s, a, p.head_tiles, p.splits, part_o, part_ml);
+    else
+        hipLaunchKernelGGL((attn_window_step_kernel<T, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a, p.head_tiles, p.splits, part_o, part_ml);
     QCN_CHECK_LAUNCH();
+    if (p.splits > 1) {
+        hipLaunchKernelGGL(attn_window_step_join_kernel<T>, dim3((unsigned)((a.batch * a.hq + 3) / 4)), dim3(256), 0, s, a, p.splits, part_o, part_ml);
+        QCN_CHECK_LAUNCH();
+    }
     return QCN_OK;
+}
+
+template <class T>
+int launch_step(const StepArgs &a, const Plan &p, float *ws, hipStream_t s)
+{
+    if (a.dim <= 16) return launch_step_dim<T, 16>(a, p, ws, s);
+    if (a.dim <= 32) return launch_step_dim<T, 32>(a, p, ws, s);
+    if (a.dim <= 64) return launch_step_dim<T, 64>(a, p, ws, s);
+    if (a.dim <= 96) return launch_step_dim<T, 96>(a, p, ws, s);
+    return launch_step_dim<T, 128>(a, p, ws, s);
 }
 
 bool cache_shape_ok(int64_t window, int64_t sinks) { return window >= 1 && sinks >= 0 && window < ((int64_t)1 << 40) && sinks < ((int64_t)1 << 40); }
@@ -160,8 +459,9 @@ extern "C" int qcn_window_cache_append(const void *k, int64_t k_tok_stride, int6
 
 extern "C" size_t qcn_attn_window_step_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int dim, int64_t window, int64_t sinks)
 {
-    (void)batch; (void)n_q_heads; (void)n_kv_heads; (void)dim; (void)window; (void)sinks;
-    return 0;
+    if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || dim < 1 || !cache_shape_ok(window, sinks)) return 0;
+    const Plan p = plan_step(batch, n_kv_heads, n_q_heads / n_kv_heads, window + sinks);
+    return p.splits > 1 ? (size_t)batch * n_q_heads * p.splits * (dim + 2) * sizeof(float) : 0;
 }
 
 extern "C" int qcn_attn_window_step(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k, int64_t k_row_stride,
@@ -182,15 +482,17 @@ extern "C" int qcn_attn_window_step(const void *q, int64_t q_row_stride, int64_t
         !rows_aligned(v_cache, 0, 0, dtype) || !rows_aligned(out, 0, 0, dtype))
         return QCN_ERR_INVALID_ARGUMENT;
     if (workspace_bytes < qcn_attn_window_step_workspace_bytes(batch, n_q_heads, n_kv_heads, dim, window, sinks) ||
-        (workspace_bytes && !workspace))
+        (workspace_bytes && (!workspace || ((uintptr_t)workspace & 3))))
         return QCN_ERR_WORKSPACE_TOO_SMALL;
     const StepArgs a = {q, k, v, {q_row_stride, q_head_stride}, {k_row_stride, k_head_stride}, {v_row_stride, v_head_stride}, lengths,
-                        key_mask, batch, n_q_heads, n_kv_heads, n_q_heads / n_kv_heads, dim, window, sinks, window + sinks, scale,
-                        k_cache, v_cache, mask_cache, out};
+                        key_mask, batch, n_q_heads, n_kv_heads, n_q_heads / n_kv_heads, dim, window, sinks, window + sinks,
+                        // an unseen slot's score is -inf and has to stay so: scale 0 becomes one that no score outgrows
+                        fmaxf(scale * kLog2e, 1e-37f), k_cache, v_cache, mask_cache, out};
+    const Plan plan = plan_step(batch, n_kv_heads, n_q_heads / n_kv_heads, window + sinks);
     hipStream_t s = qcn_stream(stream);
     switch (dtype) {
-    case QCN_DTYPE_F32: return launch_step<float>(a, s);
-    case QCN_DTYPE_F16: return launch_step<_Float16>(a, s);
-    default: return launch_step<__bf16>(a, s);
+    case QCN_DTYPE_F32: return launch_step<float>(a, plan, reinterpret_cast<float *>(workspace), s);
+    case QCN_DTYPE_F16: return launch_step<_Float16>(a, plan, reinterpret_cast<float *>(workspace), s);
+    default: return launch_step<__bf16>(a, plan, reinterpret_cast<float *>(workspace), s);
     }
 }
