@@ -506,46 +506,96 @@ int qcn_nms_select_f32(const float *traj, const float *conf, const float *gt, in
 #define QCN_POS_I32 1
 #define QCN_POS_I64 2
 
+/* The calls take their arguments as a struct of 8-byte fields (a serving loop issues one per layer and token, and filling a
+ * struct costs a caller a fraction of passing two dozen arguments one by one).  The struct is read before the call returns.
+ * Row tensors: data pointer, then {token stride, head stride} in elements. */
+
 /* Feature pair i of every head of q and k is turned by pos[token, axis(i)] * freqs[i] (inverse != 0: by the negative).
- *   pos [n_tokens, n_axes] of pos_type; freqs [pairs] f32; sections_host [n_axes] (HOST): pairs of each axis, in order;
- *   pairs = sum(sections_host), 2 * pairs <= dim; pair i is features (i, i + pairs), interleaved != 0: (2 i, 2 i + 1);
+ *   pos [n_tokens, n_axes] of pos_type; freqs [pairs] f32; sections[0 .. n_axes - 1]: pairs of each axis, in order;
+ *   pairs = sum of the sections, 2 * pairs <= dim; pair i is features (i, i + pairs), interleaved != 0: (2 i, 2 i + 1);
  *   features behind 2 * pairs are copied.  k may be NULL (n_k_heads = 0).  n_axes <= 8. */
-int qcn_rotary_embed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int n_q_heads, const void *k,
-                     int64_t k_tok_stride, int64_t k_head_stride, int n_k_heads, int64_t n_tokens, int dim, int dtype,
-                     const void *pos, int pos_type, int n_axes, const float *freqs, const int32_t *sections_host,
-                     int interleaved, int inverse, void *q_out, void *k_out, void *stream);
+typedef struct {
+    const void *q;
+    int64_t q_strides[2];
+    int64_t n_q_heads;
+    const void *k;
+    int64_t k_strides[2];
+    int64_t n_k_heads;
+    int64_t n_tokens, dim, dtype;
+    const void *pos;
+    int64_t pos_type, n_axes;
+    int64_t sections[8];
+    const float *freqs;
+    int64_t interleaved, inverse;
+    void *q_out, *k_out;
+} qcn_rotary_embed_args;
+int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream);
 
 /* Query i of a sequence of Lq queries and Lk keys stands at position p = i + Lk - Lq and sees key j when 0 <= j <= p and
  * (j > p - window or j < sinks) and key_mask[j] (uint8 [n_k_tokens], NULL: all).  out [n_q_tokens, n_q_heads, dim] =
  * softmax(scale q.k) v over what it sees; rows that see nothing and rows behind cu_q[n_seq] are 0.  Masked keys and values may
  * hold anything, NaN and infinities among it.  Query head h reads key head h / (n_q_heads / n_kv_heads).
  * scale: finite, >= 0. */
-int qcn_attn_window(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k, int64_t k_tok_stride,
-                    int64_t k_head_stride, const void *v, int64_t v_tok_stride, int64_t v_head_stride, const int64_t *cu_q,
-                    const int64_t *cu_k, const uint8_t *key_mask, int64_t n_seq, int64_t n_q_tokens, int64_t n_k_tokens,
-                    int n_q_heads, int n_kv_heads, int dim, int dtype, int64_t window, int64_t sinks, float scale, void *out,
-                    void *stream);
+typedef struct {
+    const void *q;
+    int64_t q_strides[2];
+    const void *k;
+    int64_t k_strides[2];
+    const void *v;
+    int64_t v_strides[2];
+    const int64_t *cu_q, *cu_k;
+    const uint8_t *key_mask;
+    int64_t n_seq, n_q_tokens, n_k_tokens, n_q_heads, n_kv_heads, dim, dtype;
+    int64_t window, sinks;
+    double scale;
+    void *out;
+} qcn_attn_window_args;
+int qcn_attn_window(const qcn_attn_window_args *args, void *stream);
 
 /* The cache of that attention: [n_seq, n_kv_heads, sinks + window, dim] contiguous; position p in slot p (p < sinks) or
  * sinks + (p - sinks) % window; mask_cache uint8 [n_seq, sinks + window] (NULL: every token is visible).
  * append: sequence b brings cu[b + 1] - cu[b] tokens behind the lengths[b] (int64) it has; lengths is not changed (several
  * layers share it).  Tokens that fall out of the window within the call are not written; sequences with lengths[b] < 0 and
  * rows behind cu[n_seq] are left alone.  key_mask uint8 [n_tokens] (NULL: 1) goes into mask_cache. */
-int qcn_window_cache_append(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v, int64_t v_tok_stride,
-                            int64_t v_head_stride, const int64_t *cu, const int64_t *lengths, const uint8_t *key_mask,
-                            int64_t n_seq, int64_t n_tokens, int n_kv_heads, int dim, int dtype, int64_t window,
-                            int64_t sinks, void *k_cache, void *v_cache, uint8_t *mask_cache, void *stream);
+typedef struct {
+    const void *k;
+    int64_t k_strides[2];
+    const void *v;
+    int64_t v_strides[2];
+    const int64_t *cu, *lengths;
+    const uint8_t *key_mask;
+    int64_t n_seq, n_tokens, n_kv_heads, dim, dtype;
+    int64_t window, sinks;
+    void *k_cache, *v_cache;
+    uint8_t *mask_cache;
+} qcn_window_cache_append_args;
+int qcn_window_cache_append(const qcn_window_cache_append_args *args, void *stream);
 
 /* One new token per sequence: k / v [batch, n_kv_heads, dim] go into the cache at position lengths[b], q [batch, n_q_heads,
  * dim] attends to what that position sees.  lengths[b] < 0: the row is not in use, its output is 0 and its cache untouched.
- * lengths is not changed.  key_mask uint8 [batch]: whether the new token is visible. */
-size_t qcn_attn_window_step_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int dim, int64_t window,
+ * lengths is not changed.  key_mask uint8 [batch]: whether the new token is visible.  The workspace's contents do not outlive
+ * the call's work on its stream. */
+typedef struct {
+    const void *q;
+    int64_t q_strides[2];
+    const void *k;
+    int64_t k_strides[2];
+    const void *v;
+    int64_t v_strides[2];
+    const int64_t *lengths;
+    const uint8_t *key_mask;
+    int64_t batch, n_q_heads, n_kv_heads, dim, dtype;
+    int64_t window, sinks;
+    double scale;
+    void *k_cache, *v_cache;
+    uint8_t *mask_cache;
+    void *out;
+    void *workspace;
+    int64_t workspace_bytes;
+} qcn_attn_window_step_args;
+size_t qcn_attn_window_step_workspace_bytes(int64_t batch, int64_t n_q_heads, int64_t n_kv_heads, int64_t dim, int64_t window,
                                             int64_t sinks);
-int qcn_attn_window_step(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k, int64_t k_row_stride,
-                         int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride,
-                         const int64_t *lengths, const uint8_t *key_mask, int64_t batch, int n_q_heads, int n_kv_heads,
-                         int dim, int dtype, int64_t window, int64_t sinks, float scale, void *k_cache, void *v_cache,
-                         uint8_t *mask_cache, void *out, void *workspace, size_t workspace_bytes, void *stream);
+int qcn_attn_window_step(const qcn_attn_window_step_args *args, void *stream);
 
 #ifdef __cplusplus
 }

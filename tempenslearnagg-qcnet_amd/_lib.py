@@ -123,17 +123,12 @@ def _declare(lib) -> None:
     lib.qcn_coalesce_fill.argtypes = [P, P, c_int64, c_int64, P, P, P, P]
     lib.qcn_nms_select_f32.restype = c_int
     lib.qcn_nms_select_f32.argtypes = [P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, c_float, P, P, P]
-    I, L = c_int, c_int64
-    lib.qcn_rotary_embed.restype = I
-    lib.qcn_rotary_embed.argtypes = [P, L, L, I, P, L, L, I, L, I, I, P, I, I, P, POINTER(ctypes.c_int32), I, I, P, P, P]
-    lib.qcn_attn_window.restype = I
-    lib.qcn_attn_window.argtypes = [P, L, L, P, L, L, P, L, L, P, P, P, L, L, L, I, I, I, I, L, L, c_float, P, P]
-    lib.qcn_window_cache_append.restype = I
-    lib.qcn_window_cache_append.argtypes = [P, L, L, P, L, L, P, P, P, L, L, I, I, I, L, L, P, P, P, P]
+    # argument structs of 8-byte fields, packed by the caller (sequence_ops.py); `bytes` pass as the pointer
+    for name in ('qcn_rotary_embed', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step'):
+        getattr(lib, name).restype = c_int
+        getattr(lib, name).argtypes = [ctypes.c_char_p, P]
     lib.qcn_attn_window_step_workspace_bytes.restype = c_size_t
-    lib.qcn_attn_window_step_workspace_bytes.argtypes = [L, I, I, I, L, L]
-    lib.qcn_attn_window_step.restype = I
-    lib.qcn_attn_window_step.argtypes = [P, L, L, P, L, L, P, L, L, P, P, L, I, I, I, I, L, L, c_float, P, P, P, P, P, c_size_t, P]
+    lib.qcn_attn_window_step_workspace_bytes.argtypes = [c_int64] * 6
 
 
 EXPORTED_SYMBOLS = (

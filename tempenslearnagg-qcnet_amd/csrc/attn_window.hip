@@ -576,30 +576,31 @@ int launch(const Args &a, hipStream_t s)
 
 }  // namespace
 
-extern "C" int qcn_attn_window(const void *q, int64_t q_tok_stride, int64_t q_head_stride, const void *k, int64_t k_tok_stride,
-                               int64_t k_head_stride, const void *v, int64_t v_tok_stride, int64_t v_head_stride,
-                               const int64_t *cu_q, const int64_t *cu_k, const uint8_t *key_mask, int64_t n_seq, int64_t n_q_tokens,
-                               int64_t n_k_tokens, int n_q_heads, int n_kv_heads, int dim, int dtype, int64_t window, int64_t sinks,
-                               float scale, void *out, void *stream)
+extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
 {
-    if (n_seq < 0 || n_q_tokens < 0 || n_k_tokens < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || window < 1 ||
-        sinks < 0 || !(scale >= 0.f) || scale > 3.0e38f || !dtype_known(dtype))
+    if (!args) return QCN_ERR_INVALID_ARGUMENT;
+    const qcn_attn_window_args &x = *args;
+    if (x.n_seq < 0 || x.n_q_tokens < 0 || x.n_k_tokens < 0 || x.n_q_heads < 1 || x.n_kv_heads < 1 || x.n_q_heads % x.n_kv_heads ||
+        x.window < 1 || x.sinks < 0 || !(x.scale >= 0.) || x.scale > 3.0e38 || !dtype_known(x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
-    if (dim < 8 || dim > kMaxDim || dim % 8) return QCN_ERR_UNSUPPORTED;
-    if (n_q_tokens == 0) return QCN_OK;
-    if (!q || !out || !cu_q || !cu_k || (n_k_tokens && (!k || !v))) return QCN_ERR_INVALID_ARGUMENT;
-    if (n_q_tokens >= ((int64_t)1 << 31) || n_k_tokens >= ((int64_t)1 << 31) || n_seq >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    if (!rows_aligned(q, q_tok_stride, q_head_stride, dtype) || !rows_aligned(out, 0, 0, dtype) ||
-        (n_k_tokens && (!rows_aligned(k, k_tok_stride, k_head_stride, dtype) || !rows_aligned(v, v_tok_stride, v_head_stride, dtype))))
+    const int64_t most = ((int64_t)1 << 31) - 1;
+    if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.n_q_tokens > most || x.n_k_tokens > most || x.n_seq > most)
+        return QCN_ERR_UNSUPPORTED;
+    if (x.n_q_tokens == 0) return QCN_OK;
+    if (!x.q || !x.out || !x.cu_q || !x.cu_k || (x.n_k_tokens && (!x.k || !x.v))) return QCN_ERR_INVALID_ARGUMENT;
+    if (!rows_aligned(x.q, x.q_strides[0], x.q_strides[1], x.dtype) || !rows_aligned(x.out, 0, 0, x.dtype) ||
+        (x.n_k_tokens && (!rows_aligned(x.k, x.k_strides[0], x.k_strides[1], x.dtype) ||
+                          !rows_aligned(x.v, x.v_strides[0], x.v_strides[1], x.dtype))))
         return QCN_ERR_INVALID_ARGUMENT;
-    const int64_t reach = ((int64_t)1 << 31) - 1;   // positions are below: larger windows and sinks mean the same
-    const Args a = {q, k, v, {q_tok_stride, q_head_stride}, {k_tok_stride, k_head_stride}, {v_tok_stride, v_head_stride}, cu_q, cu_k,
-                    key_mask, n_seq, n_q_tokens, n_k_tokens, n_q_heads, n_kv_heads, n_q_heads / n_kv_heads, dim,
-                    window < reach ? window : reach, sinks < reach ? sinks : reach, scale,
+    // positions are below 2^31: larger windows and sinks mean the same
+    const int64_t window = x.window < most ? x.window : most, sinks = x.sinks < most ? x.sinks : most;
+    const Args a = {x.q, x.k, x.v, {x.q_strides[0], x.q_strides[1]}, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]},
+                    x.cu_q, x.cu_k, x.key_mask, x.n_seq, x.n_q_tokens, x.n_k_tokens, (int)x.n_q_heads, (int)x.n_kv_heads,
+                    (int)(x.n_q_heads / x.n_kv_heads), (int)x.dim, window, sinks, (float)x.scale,
                     // an unseen key's score is -inf and has to stay so: scale 0 becomes one that no score outgrows
-                    fmaxf(scale * kLog2e, 1e-37f), out};
+                    fmaxf((float)x.scale * kLog2e, 1e-37f), x.out};
     hipStream_t s = qcn_stream(stream);
-    switch (dtype) {
+    switch (x.dtype) {
     case QCN_DTYPE_F32: return launch<float>(a, s);
     case QCN_DTYPE_F16: return launch<_Float16>(a, s);
     default: return launch<__bf16>(a, s);

@@ -431,25 +431,26 @@ bool cache_shape_ok(int64_t window, int64_t sinks) { return window >= 1 && sinks
 
 }  // namespace
 
-extern "C" int qcn_window_cache_append(const void *k, int64_t k_tok_stride, int64_t k_head_stride, const void *v, int64_t v_tok_stride,
-                                       int64_t v_head_stride, const int64_t *cu, const int64_t *lengths, const uint8_t *key_mask,
-                                       int64_t n_seq, int64_t n_tokens, int n_kv_heads, int dim, int dtype, int64_t window,
-                                       int64_t sinks, void *k_cache, void *v_cache, uint8_t *mask_cache, void *stream)
+extern "C" int qcn_window_cache_append(const qcn_window_cache_append_args *args, void *stream)
 {
-    if (n_seq < 0 || n_tokens < 0 || n_kv_heads < 1 || !cache_shape_ok(window, sinks) || !dtype_known(dtype) || (key_mask && !mask_cache))
+    if (!args) return QCN_ERR_INVALID_ARGUMENT;
+    const qcn_window_cache_append_args &x = *args;
+    if (x.n_seq < 0 || x.n_tokens < 0 || x.n_kv_heads < 1 || !cache_shape_ok(x.window, x.sinks) || !dtype_known(x.dtype) ||
+        (x.key_mask && !x.mask_cache))
         return QCN_ERR_INVALID_ARGUMENT;
-    if (dim < 8 || dim > kMaxDim || dim % 8 || n_kv_heads > 65535) return QCN_ERR_UNSUPPORTED;
-    if (n_tokens == 0 || n_seq == 0) return QCN_OK;
-    if (!k || !v || !cu || !lengths || !k_cache || !v_cache) return QCN_ERR_INVALID_ARGUMENT;
-    if (!rows_aligned(k, k_tok_stride, k_head_stride, dtype) || !rows_aligned(v, v_tok_stride, v_head_stride, dtype) ||
-        !rows_aligned(k_cache, 0, 0, dtype) || !rows_aligned(v_cache, 0, 0, dtype))
+    if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_kv_heads > kMaxHeads) return QCN_ERR_UNSUPPORTED;
+    if (x.n_tokens == 0 || x.n_seq == 0) return QCN_OK;
+    if (!x.k || !x.v || !x.cu || !x.lengths || !x.k_cache || !x.v_cache) return QCN_ERR_INVALID_ARGUMENT;
+    if (!rows_aligned(x.k, x.k_strides[0], x.k_strides[1], x.dtype) || !rows_aligned(x.v, x.v_strides[0], x.v_strides[1], x.dtype) ||
+        !rows_aligned(x.k_cache, 0, 0, x.dtype) || !rows_aligned(x.v_cache, 0, 0, x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
-    const int64_t blocks = (n_tokens >> kAppendShift) + n_seq + 1;
-    if (n_tokens >= ((int64_t)1 << 40) || blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    const AppendArgs a = {k, v, {k_tok_stride, k_head_stride}, {v_tok_stride, v_head_stride}, cu, lengths, key_mask, n_seq, n_tokens,
-                          n_kv_heads, dim, dim * (int)dtype_bytes(dtype) / 16, window, sinks, window + sinks, k_cache, v_cache, mask_cache};
+    const int64_t blocks = (x.n_tokens >> kAppendShift) + x.n_seq + 1;
+    if (x.n_tokens >= ((int64_t)1 << 40) || x.n_seq >= ((int64_t)1 << 31) || blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    const AppendArgs a = {x.k, x.v, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]}, x.cu, x.lengths, x.key_mask,
+                          x.n_seq, x.n_tokens, (int)x.n_kv_heads, (int)x.dim, (int)x.dim * (int)dtype_bytes(x.dtype) / 16, x.window,
+                          x.sinks, x.window + x.sinks, x.k_cache, x.v_cache, x.mask_cache};
     hipStream_t s = qcn_stream(stream);
-    if (dtype == QCN_DTYPE_F32)
+    if (x.dtype == QCN_DTYPE_F32)
         hipLaunchKernelGGL(window_cache_append_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, s, a);
     else   // moved as they are: one form for both 16-bit types
         hipLaunchKernelGGL(window_cache_append_kernel<_Float16>, dim3((unsigned)blocks), dim3(256), 0, s, a);
@@ -457,42 +458,44 @@ extern "C" int qcn_window_cache_append(const void *k, int64_t k_tok_stride, int6
     return QCN_OK;
 }
 
-extern "C" size_t qcn_attn_window_step_workspace_bytes(int64_t batch, int n_q_heads, int n_kv_heads, int dim, int64_t window, int64_t sinks)
+extern "C" size_t qcn_attn_window_step_workspace_bytes(int64_t batch, int64_t n_q_heads, int64_t n_kv_heads, int64_t dim, int64_t window,
+                                                       int64_t sinks)
 {
-    if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || dim < 1 || !cache_shape_ok(window, sinks)) return 0;
-    const Plan p = plan_step(batch, n_kv_heads, n_q_heads / n_kv_heads, window + sinks);
+    if (batch < 1 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || n_q_heads > kMaxHeads || dim < 1 ||
+        !cache_shape_ok(window, sinks))
+        return 0;
+    const Plan p = plan_step(batch, (int)n_kv_heads, (int)(n_q_heads / n_kv_heads), window + sinks);
     return p.splits > 1 ? (size_t)batch * n_q_heads * p.splits * (dim + 2) * sizeof(float) : 0;
 }
 
-extern "C" int qcn_attn_window_step(const void *q, int64_t q_row_stride, int64_t q_head_stride, const void *k, int64_t k_row_stride,
-                                    int64_t k_head_stride, const void *v, int64_t v_row_stride, int64_t v_head_stride,
-                                    const int64_t *lengths, const uint8_t *key_mask, int64_t batch, int n_q_heads, int n_kv_heads,
-                                    int dim, int dtype, int64_t window, int64_t sinks, float scale, void *k_cache, void *v_cache,
-                                    uint8_t *mask_cache, void *out, void *workspace, size_t workspace_bytes, void *stream)
+extern "C" int qcn_attn_window_step(const qcn_attn_window_step_args *args, void *stream)
 {
-    if (batch < 0 || n_q_heads < 1 || n_kv_heads < 1 || n_q_heads % n_kv_heads || !cache_shape_ok(window, sinks) || !(scale >= 0.f) ||
-        scale > 3.0e38f || !dtype_known(dtype) || (key_mask && !mask_cache))
+    if (!args) return QCN_ERR_INVALID_ARGUMENT;
+    const qcn_attn_window_step_args &x = *args;
+    if (x.batch < 0 || x.n_q_heads < 1 || x.n_kv_heads < 1 || x.n_q_heads % x.n_kv_heads || !cache_shape_ok(x.window, x.sinks) ||
+        !(x.scale >= 0.) || x.scale > 3.0e38 || !dtype_known(x.dtype) || (x.key_mask && !x.mask_cache))
         return QCN_ERR_INVALID_ARGUMENT;
-    if (dim < 8 || dim > kMaxDim || dim % 8) return QCN_ERR_UNSUPPORTED;
-    if (batch == 0) return QCN_OK;
-    if (!q || !k || !v || !lengths || !k_cache || !v_cache || !out) return QCN_ERR_INVALID_ARGUMENT;
-    if (batch >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    if (!rows_aligned(q, q_row_stride, q_head_stride, dtype) || !rows_aligned(k, k_row_stride, k_head_stride, dtype) ||
-        !rows_aligned(v, v_row_stride, v_head_stride, dtype) || !rows_aligned(k_cache, 0, 0, dtype) ||
-        !rows_aligned(v_cache, 0, 0, dtype) || !rows_aligned(out, 0, 0, dtype))
+    if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.batch >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (x.batch == 0) return QCN_OK;
+    if (!x.q || !x.k || !x.v || !x.lengths || !x.k_cache || !x.v_cache || !x.out) return QCN_ERR_INVALID_ARGUMENT;
+    if (!rows_aligned(x.q, x.q_strides[0], x.q_strides[1], x.dtype) || !rows_aligned(x.k, x.k_strides[0], x.k_strides[1], x.dtype) ||
+        !rows_aligned(x.v, x.v_strides[0], x.v_strides[1], x.dtype) || !rows_aligned(x.k_cache, 0, 0, x.dtype) ||
+        !rows_aligned(x.v_cache, 0, 0, x.dtype) || !rows_aligned(x.out, 0, 0, x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
-    if (workspace_bytes < qcn_attn_window_step_workspace_bytes(batch, n_q_heads, n_kv_heads, dim, window, sinks) ||
-        (workspace_bytes && (!workspace || ((uintptr_t)workspace & 3))))
-        return QCN_ERR_WORKSPACE_TOO_SMALL;
-    const StepArgs a = {q, k, v, {q_row_stride, q_head_stride}, {k_row_stride, k_head_stride}, {v_row_stride, v_head_stride}, lengths,
-                        key_mask, batch, n_q_heads, n_kv_heads, n_q_heads / n_kv_heads, dim, window, sinks, window + sinks,
+    const int group = (int)(x.n_q_heads / x.n_kv_heads);
+    const Plan plan = plan_step(x.batch, (int)x.n_kv_heads, group, x.window + x.sinks);
+    const size_t need = qcn_attn_window_step_workspace_bytes(x.batch, x.n_q_heads, x.n_kv_heads, x.dim, x.window, x.sinks);
+    if (need && (x.workspace_bytes < (int64_t)need || !x.workspace || ((uintptr_t)x.workspace & 3))) return QCN_ERR_WORKSPACE_TOO_SMALL;
+    const StepArgs a = {x.q, x.k, x.v, {x.q_strides[0], x.q_strides[1]}, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]},
+                        x.lengths, x.key_mask, x.batch, (int)x.n_q_heads, (int)x.n_kv_heads, group, (int)x.dim, x.window, x.sinks,
+                        x.window + x.sinks,
                         // an unseen slot's score is -inf and has to stay so: scale 0 becomes one that no score outgrows
-                        fmaxf(scale * kLog2e, 1e-37f), k_cache, v_cache, mask_cache, out};
-    const Plan plan = plan_step(batch, n_kv_heads, n_q_heads / n_kv_heads, window + sinks);
+                        fmaxf((float)x.scale * kLog2e, 1e-37f), x.k_cache, x.v_cache, x.mask_cache, x.out};
+    float *ws = need ? reinterpret_cast<float *>(x.workspace) : nullptr;
     hipStream_t s = qcn_stream(stream);
-    switch (dtype) {
-    case QCN_DTYPE_F32: return launch_step<float>(a, plan, reinterpret_cast<float *>(workspace), s);
-    case QCN_DTYPE_F16: return launch_step<_Float16>(a, plan, reinterpret_cast<float *>(workspace), s);
-    default: return launch_step<__bf16>(a, plan, reinterpret_cast<float *>(workspace), s);
+    switch (x.dtype) {
+    case QCN_DTYPE_F32: return launch_step<float>(a, plan, ws, s);
+    case QCN_DTYPE_F16: return launch_step<_Float16>(a, plan, ws, s);
+    default: return launch_step<__bf16>(a, plan, ws, s);
     }
 }

@@ -138,32 +138,33 @@ int launch_pos(const Args &a, int pos_type, int ve, bool interleaved, dim3 grid,
 
 }  // namespace
 
-extern "C" int qcn_rotary_embed(const void *q, int64_t q_tok_stride, int64_t q_head_stride, int n_q_heads, const void *k,
-                                int64_t k_tok_stride, int64_t k_head_stride, int n_k_heads, int64_t n_tokens, int dim, int dtype,
-                                const void *pos, int pos_type, int n_axes, const float *freqs, const int32_t *sections_host,
-                                int interleaved, int inverse, void *q_out, void *k_out, void *stream)
+extern "C" int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream)
 {
-    if (n_tokens < 0 || n_q_heads < 0 || n_k_heads < 0 || dim < 2 || (dim & 1) || n_axes < 1 || n_axes > kMaxAxes || !sections_host ||
-        !dtype_known(dtype) || pos_type < QCN_POS_F32 || pos_type > QCN_POS_I64)
+    if (!args) return QCN_ERR_INVALID_ARGUMENT;
+    const qcn_rotary_embed_args &x = *args;
+    if (x.n_tokens < 0 || x.n_q_heads < 0 || x.n_k_heads < 0 || x.dim < 2 || (x.dim & 1) || x.n_axes < 1 || x.n_axes > kMaxAxes ||
+        !dtype_known(x.dtype) || x.pos_type < QCN_POS_F32 || x.pos_type > QCN_POS_I64)
         return QCN_ERR_INVALID_ARGUMENT;
+    if (x.dim > 256 || x.n_q_heads > 32767 || x.n_k_heads > 32767 || x.n_tokens >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
     Args a = {};
-    for (int i = 0; i < n_axes; ++i) {
-        if (sections_host[i] < 0 || sections_host[i] > dim / 2) return QCN_ERR_INVALID_ARGUMENT;
-        a.axes.first[i + 1] = a.axes.first[i] + sections_host[i];
+    for (int i = 0; i < x.n_axes; ++i) {
+        if (x.sections[i] < 0 || x.sections[i] > x.dim / 2) return QCN_ERR_INVALID_ARGUMENT;
+        a.axes.first[i + 1] = a.axes.first[i] + (int)x.sections[i];
     }
-    a.pairs = a.axes.first[n_axes];
-    if (a.pairs < 1 || 2 * a.pairs > dim) return QCN_ERR_INVALID_ARGUMENT;
-    const int heads = n_q_heads + n_k_heads;
-    if (n_tokens == 0 || heads == 0) return QCN_OK;
-    if ((k == nullptr) != (n_k_heads == 0) || !pos || !freqs || (n_q_heads && (!q || !q_out)) || (n_k_heads && (!k || !k_out))) return QCN_ERR_INVALID_ARGUMENT;
-    if (dim > 256 || heads > 65535 || n_tokens >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    a.in[0] = q; a.in[1] = k; a.out[0] = q_out; a.out[1] = k_out;
-    a.rows[0] = {q_tok_stride, q_head_stride}; a.rows[1] = {k_tok_stride, k_head_stride};
-    a.heads[0] = n_q_heads; a.heads[1] = n_k_heads;
-    a.n_tokens = n_tokens; a.dim = dim; a.n_axes = n_axes; a.pos = pos; a.freqs = freqs; a.inverse = inverse != 0;
+    a.pairs = a.axes.first[x.n_axes];
+    if (a.pairs < 1 || 2 * a.pairs > x.dim) return QCN_ERR_INVALID_ARGUMENT;
+    const int heads = (int)(x.n_q_heads + x.n_k_heads), dim = (int)x.dim;
+    if (x.n_tokens == 0 || heads == 0) return QCN_OK;
+    if ((x.k == nullptr) != (x.n_k_heads == 0) || !x.pos || !x.freqs || (x.n_q_heads && (!x.q || !x.q_out)) || (x.n_k_heads && !x.k_out))
+        return QCN_ERR_INVALID_ARGUMENT;
+    a.in[0] = x.q; a.in[1] = x.k; a.out[0] = x.q_out; a.out[1] = x.k_out;
+    a.rows[0] = {x.q_strides[0], x.q_strides[1]}; a.rows[1] = {x.k_strides[0], x.k_strides[1]};
+    a.heads[0] = (int)x.n_q_heads; a.heads[1] = (int)x.n_k_heads;
+    a.n_tokens = x.n_tokens; a.dim = dim; a.n_axes = (int)x.n_axes; a.pos = x.pos; a.freqs = x.freqs; a.inverse = x.inverse != 0;
+    const bool interleaved = x.interleaved != 0;
 
     // widest access that every row, the pairs' second half and the passed-through features are aligned to
-    const int es = (int)dtype_bytes(dtype);
+    const int es = (int)dtype_bytes(x.dtype);
     int ve = 16 / es;
     const auto fits = [&](int n) {
         if (dim % n || (!interleaved && a.pairs % n)) return false;
@@ -175,23 +176,23 @@ extern "C" int qcn_rotary_embed(const void *q, int64_t q_tok_stride, int64_t q_h
         return true;
     };
     while (ve > 1 && !fits(ve)) ve /= 2;
-    if (interleaved && ve < 2) return QCN_ERR_INVALID_ARGUMENT;   // a pair straddles its alignment
+    if ((interleaved && ve < 2) || !fits(ve)) return QCN_ERR_INVALID_ARGUMENT;   // a pair, or an element, straddles its alignment
 
     // 32 KiB of rows per block while that leaves blocks for the card; few tokens: the heads are spread over blocks as well
     const int64_t row_bytes = (int64_t)heads * dim * es;
     int tpb = (int)((32 * 1024 + row_bytes - 1) / row_bytes);
     if (tpb > kTable / a.pairs) tpb = kTable / a.pairs;
     const int64_t cus = qcn_num_cus();
-    while (tpb > 1 && (n_tokens + tpb - 1) / tpb < 4 * cus) tpb /= 2;
+    while (tpb > 1 && (x.n_tokens + tpb - 1) / tpb < 4 * cus) tpb /= 2;
     int hpb = heads;
-    while (hpb > 4 && (n_tokens + tpb - 1) / tpb * ((heads + hpb - 1) / hpb) < 2 * cus) hpb = (hpb + 1) / 2;
+    while (hpb > 4 && (x.n_tokens + tpb - 1) / tpb * ((heads + hpb - 1) / hpb) < 2 * cus) hpb = (hpb + 1) / 2;
     a.tokens_per_block = tpb;
     a.heads_per_block = hpb;
-    const dim3 grid((unsigned)((n_tokens + tpb - 1) / tpb), (unsigned)((heads + hpb - 1) / hpb));
+    const dim3 grid((unsigned)((x.n_tokens + tpb - 1) / tpb), (unsigned)((heads + hpb - 1) / hpb));
     hipStream_t s = qcn_stream(stream);
-    switch (dtype) {
-    case QCN_DTYPE_F32: return launch_pos<float>(a, pos_type, ve, interleaved, grid, s);
-    case QCN_DTYPE_F16: return launch_pos<_Float16>(a, pos_type, ve, interleaved, grid, s);
-    default: return launch_pos<__bf16>(a, pos_type, ve, interleaved, grid, s);
+    switch (x.dtype) {
+    case QCN_DTYPE_F32: return launch_pos<float>(a, (int)x.pos_type, ve, interleaved, grid, s);
+    case QCN_DTYPE_F16: return launch_pos<_Float16>(a, (int)x.pos_type, ve, interleaved, grid, s);
+    default: return launch_pos<__bf16>(a, (int)x.pos_type, ve, interleaved, grid, s);
     }
 }

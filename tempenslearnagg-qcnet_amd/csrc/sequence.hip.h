@@ -13,25 +13,22 @@ using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 constexpr int kMaxDim = 128;
 
-template <class T> struct Elem;
-template <> struct Elem<float> { static constexpr int kDtype = QCN_DTYPE_F32; };
-template <> struct Elem<_Float16> { static constexpr int kDtype = QCN_DTYPE_F16; };
-template <> struct Elem<__bf16> { static constexpr int kDtype = QCN_DTYPE_BF16; };
-
 template <class T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
 // one rounding to nearest even at the store; everything before it is fp32
 template <class T> __device__ __forceinline__ T from_f32(float x) { return (T)x; }
 
-static inline size_t dtype_bytes(int dtype) { return dtype == QCN_DTYPE_F32 ? 4 : 2; }
-static inline bool dtype_known(int dtype) { return dtype == QCN_DTYPE_F32 || dtype == QCN_DTYPE_F16 || dtype == QCN_DTYPE_BF16; }
+static inline size_t dtype_bytes(int64_t dtype) { return dtype == QCN_DTYPE_F32 ? 4 : 2; }
+static inline bool dtype_known(int64_t dtype) { return dtype == QCN_DTYPE_F32 || dtype == QCN_DTYPE_F16 || dtype == QCN_DTYPE_BF16; }
 
 // a strided row tensor [tokens, heads, dim]: the features of a head are contiguous
 struct Rows {
     int64_t tok, head;   // strides in elements
 };
 
+constexpr int64_t kMaxHeads = 32767;   // of one tensor
+
 // rows are loaded in 16-byte pieces
-static inline bool rows_aligned(const void *p, int64_t tok, int64_t head, int dtype)
+static inline bool rows_aligned(const void *p, int64_t tok, int64_t head, int64_t dtype)
 {
     const int64_t piece = 16 / (int64_t)dtype_bytes(dtype);
     return ((uintptr_t)p & 15) == 0 && tok % piece == 0 && head % piece == 0;

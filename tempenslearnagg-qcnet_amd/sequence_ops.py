@@ -12,24 +12,47 @@ whose features are contiguous and 16-byte aligned are read in place, anything el
 are float32 and every output is rounded once.  All of them launch on torch's current stream of the tensors' device, allocate
 their outputs with torch, never synchronise, and can be captured into graphs.
 """
-import ctypes
 import math
+import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
 
 from . import _lib
-from .ops import _as_u8, _op, _ptr, _register, _require, _stream
+from .ops import _as_u8, _op, _register, _require
 
 SEQUENCE_OP_NAMES: List[str] = []
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}          # QCN_DTYPE_*
 _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}            # QCN_POS_*
 MAX_HEAD_DIM = 128
+_MOST = (1 << 62) - 1
+
+# the argument structs of include/qcnet_hip.h (8-byte fields: no padding)
+_ROTARY_ARGS = struct.Struct('=27q').pack
+_WINDOW_ARGS = struct.Struct('=21qdq').pack
+_APPEND_ARGS = struct.Struct('=19q').pack
+_STEP_ARGS = struct.Struct('=18qd6q').pack
 
 
-def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    """[tokens, heads, dim] of the wanted type and device."""
+def _plain(*tensors) -> bool:
+    """Whether the call can go to the implementation directly: plain tensors, nothing tracing, nothing to differentiate.  The
+    dispatcher costs 5 us a call, as much as everything else the host does for a decoding step."""
+    if torch._C._len_torch_dispatch_stack() or torch.compiler.is_compiling():
+        return False
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (type(t) is not torch.Tensor or (grad and t.requires_grad)):
+            return False
+    return True
+
+
+def _is(t, dtype: torch.dtype, index: int, shape) -> bool:
+    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.shape == shape and t.is_contiguous()
+
+
+def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) -> None:
+    """[tokens, heads, dim] of the wanted type and device, or the error."""
     if not torch.is_tensor(t):
         raise TypeError('%s must be a tensor' % name)
     if not t.is_cuda:
@@ -40,42 +63,41 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) 
         raise TypeError('%s has dtype %s, expected %s' % (name, t.dtype, dtype))
     if t.dim() != 3:
         raise ValueError('%s must be [tokens, heads, dim], got %s' % (name, tuple(t.shape)))
-    return t
 
 
-def _in_place(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself when its rows can be read in 16-byte pieces, else a contiguous copy."""
-    tok, head, feat = t.stride()
-    piece = 16 // t.element_size()
-    if feat == 1 and tok % piece == 0 and head % piece == 0 and t.data_ptr() % 16 == 0:
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _in_place(t: torch.Tensor):
+    """(t, its strides) when its rows can be read in 16-byte pieces, else of a contiguous copy."""
+    tok, head, feat = strides = t.stride()
+    if feat == 1 and (tok | head) % (16 // t.element_size()) == 0 and t.data_ptr() % 16 == 0:
+        return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:
+    if not torch.is_tensor(t):
+        raise TypeError('%s must be a tensor' % name)
     if t.dtype not in _DTYPES:
         raise TypeError('%s has dtype %s, expected float32, float16 or bfloat16' % (name, t.dtype))
     return _DTYPES[t.dtype]
 
 
-def _head_dim(dim: int) -> None:
-    if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
-        raise _lib.QcnError('head dim %d is not supported (a multiple of 8, 8 .. %d)' % (dim, MAX_HEAD_DIM))
-
-
-def _launch(device: torch.device, what: str, *args) -> None:
-    """One C ABI call on the tensors' own device."""
+def _launch(index: int, what: str, args: bytes) -> None:
+    """One C ABI call on the tensors' own device and its current stream."""
     fn = getattr(_lib.lib(), what)
-    if torch.cuda.current_device() == device.index:
-        _lib.check(fn(*args, _stream(device)), what)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, _stream(device)), what)
+        with torch.cuda.device(index):
+            status = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        _lib.check(status, what)
 
 
 def _scale(scale: Optional[float], dim: int) -> float:
-    scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
+    if scale is None:
+        return max(dim, 1) ** -0.5
+    scale = float(scale)
     if not (math.isfinite(scale) and 0 <= scale <= 3e38):
         raise ValueError('scale must be finite and not negative, got %r' % scale)
     return scale
@@ -92,7 +114,9 @@ def rotary_embed(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, 
     ``sections``: how many feature pairs each axis turns, in order; ``freqs`` [sum(sections)] float32: radians per unit of
     position and pair.  Pair i is features (i, i + pairs), ``interleaved``: (2 i, 2 i + 1); features behind the pairs stay as
     they are.  Angles are formed in float64 (far positions keep their fraction of a turn).  ``inverse`` turns back."""
-    out = _op('rotary_embed')(q, k, pos, freqs, [int(s) for s in sections], bool(interleaved), bool(inverse))
+    sections = [int(s) for s in sections]
+    call = _rotary_embed if _plain(q, k, pos, freqs) else _op('rotary_embed')
+    out = call(q, k, pos, freqs, sections, bool(interleaved), bool(inverse))
     return out[0], (out[1] if k is not None else None)
 
 
@@ -100,63 +124,79 @@ def _rotary_embed_fake(q, k, pos, freqs, sections, interleaved, inverse):
     return [q.new_empty(q.shape)] + ([k.new_empty(k.shape)] if k is not None else [])
 
 
+def _even_rows(t):
+    """(t, its strides): any strides will do as long as a row's features are contiguous and no pair straddles its alignment."""
+    tok, head, feat = strides = t.stride()
+    if feat == 1 and not (tok | head) & 1 and t.data_ptr() % (2 * t.element_size()) == 0:
+        return t, strides
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
+
+
 @_register('rotary_embed', '(Tensor q, Tensor? k, Tensor pos, Tensor freqs, int[] sections, bool interleaved, bool inverse) -> Tensor[]',
            _rotary_embed_fake, SEQUENCE_OP_NAMES)
 def _rotary_embed(q, k, pos, freqs, sections, interleaved, inverse):
-    dev = q.device
     code = _dtype_code(q, 'q')
-    _rows(q, 'q', q.dtype, dev)
+    _rows(q, 'q', q.dtype, q.device)
     n, hq, dim = q.shape
+    index = q.get_device()
     if dim % 2 or not 2 <= dim <= 256:
         raise _lib.QcnError('head dim %d is not supported (even, 2 .. 256)' % dim)
     pairs, axes = sum(sections), len(sections)
-    if not 1 <= axes <= 8 or any(s < 0 for s in sections) or pairs < 1 or 2 * pairs > dim:
+    if not 1 <= axes <= 8 or min(sections) < 0 or pairs < 1 or 2 * pairs > dim:
         raise ValueError('sections %s: one to eight axes, at least one pair, at most dim / 2 = %d pairs' % (list(sections), dim // 2))
-    if pos.dtype not in _POS_TYPES:
-        raise TypeError('pos has dtype %s, expected float32, int32 or int64' % pos.dtype)
-    _require(pos, 'pos', pos.dtype, dev, (n, axes))
-    _require(freqs, 'freqs', torch.float32, dev, (pairs,))
+    if not torch.is_tensor(pos) or pos.dtype not in _POS_TYPES:
+        raise TypeError('pos must be a float32, int32 or int64 tensor')
+    if not _is(pos, pos.dtype, index, (n, axes)):
+        _require(pos, 'pos', pos.dtype, q.device, (n, axes))
+    if not _is(freqs, torch.float32, index, (pairs,)):
+        _require(freqs, 'freqs', torch.float32, q.device, (pairs,))
     hk = 0
     if k is not None:
-        _rows(k, 'k', q.dtype, dev)
+        _rows(k, 'k', q.dtype, q.device)
         hk = k.size(1)
         if k.size(0) != n or k.size(2) != dim:
             raise ValueError('k has shape %s, expected (%d, heads, %d)' % (tuple(k.shape), n, dim))
         if hk == 0:
             raise ValueError('k has no heads: pass None')
-    # any stride is fine as long as a row's features are contiguous and no pair straddles its alignment
-    ok = lambda t: t.stride(2) == 1 and t.stride(0) % 2 == 0 and t.stride(1) % 2 == 0 and t.data_ptr() % (2 * t.element_size()) == 0
-    q = q if ok(q) else q.clone(memory_format=torch.contiguous_format)
-    q_out = torch.empty(n, hq, dim, dtype=q.dtype, device=dev)
-    k_out = None
-    if k is not None:
-        k = k if ok(k) else k.clone(memory_format=torch.contiguous_format)
-        k_out = torch.empty(n, hk, dim, dtype=q.dtype, device=dev)
-    _launch(dev, 'qcn_rotary_embed', q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr() if hk else None,
-            k.stride(0) if hk else 0, k.stride(1) if hk else 0, hk, n, dim, code, pos.data_ptr(), _POS_TYPES[pos.dtype], axes,
-            freqs.data_ptr(), (ctypes.c_int32 * axes)(*sections), int(interleaved), int(inverse), q_out.data_ptr(),
-            k_out.data_ptr() if hk else None)
-    return [q_out] + ([k_out] if hk else [])
+    q, qs = _even_rows(q)
+    outs = [q.new_empty((n, hq, dim))]
+    kp = ks0 = ks1 = k_out = 0
+    if hk:
+        k, (ks0, ks1, _) = _even_rows(k)
+        kp = k.data_ptr()
+        outs.append(q.new_empty((n, hk, dim)))
+        k_out = outs[1].data_ptr()
+    if n and (hq or hk):
+        _launch(index, 'qcn_rotary_embed', _ROTARY_ARGS(
+            q.data_ptr(), qs[0], qs[1], hq, kp, ks0, ks1, hk, n, dim, code, pos.data_ptr(), _POS_TYPES[pos.dtype], axes,
+            *sections, *([0] * (8 - axes)), freqs.data_ptr(), interleaved, inverse, outs[0].data_ptr(), k_out))
+    return outs
 
 
 # ------------------------------------------------------------------------------------------------
 # attention over ragged sequences
 # ------------------------------------------------------------------------------------------------
-def _check_kv(q, k, v):
+def _check_kv(q, k, v) -> int:
+    """The type code of a matching set of rows, or the error."""
     code = _dtype_code(k, 'k')
-    dev = k.device
-    _rows(k, 'k', k.dtype, dev)
-    _rows(v, 'v', k.dtype, dev)
-    if k.shape != v.shape:
-        raise ValueError('k and v differ in shape: %s and %s' % (tuple(k.shape), tuple(v.shape)))
-    _head_dim(k.size(2))
-    if k.size(1) < 1:
+    dtype, index = k.dtype, k.get_device()
+    ks = k.shape
+    if not (index >= 0 and len(ks) == 3 and isinstance(v, torch.Tensor) and v.dtype is dtype and v.get_device() == index and v.shape == ks):
+        _rows(k, 'k', dtype, k.device)
+        _rows(v, 'v', dtype, k.device)
+        raise ValueError('k and v differ in shape: %s and %s' % (tuple(ks), tuple(v.shape)))
+    _, hk, dim = ks
+    if dim % 8 or not 8 <= dim <= MAX_HEAD_DIM:
+        raise _lib.QcnError('head dim %d is not supported (a multiple of 8, 8 .. %d)' % (dim, MAX_HEAD_DIM))
+    if hk < 1:
         raise ValueError('k has no heads')
     if q is not None:
-        _rows(q, 'q', k.dtype, dev)
-        if q.size(2) != k.size(2) or q.size(1) < 1 or q.size(1) % k.size(1):
-            raise ValueError('q has shape %s: its dim must be %d and its heads a multiple of %d' % (tuple(q.shape), k.size(2), k.size(1)))
-    return code, dev
+        if not (isinstance(q, torch.Tensor) and q.dtype is dtype and q.get_device() == index and q.dim() == 3):
+            _rows(q, 'q', dtype, k.device)
+        if q.size(2) != dim or q.size(1) < 1 or q.size(1) % hk:
+            raise ValueError('q has shape %s: its dim must be %d and its heads a multiple of %d' % (tuple(q.shape), dim, hk))
+    return code
 
 
 def attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, window: int, sinks: int = 0,
@@ -169,62 +209,82 @@ def attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     (ascending from 0); ``cu_k``: those in k and v, if a sequence has keys in front of its queries (a chunk behind a prefix: the
     queries are its last positions).  ``key_mask`` bool [Nk]: false keys are seen by nobody, whatever k and v hold there.  A row
     that sees nothing is zero, and so are rows behind ``cu_q[-1]``.  ``scale`` defaults to D ** -0.5."""
-    return _op('attn_window')(q, k, v, cu_q, int(window), int(sinks), cu_k, key_mask, _scale(scale, q.size(-1)))
+    call = _attn_window if _plain(q, k, v, cu_q, cu_k, key_mask) else _op('attn_window')
+    return call(q, k, v, cu_q, int(window), int(sinks), cu_k, key_mask, _scale(scale, q.size(-1)))
 
 
 @_register('attn_window', '(Tensor q, Tensor k, Tensor v, Tensor cu_q, int window, int sinks, Tensor? cu_k, Tensor? key_mask, '
            'float scale) -> Tensor', lambda q, k, v, cu_q, window, sinks, cu_k, key_mask, scale: q.new_empty(q.shape),
            SEQUENCE_OP_NAMES)
 def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
-    code, dev = _check_kv(q, k, v)
+    code = _check_kv(q, k, v)
+    index = k.get_device()
     nq, hq, dim = q.shape
-    nk, hk = k.size(0), k.size(1)
+    nk, hk, _ = k.shape
     if window < 1 or sinks < 0:
         raise ValueError('window must be at least 1 and sinks at least 0, got %d and %d' % (window, sinks))
-    _require(cu_q, 'cu_q', torch.int64, dev, (None,))
-    if cu_q.numel() < 1:
+    if not torch.is_tensor(cu_q) or cu_q.dim() != 1 or cu_q.numel() < 1:
         raise ValueError('cu_q must hold B + 1 boundaries')
+    n_cu = cu_q.size(0)
+    if not _is(cu_q, torch.int64, index, (n_cu,)):
+        _require(cu_q, 'cu_q', torch.int64, k.device, (n_cu,))
+    cu_k_ptr = cu_q.data_ptr()
     if cu_k is None:
         if nk != nq:
             raise ValueError('k has %d tokens and q %d: pass cu_k' % (nk, nq))
-        cu_k = cu_q
     else:
-        _require(cu_k, 'cu_k', torch.int64, dev, (cu_q.numel(),))
+        if not _is(cu_k, torch.int64, index, (n_cu,)):
+            _require(cu_k, 'cu_k', torch.int64, k.device, (n_cu,))
+        cu_k_ptr = cu_k.data_ptr()
+    mask_ptr = 0
     if key_mask is not None:
-        key_mask = _as_u8(key_mask, 'key_mask', dev, (nk,))
+        if not _is(key_mask, torch.bool, index, (nk,)):
+            key_mask = _as_u8(key_mask, 'key_mask', k.device, (nk,))
+        mask_ptr = key_mask.data_ptr()
     scale = _scale(scale, dim)
-    q, k, v = _in_place(q), _in_place(k), _in_place(v)
-    out = torch.empty(nq, hq, dim, dtype=q.dtype, device=dev)
-    _launch(dev, 'qcn_attn_window', q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), cu_q.data_ptr(), cu_k.data_ptr(), key_mask.data_ptr() if key_mask is not None else None,
-            cu_q.numel() - 1, nq, nk, hq, hk, dim, code, min(window, 1 << 62), min(sinks, 1 << 62), scale, out.data_ptr())
+    q, qs = _in_place(q)
+    k, ks = _in_place(k)
+    v, vs = _in_place(v)
+    out = q.new_empty((nq, hq, dim))
+    if nq:
+        _launch(index, 'qcn_attn_window', _WINDOW_ARGS(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
+            n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr()))
     return out
 
 
 # ------------------------------------------------------------------------------------------------
 # the bounded cache
 # ------------------------------------------------------------------------------------------------
-def _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch, dev):
-    hk, dim = k.size(1), k.size(2)
+def _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch):
+    """(window, pointer of the mask cache) of a matching cache, or the error.  Caches are written in place: no copy stands in."""
+    _, hk, dim = k.shape
+    dtype, index = k.dtype, k.get_device()
     if sinks < 0:
         raise ValueError('sinks must be at least 0, got %d' % sinks)
-    _require(k_cache, 'k_cache', k.dtype, dev, (batch, hk, None, dim))
-    slots = k_cache.size(2)
-    _require(v_cache, 'v_cache', k.dtype, dev, (batch, hk, slots, dim))
+    slots = k_cache.size(2) if torch.is_tensor(k_cache) and k_cache.dim() == 4 else -1
+    shape = (batch, hk, slots, dim)
+    if not (_is(k_cache, dtype, index, shape) and _is(v_cache, dtype, index, shape)):
+        _require(k_cache, 'k_cache', dtype, k.device, (batch, hk, None, dim))
+        _require(v_cache, 'v_cache', dtype, k.device, shape)
     if slots <= sinks:
         raise ValueError('the cache has %d slots: sinks + window, with a window of at least 1 behind %d sinks' % (slots, sinks))
-    if k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
+    kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
+    if (kp | vp) % 16:
         raise ValueError('the caches must start on 16-byte boundaries')
-    if batch and k_cache.data_ptr() == v_cache.data_ptr():
+    if batch and kp == vp:
         raise ValueError('k_cache and v_cache are the same memory')
-    _require(lengths, 'lengths', torch.int64, dev, (batch,))
+    if not _is(lengths, torch.int64, index, (batch,)):
+        _require(lengths, 'lengths', torch.int64, k.device, (batch,))
     if mask_cache is not None:
-        if mask_cache.dtype == torch.bool:
-            mask_cache = mask_cache.view(torch.uint8)
-        _require(mask_cache, 'mask_cache', torch.uint8, dev, (batch, slots))      # written in place: no copy may stand in for it
-    elif key_mask is not None:
+        if not _is(mask_cache, torch.bool, index, (batch, slots)):
+            if torch.is_tensor(mask_cache) and mask_cache.dtype == torch.bool:
+                mask_cache = mask_cache.view(torch.uint8)
+            _require(mask_cache, 'mask_cache', torch.uint8, k.device, (batch, slots))
+        return slots - sinks, mask_cache.data_ptr()
+    if key_mask is not None:
         raise ValueError('key_mask needs a mask_cache to keep it in')
-    return slots - sinks, mask_cache
+    return slots - sinks, 0
 
 
 def window_cache_append(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, lengths: torch.Tensor, k_cache: torch.Tensor,
@@ -236,26 +296,34 @@ def window_cache_append(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, leng
     Position p lies in slot p (p < sinks) or sinks + (p - sinks) % window.  ``lengths`` is left as it is, so that the layers of a
     model share it: advance it once per call of the model.  Sequences with a negative length and rows behind ``cu[-1]`` are left
     alone.  ``mask_cache`` bool [B, sinks + window] takes ``key_mask`` [N] (true where that is None)."""
-    _op('window_cache_append')(k, v, cu, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache)
+    call = _window_cache_append if _plain(k, v, cu, lengths, k_cache, v_cache, key_mask, mask_cache) else _op('window_cache_append')
+    call(k, v, cu, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache)
 
 
 @_register('window_cache_append', '(Tensor k, Tensor v, Tensor cu, Tensor lengths, Tensor(a!) k_cache, Tensor(b!) v_cache, int sinks, '
            'Tensor? key_mask, Tensor(c!)? mask_cache) -> ()',
            lambda k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, mask_cache: None, SEQUENCE_OP_NAMES)
 def _window_cache_append(k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, mask_cache):
-    code, dev = _check_kv(None, k, v)
+    code = _check_kv(None, k, v)
+    index = k.get_device()
     n, hk, dim = k.shape
-    _require(cu, 'cu', torch.int64, dev, (None,))
-    batch = cu.numel() - 1
-    if batch < 0:
+    if not torch.is_tensor(cu) or cu.dim() != 1 or cu.numel() < 1:
         raise ValueError('cu must hold B + 1 boundaries')
-    window, mask_cache = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch, dev)
+    batch = cu.size(0) - 1
+    if not _is(cu, torch.int64, index, (batch + 1,)):
+        _require(cu, 'cu', torch.int64, k.device, (batch + 1,))
+    window, mask_cache_ptr = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch)
+    mask_ptr = 0
     if key_mask is not None:
-        key_mask = _as_u8(key_mask, 'key_mask', dev, (n,))
-    k, v = _in_place(k), _in_place(v)
-    _launch(dev, 'qcn_window_cache_append', k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-            cu.data_ptr(), lengths.data_ptr(), key_mask.data_ptr() if key_mask is not None else None, batch, n, hk, dim, code,
-            window, sinks, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache.data_ptr() if mask_cache is not None else None)
+        if not _is(key_mask, torch.bool, index, (n,)):
+            key_mask = _as_u8(key_mask, 'key_mask', k.device, (n,))
+        mask_ptr = key_mask.data_ptr()
+    k, ks = _in_place(k)
+    v, vs = _in_place(v)
+    if n and batch:
+        _launch(index, 'qcn_window_cache_append', _APPEND_ARGS(
+            k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu.data_ptr(), lengths.data_ptr(), mask_ptr, batch, n, hk, dim,
+            code, window, sinks, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache_ptr))
 
 
 def attn_window_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, k_cache: torch.Tensor,
@@ -266,29 +334,36 @@ def attn_window_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
 
     ``lengths`` is left as it is (see :func:`window_cache_append`).  A negative length marks a row that is not in use: its output
     is zero and its cache untouched.  ``key_mask`` bool [B]: whether the new token is visible, kept in ``mask_cache``."""
-    return _op('attn_window_step')(q, k, v, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache, _scale(scale, q.size(-1)))
+    call = _attn_window_step if _plain(q, k, v, lengths, k_cache, v_cache, key_mask, mask_cache) else _op('attn_window_step')
+    return call(q, k, v, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache, _scale(scale, q.size(-1)))
 
 
 @_register('attn_window_step', '(Tensor q, Tensor k, Tensor v, Tensor lengths, Tensor(a!) k_cache, Tensor(b!) v_cache, int sinks, '
            'Tensor? key_mask, Tensor(c!)? mask_cache, float scale) -> Tensor',
            lambda q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_cache, scale: q.new_empty(q.shape), SEQUENCE_OP_NAMES)
 def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_cache, scale):
-    code, dev = _check_kv(q, k, v)
+    code = _check_kv(q, k, v)
+    index = k.get_device()
     batch, hq, dim = q.shape
     hk = k.size(1)
     if k.size(0) != batch:
         raise ValueError('k has %d rows, expected %d' % (k.size(0), batch))
-    window, mask_cache = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch, dev)
+    window, mask_cache_ptr = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch)
+    mask_ptr = 0
     if key_mask is not None:
-        key_mask = _as_u8(key_mask, 'key_mask', dev, (batch,))
+        if not _is(key_mask, torch.bool, index, (batch,)):
+            key_mask = _as_u8(key_mask, 'key_mask', k.device, (batch,))
+        mask_ptr = key_mask.data_ptr()
     scale = _scale(scale, dim)
-    q, k, v = _in_place(q), _in_place(k), _in_place(v)
-    out = torch.empty(batch, hq, dim, dtype=q.dtype, device=dev)
-    ws_bytes = _lib.lib().qcn_attn_window_step_workspace_bytes(batch, hq, hk, dim, window, sinks)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    _launch(dev, 'qcn_attn_window_step', q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-            v.stride(0), v.stride(1), lengths.data_ptr(), key_mask.data_ptr() if key_mask is not None else None, batch, hq, hk, dim,
-            code, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(),
-            mask_cache.data_ptr() if mask_cache is not None else None, out.data_ptr(), ws.data_ptr() if ws is not None else None,
-            ws_bytes)
+    q, qs = _in_place(q)
+    k, ks = _in_place(k)
+    v, vs = _in_place(v)
+    out = q.new_empty((batch, hq, dim))
+    if batch:
+        ws_bytes = _lib.lib().qcn_attn_window_step_workspace_bytes(batch, hq, hk, dim, window, sinks)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=k.device) if ws_bytes else None
+        _launch(index, 'qcn_attn_window_step', _STEP_ARGS(
+            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], lengths.data_ptr(), mask_ptr, batch, hq,
+            hk, dim, code, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache_ptr, out.data_ptr(),
+            ws.data_ptr() if ws_bytes else 0, ws_bytes))
     return out

@@ -1,6 +1,6 @@
 """CPU: the sequence operators are registered, refuse CPU tensors, and their C entry points refuse bad calls before any launch;
 the float64 forms they are tested against agree with each other."""
-import ctypes
+import struct
 
 import pytest
 import torch
@@ -31,58 +31,65 @@ def test_registered_and_refusing_cpu_tensors():
             ops.attn_window(x, x, x, torch.tensor([0, 4]), 3, scale=bad)
 
 
-def _window(lib, q=FAKE, k=FAKE, v=FAKE, tok=32, head=16, cu=FAKE, n_seq=1, nq=4, nk=4, hq=2, hk=2, dim=16, dtype=0, win=3, sinks=0,
-            scale=1.0, out=FAKE):
-    return lib.qcn_attn_window(q, tok, head, k, tok, head, v, tok, head, cu, cu, None, n_seq, nq, nk, hq, hk, dim, dtype, win, sinks,
-                               ctypes.c_float(scale), out, None)
+def _call(lib, name, fmt, fields, **over):
+    """The entry point on its argument struct: ``fields`` in the header's order, with some of them replaced."""
+    values = dict(fields, **over)
+    assert list(values) == list(fields)
+    return getattr(lib, name)(struct.pack('=' + fmt, *[x for v in values.values() for x in (v if isinstance(v, tuple) else (v,))]), None)
 
 
 def test_window_entry_point_refusals():
     lib = _lib.lib()
-    for bad in (dict(hq=3), dict(hq=0), dict(hk=0), dict(n_seq=-1), dict(nq=-1), dict(nk=-1), dict(win=0), dict(sinks=-1), dict(dtype=3),
-                dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(q=None), dict(k=None), dict(cu=None),
-                dict(out=None), dict(q=FAKE + 4), dict(k=FAKE + 8), dict(tok=33), dict(head=2), dict(out=FAKE + 4)):
-        assert _window(lib, **bad) == INVALID, bad
-    for bad in (dict(dim=20), dict(dim=136), dict(dim=0), dict(nq=1 << 41)):
-        assert _window(lib, **bad) == UNSUPPORTED, bad
-    assert _window(lib, nq=0) == 0
-
-
-def _step(lib, q=FAKE, k=FAKE, v=FAKE, lengths=FAKE, key_mask=None, batch=2, hq=4, hk=2, dim=64, dtype=2, win=4, sinks=1, kc=FAKE, vc=FAKE,
-          mc=None, out=FAKE, ws=None, ws_bytes=0, tok=512, head=64):
-    return lib.qcn_attn_window_step(q, tok, head, k, tok, head, v, tok, head, lengths, key_mask, batch, hq, hk, dim, dtype, win, sinks,
-                                    ctypes.c_float(1.0), kc, vc, mc, out, ws, ws_bytes, None)
+    fields = dict(q=FAKE, qs=(32, 16), k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu_q=FAKE, cu_k=FAKE, mask=0, n_seq=1, nq=4, nk=4, hq=2,
+                  hk=2, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE)
+    call = lambda **over: _call(lib, 'qcn_attn_window', '21qdq', fields, **over)
+    for bad in (dict(hq=3), dict(hq=0), dict(hk=0), dict(n_seq=-1), dict(nq=-1), dict(nk=-1), dict(window=0), dict(sinks=-1), dict(dtype=3),
+                dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(q=0), dict(k=0), dict(v=0), dict(cu_q=0),
+                dict(cu_k=0), dict(out=0), dict(q=FAKE + 4), dict(k=FAKE + 8), dict(qs=(33, 16)), dict(vs=(32, 2)), dict(out=FAKE + 4)):
+        assert call(**bad) == INVALID, bad
+    for bad in (dict(dim=20), dict(dim=136), dict(dim=0), dict(nq=1 << 31), dict(nk=1 << 31), dict(n_seq=1 << 31), dict(hq=1 << 16)):
+        assert call(**bad) == UNSUPPORTED, bad
+    assert call(nq=0) == 0
+    assert lib.qcn_attn_window(None, None) == INVALID
 
 
 def test_step_and_append_entry_point_refusals():
     lib = _lib.lib()
-    for bad in (dict(hq=3), dict(hk=0), dict(batch=-1), dict(win=0), dict(sinks=-1), dict(dtype=-1), dict(q=None), dict(lengths=None),
-                dict(kc=None), dict(vc=FAKE + 2), dict(out=None), dict(key_mask=FAKE), dict(head=60), dict(win=1 << 41)):
-        assert _step(lib, **bad) == INVALID, bad
-    assert _step(lib, dim=12) == UNSUPPORTED
-    assert _step(lib, batch=0) == 0
-    app = lambda k=FAKE, n_seq=1, n=4, hk=2, dim=16, dtype=0, win=3, sinks=0, kc=FAKE, km=None, mc=None, tok=32: \
-        lib.qcn_window_cache_append(k, tok, 16, FAKE, 32, 16, FAKE, FAKE, km, n_seq, n, hk, dim, dtype, win, sinks, kc, FAKE, mc, None)
-    for bad in (dict(k=None), dict(n_seq=-1), dict(n=-1), dict(hk=0), dict(dtype=9), dict(win=0), dict(sinks=-2), dict(kc=None),
-                dict(km=FAKE), dict(tok=31)):
+    fields = dict(q=FAKE, qs=(512, 64), k=FAKE, ks=(512, 64), v=FAKE, vs=(512, 64), lengths=FAKE, key_mask=0, batch=2, hq=4, hk=2, dim=64,
+                  dtype=2, window=4, sinks=1, scale=1.0, kc=FAKE, vc=FAKE, mc=0, out=FAKE, ws=0, ws_bytes=0)
+    step = lambda **over: _call(lib, 'qcn_attn_window_step', '18qd6q', fields, **over)
+    for bad in (dict(hq=3), dict(hk=0), dict(batch=-1), dict(window=0), dict(sinks=-1), dict(dtype=-1), dict(q=0), dict(lengths=0), dict(kc=0),
+                dict(vc=FAKE + 2), dict(out=0), dict(key_mask=FAKE), dict(qs=(512, 60)), dict(window=1 << 41), dict(scale=-1.0)):
+        assert step(**bad) == INVALID, bad
+    assert step(dim=12) == UNSUPPORTED and step(batch=1 << 31) == UNSUPPORTED
+    assert step(batch=0) == 0
+    need = lib.qcn_attn_window_step_workspace_bytes(2, 4, 2, 64, 4096, 1)
+    assert need > 0 and lib.qcn_attn_window_step_workspace_bytes(2, 4, 2, 64, 50, 1) == 0
+    assert step(window=4096) == WORKSPACE and step(window=4096, ws=FAKE, ws_bytes=need - 1) == WORKSPACE
+    assert lib.qcn_attn_window_step(None, None) == INVALID
+    fields2 = dict(k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu=FAKE, lengths=FAKE, key_mask=0, n_seq=1, n=4, hk=2, dim=16, dtype=0, window=3,
+                   sinks=0, kc=FAKE, vc=FAKE, mc=0)
+    app = lambda **over: _call(lib, 'qcn_window_cache_append', '19q', fields2, **over)
+    for bad in (dict(k=0), dict(n_seq=-1), dict(n=-1), dict(hk=0), dict(dtype=9), dict(window=0), dict(sinks=-2), dict(kc=0),
+                dict(key_mask=FAKE), dict(ks=(31, 16)), dict(cu=0), dict(lengths=0)):
         assert app(**bad) == INVALID, bad
     assert app(dim=18) == UNSUPPORTED
     assert app(n=0) == 0 and app(n_seq=0) == 0
+    assert lib.qcn_window_cache_append(None, None) == INVALID
 
 
 def test_rotary_entry_point_refusals():
     lib = _lib.lib()
-
-    def call(sections=(8,), n=4, hq=2, hk=0, k=None, dim=16, dtype=0, pos=FAKE, pos_type=0, q=FAKE, out=FAKE, interleaved=0, tok=32):
-        arr = (ctypes.c_int32 * max(1, len(sections)))(*sections)
-        return lib.qcn_rotary_embed(q, tok, 16, hq, k, tok, 16, hk, n, dim, dtype, pos, pos_type, len(sections), FAKE, arr, interleaved, 0,
-                                    out, out, None)
-    for bad in (dict(sections=()), dict(sections=(1,) * 9), dict(sections=(9,)), dict(sections=(0,)), dict(sections=(-1, 4)), dict(dim=15),
-                dict(dtype=5), dict(pos_type=3), dict(pos=None), dict(q=None), dict(hk=1), dict(k=FAKE), dict(n=-1),
-                dict(interleaved=1, tok=33)):
+    fields = dict(q=FAKE, qs=(32, 16), hq=2, k=0, ks=(0, 0), hk=0, n=4, dim=16, dtype=0, pos=FAKE, pos_type=0, axes=1,
+                  sections=(8,) + (0,) * 7, freqs=FAKE, interleaved=0, inverse=0, q_out=FAKE, k_out=0)
+    call = lambda **over: _call(lib, 'qcn_rotary_embed', '27q', fields, **over)
+    for bad in (dict(axes=0), dict(axes=9), dict(sections=(9,) + (0,) * 7), dict(sections=(0,) * 8), dict(sections=(-1, 4) + (0,) * 6, axes=2),
+                dict(dim=15), dict(dtype=5), dict(pos_type=3), dict(pos=0), dict(freqs=0), dict(q=0), dict(q_out=0), dict(hk=1), dict(k=FAKE),
+                dict(n=-1), dict(interleaved=1, qs=(33, 16)), dict(q=FAKE + 2)):
         assert call(**bad) == INVALID, bad
-    assert call(dim=258) == UNSUPPORTED and call(n=1 << 31) == UNSUPPORTED
+    assert call(dim=258) == UNSUPPORTED and call(n=1 << 31) == UNSUPPORTED and call(hq=1 << 16) == UNSUPPORTED
     assert call(n=0) == 0
+    assert lib.qcn_rotary_embed(None, None) == INVALID
 
 
 def test_the_cache_holds_what_a_position_sees():
