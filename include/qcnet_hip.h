@@ -535,7 +535,8 @@ int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream);
  * (j > p - window or j < sinks) and key_mask[j] (uint8 [n_k_tokens], NULL: all).  out [n_q_tokens, n_q_heads, dim] =
  * softmax(scale q.k) v over what it sees; rows that see nothing and rows behind cu_q[n_seq] are 0.  Masked keys and values may
  * hold anything, NaN and infinities among it.  Query head h reads key head h / (n_q_heads / n_kv_heads).
- * scale: finite, >= 0. */
+ * scale: finite, >= 0.  Token strides of k and v below 2^24 elements.  The workspace's contents do not outlive the call's work
+ * on its stream. */
 typedef struct {
     const void *q;
     int64_t q_strides[2];
@@ -549,7 +550,11 @@ typedef struct {
     int64_t window, sinks;
     double scale;
     void *out;
+    void *workspace;
+    int64_t workspace_bytes;
 } qcn_attn_window_args;
+/* what the call needs for these sizes (it reads sizes and types only): 0 unless few query tokens meet long windows */
+int64_t qcn_attn_window_workspace_bytes(const qcn_attn_window_args *args);
 int qcn_attn_window(const qcn_attn_window_args *args, void *stream);
 
 /* The cache of that attention: [n_seq, n_kv_heads, sinks + window, dim] contiguous; position p in slot p (p < sinks) or

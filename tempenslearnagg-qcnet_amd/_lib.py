@@ -124,9 +124,11 @@ def _declare(lib) -> None:
     lib.qcn_nms_select_f32.restype = c_int
     lib.qcn_nms_select_f32.argtypes = [P, P, P, c_int64, c_int, c_int, c_int, c_int, c_int, c_float, c_float, P, P, P]
     # argument structs of 8-byte fields, packed by the caller (sequence_ops.py); `bytes` pass as the pointer
-    for name in ('qcn_rotary_embed', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step'):
+    for name in ('qcn_rotary_embed', 'qcn_attn_window_workspace_bytes', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step'):
         getattr(lib, name).restype = c_int
         getattr(lib, name).argtypes = [ctypes.c_char_p, P]
+    lib.qcn_attn_window_workspace_bytes.restype = c_int64
+    lib.qcn_attn_window_workspace_bytes.argtypes = [ctypes.c_char_p]
     lib.qcn_attn_window_step_workspace_bytes.restype = c_size_t
     lib.qcn_attn_window_step_workspace_bytes.argtypes = [c_int64] * 6
 
@@ -139,7 +141,7 @@ EXPORTED_SYMBOLS = (
     'qcn_attn_modes_store_f32', 'qcn_attn_modes_store_bf16', 'qcn_attn_modes_cached_f32', 'qcn_attn_modes_table_slots', 'qcn_stream_copy', 'qcn_gru_blocked_rows', 'qcn_fourier_gru_input_f32', 'qcn_gru_blocked_f32',
     'qcn_motion_metrics_f32', 'qcn_to_agent_frame_f32', 'qcn_to_world_frame_f32', 'qcn_nms_select_f32',
     'qcn_csr_static_max_edges', 'qcn_csr_build_static',
-    'qcn_rotary_embed', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step_workspace_bytes', 'qcn_attn_window_step',
+    'qcn_rotary_embed', 'qcn_attn_window_workspace_bytes', 'qcn_attn_window', 'qcn_window_cache_append', 'qcn_attn_window_step_workspace_bytes', 'qcn_attn_window_step',
     'qcn_mask_pairs_count', 'qcn_mask_pairs_fill', 'qcn_coalesce_workspace_bytes', 'qcn_coalesce_count', 'qcn_coalesce_fill',
 )
 

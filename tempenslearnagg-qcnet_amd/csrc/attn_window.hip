@@ -90,6 +90,14 @@ struct Keys {
     __device__ __forceinline__ int key(int j) const { return j < sinks ? j : j - sinks + start; }
 };
 
+// What one row sees of that range:  [0, sinks)  and  [lo, hi).
+struct Sees {
+    int sinks, lo, hi;
+    // bits of the 64 indexes from j0 on
+    static __device__ __forceinline__ uint64_t below(int n) { return n <= 0 ? 0 : (n >= 64 ? ~0ull : (1ull << n) - 1); }
+    __device__ __forceinline__ uint64_t bits(int j0) const { return below(sinks - j0) | (below(hi - j0) & ~below(lo - j0)); }
+};
+
 __device__ __forceinline__ int window_start(const Args &a, int p) { return a.window > (int64_t)p ? 0 : (int)(p + 1 - a.window); }
 
 __device__ __forceinline__ Keys key_range(const Args &a, int p0, int p1)
@@ -99,6 +107,21 @@ __device__ __forceinline__ Keys key_range(const Args &a, int p0, int p1)
     k.sinks = a.sinks < k.start ? (int)a.sinks : k.start;
     k.total = p1 < 0 ? 0 : k.sinks + p1 + 1 - k.start;
     return k;
+}
+
+// Sinks in front of the window keep their own index, and so do those inside it (then the range starts at the window, sinks
+// reaching into it, and index = key): either way the sinks up to p are the first min(sinks, p + 1) indexes.
+__device__ __forceinline__ Sees row_sees(const Args &a, const Keys &k, int p)
+{
+    if (p < 0) return {0, 0, 0};
+    return {a.sinks < (int64_t)p + 1 ? (int)a.sinks : p + 1, window_start(a, p) - k.start + k.sinks, p + 1 - k.start + k.sinks};
+}
+
+// x where the bit is set, else -inf
+__device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
+{
+    const int keep = __builtin_amdgcn_sbfe((int)bits, bit, 1);
+    return __builtin_bit_cast(float, (__builtin_bit_cast(int, x) & keep) | ((int)0xff800000 & ~keep));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -144,7 +167,7 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     const int p = (int)qi + t.shift;
     const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
-    const int lo = p < 0 ? 0 : window_start(a, p);
+    const Sees sees = row_sees(a, keys, p);
     const int lo1 = p1 < 0 ? 0 : window_start(a, p1);
 
     const T *q = reinterpret_cast<const T *>(a.q) + (t.q_beg + qi) * a.qr.tok + head * a.qr.head;
@@ -201,17 +224,20 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         // the last row's window
         const int jz = j0 + 16 * NU - 1;
         const bool full = !mask && j0 >= keys.sinks && jz < keys.total && keys.key(jz) <= p0 && keys.key(j0) >= lo1;
+        if (!full) {
+            const uint64_t vis = sees.bits(j0);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const unsigned w = ((unsigned)(vis >> (16 * u)) & seen[u]) >> (4 * g);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[u][r] = seen_or_inf(w, r, s[u][r]);
+            }
+        }
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (!full) {
-                    const int key = keys.key(j0 + 16 * u + 4 * g + r);
-                    if (!(((seen[u] >> (4 * g + r)) & 1) && key <= p && (key >= lo || key < a.sinks))) s[u][r] = -INFINITY;
-                }
-                top = fmaxf(top, s[u][r]);
-            }
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
@@ -312,13 +338,17 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
 // ---------------------------------------------------------------------------------------------------------------------
 // 128 rows per block, keys through LDS (16-bit types)
 // ---------------------------------------------------------------------------------------------------------------------
-// Four waves of 32 rows share tiles of 64 keys, double-buffered in LDS; the next tile's loads are in flight while the matrix
-// units work on this one, one barrier per tile.  v_mfma_f32_32x32x16: A = 32 keys (S^T) or 32 features (O^T), B = 32 rows.
-// With the accumulator's row order, k-step t of key half-tile u contracts keys  32 u + 16 t + {4 h .. 4 h + 3, 8 + 4 h ..}  in lane
-// half h: V^T is fetched in that order by two transposing LDS reads, P^T is the S^T registers rounded to 16 bits.
+// Four waves of 32 rows share tiles of 64 keys, double-buffered in LDS; the next tile's copies (global -> LDS, no registers) are
+// in flight while the matrix units work on this one, one barrier per tile.  v_mfma_f32_32x32x16: A = 32 keys (S^T) or 32 features
+// (O^T), B = 32 rows.  With the accumulator's row order, k-step t of key half-tile u contracts keys
+// 32 u + 16 t + {4 h .. 4 h + 3, 8 + 4 h ..}  in lane half h: V^T is fetched in that order by two transposing LDS reads, P^T is the
+// S^T registers rounded to 16 bits.
 //
 // LDS rows are swizzled in 16-byte pieces so that 16 neighbouring keys' pieces (K) and the 4 x 64 bytes of a transposing read
-// (V) cover all 64 banks.
+// (V) cover all 64 banks; the copies write LDS in order and permute their source addresses.
+//
+// With few blocks (a short chunk of queries behind a long prefix) the key tiles are split over blocks as well and joined by a
+// second kernel.
 template <int DP> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (DP == 128 ? row & 15 : DP == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
@@ -328,36 +358,51 @@ template <int DP> __device__ __forceinline__ int v_piece(int row, int piece)
     return piece ^ (DP == 128 ? (row & 3) << 2 : DP == 64 ? ((row >> 1) & 1) << 2 : 0);
 }
 
-constexpr int kRowShift = 7, kKeys = 64;
+constexpr int64_t kMost = ((int64_t)1 << 31) - 1;   // positions are 32-bit
+constexpr int kRowShift = 7, kKeys = 64, kMaxSplits = 8;
+
+__device__ __forceinline__ void copy_to_lds(const void *src, void *dst)
+{
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst,
+                                     16, 0, 0);
+}
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_t n_tiles)
+__global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_t n_tiles, int splits, float *part_o, float *part_ml)
 {
-    constexpr int PIECES = DP / 8, PER = kKeys * PIECES / 256, NK = DP / 16, ND = DP / 32;
+    constexpr int PIECES = DP / 8, PER = DP / 32, NK = DP / 16, ND = DP / 32, TILE = kKeys * DP;
     using V8 = typename Mat<T>::V8;
-    __shared__ T lds[2][2][kKeys * DP];                    // [buffer][K, V]
+    __shared__ __attribute__((aligned(16))) T lds[4 * TILE];   // K, V of one buffer, K, V of the other
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t item = qcn_xcd_remap(blockIdx.x, gridDim.x);
-    const int64_t tile = item % n_tiles;
-    const int kvh = (int)(item / n_tiles);
+    unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
+    const int split = (int)(item % (unsigned)splits);
+    item /= (unsigned)splits;
+    const int64_t tile = item % (unsigned)n_tiles;
+    const int kvh = (int)(item / (unsigned)n_tiles);
     const Tile t = find_tile(a, tile, kRowShift, lane);
     if (t.row0 < 0 || t.row0 >= t.rows) return;
     const int64_t left = t.rows - 1 - t.row0;
-    const int last = (int)(left < 127 ? left : 127);       // last row of the tile
-    if (t.behind) {
-        for (int r = wave; r <= last; r += 4)
-            zero_row<T>(a, t.q_beg + (t.row0 + r) / a.group, kvh * a.group + (int)((t.row0 + r) % a.group), lane, 64);
-        return;
-    }
+    const int last = (int)(left < 127 ? left : 127);           // last row of the tile
     const int r_local = wave * 32 + n;
     const bool real = r_local <= last;
     const int64_t row = t.row0 + (real ? r_local : last);
     const int64_t qi = row / a.group;
     const int head = kvh * a.group + (int)(row % a.group);
-    const int p = (int)qi + t.shift, lo = p < 0 ? 0 : window_start(a, p);
+    const int64_t out_row = (t.q_beg + qi) * a.hq + head;
+    if (t.behind) {
+        if (splits > 1) {
+            if (real && h == 0) part_ml[2 * (out_row * splits + split)] = -INFINITY;
+            return;
+        }
+        for (int r = wave; r <= last; r += 4)
+            zero_row<T>(a, t.q_beg + (t.row0 + r) / a.group, kvh * a.group + (int)((t.row0 + r) % a.group), lane, 64);
+        return;
+    }
+    const int p = (int)qi + t.shift;
     const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
+    const Sees sees = row_sees(a, keys, p);
     // the wave's own rows
     const int wa = wave * 32 < last ? wave * 32 : last, wz = wave * 32 + 31 < last ? wave * 32 + 31 : last;
     const int wp0 = (int)((t.row0 + wa) / a.group) + t.shift, wp1 = (int)((t.row0 + wz) / a.group) + t.shift;
@@ -383,41 +428,63 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
     float m = -INFINITY, l = 0.f;
     const float c2 = a.c2;
-    const int n_steps = (keys.total + kKeys - 1) / kKeys;
+    const int all_steps = (keys.total + kKeys - 1) / kKeys;
+    const int per_split = (all_steps + splits - 1) / splits;
+    const int s0 = split * per_split, s1 = s0 + per_split < all_steps ? s0 + per_split : all_steps;
 
-    u32x4 kreg[PER], vreg[PER];
-    const auto load = [&](int j0) {
+    // piece i of a wave: LDS bytes [1024 (PER wave + i), + 1024) of a K or V tile, 16 per lane.  Features past the end of a
+    // row (dim < DP) are copied from its start: they meet zeros of q, or are never stored.
+    unsigned k_off[PER], v_off[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int x = tid + 256 * i, j = j0 + x / PIECES, d = x % PIECES * 8;
-            const bool in = j < keys.total;
-            const int key = keys.key(in ? j : keys.total - 1);
-            const int at = d < a.dim ? d : 0;
-            kreg[i] = *reinterpret_cast<const u32x4 *>(kb + key * a.kr.tok + at);
-            vreg[i] = *reinterpret_cast<const u32x4 *>(vb + key * a.vr.tok + at);
-            if (d >= a.dim) kreg[i] = u32x4{0, 0, 0, 0};
-            if (!in || (mask && !mask[key])) vreg[i] = u32x4{0, 0, 0, 0};   // 0 times what a masked key holds must stay 0
-        }
-    };
-    const auto store = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int x = tid + 256 * i, r = x / PIECES, c = x % PIECES;
-            *reinterpret_cast<u32x4 *>(&lds[buf][0][r * DP + 8 * k_piece<DP>(r, c)]) = kreg[i];
-            *reinterpret_cast<u32x4 *>(&lds[buf][1][r * DP + 8 * v_piece<DP>(r, c)]) = vreg[i];
-        }
-    };
-    if (n_steps > 0) {
-        load(0);
-        store(0);
+    for (int i = 0; i < PER; ++i) {
+        const int x = (PER * wave + i) * 64 + lane, r = x / PIECES, c = x % PIECES;
+        const int kd = 8 * k_piece<DP>(r, c), vd = 8 * v_piece<DP>(r, c);
+        k_off[i] = (unsigned)r * (unsigned)a.kr.tok + (kd < a.dim ? kd : 0);
+        v_off[i] = (unsigned)r * (unsigned)a.vr.tok + (vd < a.dim ? vd : 0);
     }
+    const auto load = [&](int step) {
+        const int j0 = step * kKeys;
+        T *lk = lds + (step & 1) * 2 * TILE + PER * wave * 512, *lv = lk + TILE;
+        if (j0 >= keys.sinks && j0 + kKeys <= keys.total) {     // 64 neighbouring keys
+            const T *k0 = kb + (int64_t)keys.key(j0) * a.kr.tok, *v0 = vb + (int64_t)keys.key(j0) * a.vr.tok;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                copy_to_lds(k0 + k_off[i], lk + 512 * i);
+                copy_to_lds(v0 + v_off[i], lv + 512 * i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int r = ((PER * wave + i) * 64 + lane) / PIECES, j = j0 + r;
+                const int64_t key = keys.key(j < keys.total ? j : keys.total - 1);
+                copy_to_lds(kb + (key - r) * a.kr.tok + k_off[i], lk + 512 * i);
+                copy_to_lds(vb + (key - r) * a.vr.tok + v_off[i], lv + 512 * i);
+            }
+        }
+    };
+    if (s0 < s1) load(s0);
     __syncthreads();
-    for (int step = 0; step < n_steps; ++step) {
+    for (int step = s0; step < s1; ++step) {
         const int j0 = step * kKeys, jz = j0 + kKeys - 1;
-        if (step + 1 < n_steps) load(j0 + kKeys);
-        const T *lk = lds[step & 1][0], *lv = lds[step & 1][1];
+        T *lk = lds + (step & 1) * 2 * TILE, *lv = lk + TILE;
         const int kmin = keys.key(j0), kmax = keys.key(jz < keys.total ? jz : keys.total - 1);
         const bool window_only = j0 >= keys.sinks;
+        uint64_t seen = ~0ull;                                 // inside the range and not masked
+        if (mask || jz >= keys.total) {
+            const int j = j0 + lane;
+            const bool in = j < keys.total;
+            seen = __ballot(in && (!mask || mask[keys.key(in ? j : keys.total - 1)] != 0));
+            if (mask && seen != ~0ull) {
+                // 0 times what a masked key holds must stay 0
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const int x = (PER * wave + i) * 64 + lane;
+                    if (!((seen >> (x / PIECES)) & 1)) *reinterpret_cast<u32x4 *>(lv + 8 * x) = u32x4{0, 0, 0, 0};
+                }
+                __syncthreads();
+            }
+        }
+        if (step + 1 < s1) load(step + 1);
         const bool none = wp1 < 0 || (window_only && (kmin > wp1 || (kmax < wlo0 && kmin >= a.sinks)));
         if (!none) {
             f32x16 s[2];
@@ -432,19 +499,17 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
                     s[u] = Mat<T>::mul32(kf, qf[c], s[u]);
                 }
             }
-            const bool full = !mask && window_only && jz < keys.total && kmax <= wp0 && kmin >= wlo1;
+            // a tile whose keys all rows of the wave see needs no mask: inside the range, unmasked, up to the first row's
+            // position, inside the last row's window
+            const bool full = seen == ~0ull && window_only && kmax <= wp0 && kmin >= wlo1;
             if (!full) {
-                const int j = j0 + lane;
-                const bool in = j < keys.total;
-                const uint64_t seen = __ballot(in && (!mask || mask[keys.key(in ? j : keys.total - 1)] != 0));
+                const uint64_t vis = sees.bits(j0) & seen;
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 2; ++u) {
+                    const unsigned w = (unsigned)(vis >> (32 * u)) >> (4 * h);
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int i = 32 * u + (r & 3) + 8 * (r >> 2) + 4 * h;
-                        const int key = keys.key(j0 + i);
-                        if (!(((seen >> i) & 1) && key <= p && (key >= lo || key < a.sinks))) s[u][r] = -INFINITY;
-                    }
+                    for (int r = 0; r < 16; ++r) s[u][r] = seen_or_inf(w, (r & 3) + 8 * (r >> 2), s[u][r]);
+                }
             }
             float top = -INFINITY;
 #pragma unroll
@@ -490,10 +555,24 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
                 }
             }
         }
-        if (step + 1 < n_steps) store((step + 1) & 1);
-        __syncthreads();
+        __syncthreads();                                       // the next tile has landed, this one is no longer read
     }
     l += other_half(l);
+    if (splits > 1) {
+        // joined by attn_window_join_kernel: this part's maximum, sum and numerators
+        const int64_t at = out_row * splits + split;
+        if (real && h == 0) { part_ml[2 * at] = m; part_ml[2 * at + 1] = l; }
+        if (real && m != -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int d = 32 * i + 8 * x + 4 * h;
+                    if (d < a.dim) *reinterpret_cast<f32x4 *>(part_o + at * a.dim + d) = f32x4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]};
+                }
+        }
+        return;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     bool bad = false;
 #pragma unroll
@@ -508,12 +587,12 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
         const uint64_t b = __ballot(bad && real);
         repair = (unsigned)(b | (b >> 32));
     }
-    T *out = reinterpret_cast<T *>(a.out) + ((t.q_beg + qi) * a.hq + head) * (int64_t)a.dim;
+    T *out = reinterpret_cast<T *>(a.out) + out_row * a.dim;
     const bool keep = real && !((repair >> n) & 1);
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {                      // 16 features: halves hold {0-3, 8-11} and {4-7, 12-15}
+        for (int x = 0; x < 2; ++x) {                          // 16 features: halves hold {0-3, 8-11} and {4-7, 12-15}
             unsigned w[2][2];
 #pragma unroll
             for (int y = 0; y < 2; ++y)
@@ -523,16 +602,70 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
                     Pack<T, 2> two = {{from_f32<T>(o[i][r]), from_f32<T>(o[i][r + 1])}};
                     w[y][z] = __builtin_bit_cast(unsigned, two);
                 }
-            const auto s0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            const int d = 32 * i + 16 * x + 8 * h;         // after the exchange a lane holds 8 neighbouring features
-            if (keep && d < a.dim) *reinterpret_cast<u32x4 *>(out + d) = u32x4{s0[0], s1[0], s0[1], s1[1]};
+            const auto w0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+            const auto w1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+            const int d = 32 * i + 16 * x + 8 * h;             // after the exchange a lane holds 8 neighbouring features
+            if (keep && d < a.dim) *reinterpret_cast<u32x4 *>(out + d) = u32x4{w0[0], w1[0], w0[1], w1[1]};
         }
     // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
     // Rows that came out not finite are formed again key by key.
     for (; repair; repair &= repair - 1) {
         const int64_t r = t.row0 + wave * 32 + __builtin_ctz(repair);
         row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+    }
+}
+
+// Joins the parts of a row: a wave per (token, query head).
+template <class T>
+__global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int splits, const float *__restrict__ part_o,
+                                                               const float *__restrict__ part_ml)
+{
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
+    if (row >= a.nq * a.hq) return;
+    const int d = 2 * lane;
+    float ms[kMaxSplits], ls[kMaxSplits], top = -INFINITY;
+    float2 ov[kMaxSplits];
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s) {
+        const int64_t at = row * splits + (s < splits ? s : 0);
+        ms[s] = s < splits ? part_ml[2 * at] : -INFINITY;
+        ls[s] = part_ml[2 * at + 1];
+        ov[s] = *reinterpret_cast<const float2 *>(part_o + at * a.dim + (d < a.dim ? d : 0));
+        top = fmaxf(top, ms[s]);
+    }
+    float sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+    for (int s = 0; s < kMaxSplits; ++s) {
+        if (ms[s] == -INFINITY) continue;                      // a part that saw nothing has no numerators
+        const float f = __builtin_amdgcn_exp2f(ms[s] - top);
+        sum = fmaf(f, ls[s], sum);
+        x = fmaf(f, ov[s].x, x);
+        y = fmaf(f, ov[s].y, y);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    x *= inv;
+    y *= inv;
+    const int64_t token = row / a.hq;
+    const int head = (int)(row % a.hq);
+    if (__ballot(d < a.dim && !(fabsf(x) < INFINITY && fabsf(y) < INFINITY))) {   // see the end of the tile kernel
+        int64_t lo = 0, hi = a.n_seq;                                             // last sequence that starts at or before token
+        while (lo + 1 < hi) {
+            const int64_t mid = (lo + hi) / 2;
+            if (clamp64(a.cu_q[mid], 0, a.nq) <= token) lo = mid;
+            else hi = mid;
+        }
+        int64_t q_beg, q_end, k_beg, k_end;
+        seq_range(a.cu_q, lo, a.nq, q_beg, q_end);
+        seq_range(a.cu_k, lo, a.nk, k_beg, k_end);
+        if (token >= q_beg && token < q_end)
+            row_by_wave<T>(a, k_beg, token - q_beg + (k_end - k_beg) - (q_end - q_beg), token, head, lane);
+        return;
+    }
+    if (d < a.dim) {
+        Pack<T, 2> two = {{from_f32<T>(x), from_f32<T>(y)}};
+        *reinterpret_cast<Pack<T, 2> *>(reinterpret_cast<T *>(a.out) + row * a.dim + d) = two;
     }
 }
 
@@ -546,18 +679,40 @@ int launch_direct(const Args &a, hipStream_t s)
     return QCN_OK;
 }
 
-template <class T, int DP>
-int launch_tile(const Args &a, hipStream_t s)
+// Blocks of the 128-row kernel for one part of the keys, and the parts: 2 blocks fit a CU, and a launch wants several rounds of
+// them.  A part keeps at least 8 key tiles.  Sizes only: lengths are on the device.
+int plan_splits(const Args &a)
 {
-    const int64_t tiles = (a.nq * a.group >> kRowShift) + a.n_seq + 1, blocks = tiles * a.hk;
+    if (a.dim <= 16) return 1;
+    const int64_t blocks = ((a.nq * a.group >> kRowShift) + a.n_seq + 1) * a.hk, want = 4 * (int64_t)qcn_num_cus();
+    int64_t reach = a.window + a.sinks + 128 / a.group;
+    if (reach > a.nk) reach = a.nk;
+    int64_t s = (want + blocks - 1) / blocks;
+    if (s > reach / (8 * kKeys)) s = reach / (8 * kKeys);
+    if (s > kMaxSplits) s = kMaxSplits;
+    return s < 1 ? 1 : (int)s;
+}
+
+template <class T, int DP>
+int launch_tile(const Args &a, void *workspace, int64_t workspace_bytes, hipStream_t s)
+{
+    const int splits = plan_splits(a);
+    const int64_t rows = a.nq * a.hq * splits;
+    if (splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rows * (a.dim + 2) * 4)) return QCN_ERR_WORKSPACE_TOO_SMALL;
+    const int64_t tiles = (a.nq * a.group >> kRowShift) + a.n_seq + 1, blocks = tiles * a.hk * splits;
     if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((attn_window_tile_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles);
+    float *part_o = reinterpret_cast<float *>(workspace), *part_ml = splits > 1 ? part_o + rows * a.dim : nullptr;
+    hipLaunchKernelGGL((attn_window_tile_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles, splits, part_o, part_ml);
     QCN_CHECK_LAUNCH();
+    if (splits > 1) {
+        hipLaunchKernelGGL(attn_window_join_kernel<T>, dim3((unsigned)((a.nq * a.hq + 3) / 4)), dim3(256), 0, s, a, splits, part_o, part_ml);
+        QCN_CHECK_LAUNCH();
+    }
     return QCN_OK;
 }
 
 template <class T>
-int launch(const Args &a, hipStream_t s)
+int launch(const Args &a, void *ws, int64_t ws_bytes, hipStream_t s)
 {
     if constexpr (sizeof(T) == 4) {
         if (a.dim <= 16) return launch_direct<T, 16>(a, s);
@@ -567,14 +722,26 @@ int launch(const Args &a, hipStream_t s)
         return launch_direct<T, 128>(a, s);
     } else {
         if (a.dim <= 16) return launch_direct<T, 16>(a, s);
-        if (a.dim <= 32) return launch_tile<T, 32>(a, s);
-        if (a.dim <= 64) return launch_tile<T, 64>(a, s);
-        if (a.dim <= 96) return launch_tile<T, 96>(a, s);
-        return launch_tile<T, 128>(a, s);
+        if (a.dim <= 32) return launch_tile<T, 32>(a, ws, ws_bytes, s);
+        if (a.dim <= 64) return launch_tile<T, 64>(a, ws, ws_bytes, s);
+        if (a.dim <= 96) return launch_tile<T, 96>(a, ws, ws_bytes, s);
+        return launch_tile<T, 128>(a, ws, ws_bytes, s);
     }
 }
 
 }  // namespace
+
+extern "C" int64_t qcn_attn_window_workspace_bytes(const qcn_attn_window_args *args)
+{
+    if (!args || args->dtype == QCN_DTYPE_F32 || args->n_q_tokens < 1 || args->n_kv_heads < 1 || args->n_q_heads < args->n_kv_heads) return 0;
+    Args a = {};
+    a.nq = args->n_q_tokens; a.nk = args->n_k_tokens; a.n_seq = args->n_seq; a.hk = (int)args->n_kv_heads;
+    a.group = (int)(args->n_q_heads / args->n_kv_heads); a.dim = (int)args->dim;
+    a.window = args->window < kMost ? args->window : kMost;
+    a.sinks = args->sinks < kMost ? args->sinks : kMost;
+    const int splits = plan_splits(a);
+    return splits > 1 ? a.nq * args->n_q_heads * splits * (a.dim + 2) * (int64_t)sizeof(float) : 0;
+}
 
 extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
 {
@@ -583,8 +750,9 @@ extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
     if (x.n_seq < 0 || x.n_q_tokens < 0 || x.n_k_tokens < 0 || x.n_q_heads < 1 || x.n_kv_heads < 1 || x.n_q_heads % x.n_kv_heads ||
         x.window < 1 || x.sinks < 0 || !(x.scale >= 0.) || x.scale > 3.0e38 || !dtype_known(x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
-    const int64_t most = ((int64_t)1 << 31) - 1;
-    if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.n_q_tokens > most || x.n_k_tokens > most || x.n_seq > most)
+    const int64_t most = kMost;
+    if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.n_q_tokens > most || x.n_k_tokens > most || x.n_seq > most ||
+        x.k_strides[0] >= kMaxTokStride || x.v_strides[0] >= kMaxTokStride)
         return QCN_ERR_UNSUPPORTED;
     if (x.n_q_tokens == 0) return QCN_OK;
     if (!x.q || !x.out || !x.cu_q || !x.cu_k || (x.n_k_tokens && (!x.k || !x.v))) return QCN_ERR_INVALID_ARGUMENT;
@@ -601,8 +769,8 @@ extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
                     fmaxf((float)x.scale * kLog2e, 1e-37f), x.out};
     hipStream_t s = qcn_stream(stream);
     switch (x.dtype) {
-    case QCN_DTYPE_F32: return launch<float>(a, s);
-    case QCN_DTYPE_F16: return launch<_Float16>(a, s);
-    default: return launch<__bf16>(a, s);
+    case QCN_DTYPE_F32: return launch<float>(a, x.workspace, x.workspace_bytes, s);
+    case QCN_DTYPE_F16: return launch<_Float16>(a, x.workspace, x.workspace_bytes, s);
+    default: return launch<__bf16>(a, x.workspace, x.workspace_bytes, s);
     }
 }

@@ -25,7 +25,8 @@ struct Rows {
     int64_t tok, head;   // strides in elements
 };
 
-constexpr int64_t kMaxHeads = 32767;   // of one tensor
+constexpr int64_t kMaxHeads = 32767;            // of one tensor
+constexpr int64_t kMaxTokStride = (int64_t)1 << 24;   // elements: 64 rows' offsets are 32-bit
 
 // rows are loaded in 16-byte pieces
 static inline bool rows_aligned(const void *p, int64_t tok, int64_t head, int64_t dtype)

@@ -27,10 +27,11 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}          # QCN
 _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}            # QCN_POS_*
 MAX_HEAD_DIM = 128
 _MOST = (1 << 62) - 1
+_MOST_TOK = 1 << 24      # token stride in elements
 
 # the argument structs of include/qcnet_hip.h (8-byte fields: no padding)
 _ROTARY_ARGS = struct.Struct('=27q').pack
-_WINDOW_ARGS = struct.Struct('=21qdq').pack
+_WINDOW_ARGS = struct.Struct('=21qd3q').pack
 _APPEND_ARGS = struct.Struct('=19q').pack
 _STEP_ARGS = struct.Struct('=18qd6q').pack
 
@@ -68,7 +69,7 @@ def _rows(t: torch.Tensor, name: str, dtype: torch.dtype, device: torch.device) 
 def _in_place(t: torch.Tensor):
     """(t, its strides) when its rows can be read in 16-byte pieces, else of a contiguous copy."""
     tok, head, feat = strides = t.stride()
-    if feat == 1 and (tok | head) % (16 // t.element_size()) == 0 and t.data_ptr() % 16 == 0:
+    if feat == 1 and (tok | head) % (16 // t.element_size()) == 0 and tok < _MOST_TOK and t.data_ptr() % 16 == 0:
         return t, strides
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride()
@@ -82,14 +83,17 @@ def _dtype_code(t: torch.Tensor, name: str) -> int:
     return _DTYPES[t.dtype]
 
 
-def _launch(index: int, what: str, args: bytes) -> None:
-    """One C ABI call on the tensors' own device and its current stream."""
-    fn = getattr(_lib.lib(), what)
+def _on_device(index: int, fn, *args):
+    """One C ABI call with the tensors' own device current."""
     if torch._C._cuda_getDevice() == index:
-        status = fn(args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(args, torch._C._cuda_getCurrentRawStream(index))
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _launch(index: int, what: str, args: bytes) -> None:
+    """A launch on the tensors' own device and its current stream."""
+    status = _on_device(index, getattr(_lib.lib(), what), args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, what)
 
@@ -247,9 +251,14 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
     v, vs = _in_place(v)
     out = q.new_empty((nq, hq, dim))
     if nq:
-        _launch(index, 'qcn_attn_window', _WINDOW_ARGS(
-            q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
-            n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr()))
+        args = (q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
+                n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr())
+        packed = _WINDOW_ARGS(*args, 0, 0)
+        ws_bytes = _on_device(index, _lib.lib().qcn_attn_window_workspace_bytes, packed)
+        if ws_bytes:
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=k.device)
+            packed = _WINDOW_ARGS(*args, ws.data_ptr(), ws_bytes)
+        _launch(index, 'qcn_attn_window', packed)
     return out
 
 
@@ -360,7 +369,7 @@ def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_
     v, vs = _in_place(v)
     out = q.new_empty((batch, hq, dim))
     if batch:
-        ws_bytes = _lib.lib().qcn_attn_window_step_workspace_bytes(batch, hq, hk, dim, window, sinks)
+        ws_bytes = _on_device(index, _lib.lib().qcn_attn_window_step_workspace_bytes, batch, hq, hk, dim, window, sinks)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=k.device) if ws_bytes else None
         _launch(index, 'qcn_attn_window_step', _STEP_ARGS(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], lengths.data_ptr(), mask_ptr, batch, hq,

@@ -136,6 +136,10 @@ CASES = [
     ([20, 30], [-7, -30], 2, 1, 32, 6, 2, False),          # fewer keys than queries: the first rows stand before the first key
     ([70], [200], 2, 1, 48, 1 << 50, 1 << 50, False),
     ([66, 66], None, 1, 1, 24, 2, 65, False),
+    # few queries behind long prefixes: the keys are split over blocks and joined
+    ([9, 1, 0, 30], [2100, 1500, 64, 0], 2, 1, 64, 1400, 3, False),
+    ([1], [3000], 5, 1, 128, 4000, 0, True),
+    ([17], [4200], 1, 1, 32, 4100, 70, True),
 ]
 
 
@@ -211,6 +215,28 @@ def test_window_ignores_what_masked_and_unseen_places_hold(dim, hq, hk, dtype):
             assert bool(((got.double() - w2[0]).abs() <= tol)[keep].all())
         else:
             assert bool(torch.isfinite(got[~sees]).all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_window_split_over_blocks_with_rows_behind_and_unseen_infinities(dtype):
+    lens, extra, hq, hk, dim = [20, 6], [2500, 1100], 2, 1, 64
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hk, dim, dtype, True, seed=8)
+    behind = 5
+    qq = torch.cat([q, torch.ones(behind, hq, dim, dtype=dtype)])
+    want = ref.window(q, k, v, cu_q, 2200, 2, cu_k, mask)
+    vv = v.clone()
+    vv[~mask] = float('nan')
+    last = int(cu_k[1]) - 3                                    # seen by the first sequence's last three queries only
+    mask2 = mask.clone()
+    mask2[last] = True
+    vv[last] = float('inf')
+    got = ops.attn_window(*_dev(qq, k, vv, cu_q), 2200, 2, cu_k=cu_k.to(DEV), key_mask=mask2.to(DEV)).cpu().double()
+    assert bool((got[26:] == 0).all())
+    keep = torch.ones(26, dtype=torch.bool)
+    keep[17:20] = False
+    assert not bool(torch.isfinite(got[17:20]).any())
+    tol = ref.tolerance(dtype, dim, *want, float(v.double().abs().max()))
+    assert bool(((got[:26] - want[0]).abs() <= tol)[keep].all())
 
 
 @pytest.mark.parametrize('dtype', DTYPES)

@@ -41,15 +41,18 @@ def _call(lib, name, fmt, fields, **over):
 def test_window_entry_point_refusals():
     lib = _lib.lib()
     fields = dict(q=FAKE, qs=(32, 16), k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu_q=FAKE, cu_k=FAKE, mask=0, n_seq=1, nq=4, nk=4, hq=2,
-                  hk=2, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE)
-    call = lambda **over: _call(lib, 'qcn_attn_window', '21qdq', fields, **over)
+                  hk=2, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE, ws=0, ws_bytes=0)
+    call = lambda **over: _call(lib, 'qcn_attn_window', '21qd3q', fields, **over)
     for bad in (dict(hq=3), dict(hq=0), dict(hk=0), dict(n_seq=-1), dict(nq=-1), dict(nk=-1), dict(window=0), dict(sinks=-1), dict(dtype=3),
                 dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf')), dict(q=0), dict(k=0), dict(v=0), dict(cu_q=0),
                 dict(cu_k=0), dict(out=0), dict(q=FAKE + 4), dict(k=FAKE + 8), dict(qs=(33, 16)), dict(vs=(32, 2)), dict(out=FAKE + 4)):
         assert call(**bad) == INVALID, bad
-    for bad in (dict(dim=20), dict(dim=136), dict(dim=0), dict(nq=1 << 31), dict(nk=1 << 31), dict(n_seq=1 << 31), dict(hq=1 << 16)):
+    for bad in (dict(dim=20), dict(dim=136), dict(dim=0), dict(nq=1 << 31), dict(nk=1 << 31), dict(n_seq=1 << 31), dict(hq=1 << 16),
+                dict(ks=(1 << 24, 16))):
         assert call(**bad) == UNSUPPORTED, bad
     assert call(nq=0) == 0
+    # 32 queries behind 8192 keys: split over blocks, which takes a workspace
+    assert call(dtype=2, dim=64, qs=(128, 64), ks=(128, 64), vs=(128, 64), nq=32, nk=8192, window=4096) == WORKSPACE
     assert lib.qcn_attn_window(None, None) == INVALID
 
 
