@@ -6,6 +6,8 @@
 // Hkv key heads are shared by Hq / Hkv query heads each.
 #include "sequence.hip.h"
 
+#include <type_traits>
+
 namespace {
 
 using namespace qcn_seq;
@@ -349,28 +351,46 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
 //
 // With few blocks (a short chunk of queries behind a long prefix) the key tiles are split over blocks as well and joined by a
 // second kernel.
-template <int DP> __device__ __forceinline__ int k_piece(int row, int piece)
+template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
-    return piece ^ (DP == 128 ? row & 15 : DP == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
+    return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
 }
-template <int DP> __device__ __forceinline__ int v_piece(int row, int piece)
+template <int LS> __device__ __forceinline__ int v_piece(int row, int piece)
 {
-    return piece ^ (DP == 128 ? (row & 3) << 2 : DP == 64 ? ((row >> 1) & 1) << 2 : 0);
+    return piece ^ (LS == 128 ? (row & 3) << 2 : LS == 64 ? ((row >> 1) & 1) << 2 : 0);
 }
 
 constexpr int64_t kMost = ((int64_t)1 << 31) - 1;   // positions are 32-bit
 constexpr int kRowShift = 7, kKeys = 64, kMaxSplits = 8;
 
-__device__ __forceinline__ void copy_to_lds(const void *src, void *dst)
+// 64 x 16 bytes, lane's own source, to LDS bytes dst .. dst + 1023 (dst the same in the wave).  Written out, and not as the builtin:
+// the compiler takes every transposing read for a possible reader of every copy in flight and waits for all of them; the copies
+// of a step belong to the NEXT step's tiles, and copies_landed() at that step's barrier is the wait they need.
+__device__ __forceinline__ void copy_to_lds(const void *base, uint32_t offset, uint32_t dst)
 {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src, (__attribute__((address_space(3))) void *)dst,
-                                     16, 0, 0);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void copy_to_lds(const void *src, uint32_t dst)
+{
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory");
+}
+
+__device__ __forceinline__ void copies_landed()
+{
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void *p)
+{
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
 }
 
 template <class T, int DP>
 __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_t n_tiles, int splits, float *part_o, float *part_ml)
 {
-    constexpr int PIECES = DP / 8, PER = DP / 32, NK = DP / 16, ND = DP / 32, TILE = kKeys * DP;
+    constexpr int LS = DP == 96 ? 128 : DP;                    // elements of an LDS row
+    constexpr int PIECES = LS / 8, PER = LS / 32, NK = DP / 16, ND = DP / 32, TILE = kKeys * LS;
     using V8 = typename Mat<T>::V8;
     __shared__ __attribute__((aligned(16))) T lds[4 * TILE];   // K, V of one buffer, K, V of the other
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
@@ -426,137 +446,189 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, l2 = 0.f;                    // two chains of the sum
     const float c2 = a.c2;
     const int all_steps = (keys.total + kKeys - 1) / kKeys;
     const int per_split = (all_steps + splits - 1) / splits;
     const int s0 = split * per_split, s1 = s0 + per_split < all_steps ? s0 + per_split : all_steps;
 
-    // piece i of a wave: LDS bytes [1024 (PER wave + i), + 1024) of a K or V tile, 16 per lane.  Features past the end of a
-    // row (dim < DP) are copied from its start: they meet zeros of q, or are never stored.
-    unsigned k_off[PER], v_off[PER];
+    // tiles alternate between two buffers, counted from the first step
+    const auto buffer = [&](int parity, int kv) { return lds + (parity * 2 + kv) * TILE; };
+    // Copy i of a wave fills 1024 LDS bytes in order, 16 per lane.  Features past the end of a row (dim < DP) are copied from its
+    // start: they meet zeros of q, or are never stored.
+    const T *k_window = kb + (int64_t)(keys.start - keys.sinks) * a.kr.tok, *v_window = vb + (int64_t)(keys.start - keys.sinks) * a.vr.tok;
+    const int r0 = lane / PIECES, slot = lane % PIECES;
+    const auto piece = [&](int i, auto want_v) {                // first feature of the lane's 16 bytes
+        const int r = (PER * wave + i) * (64 / PIECES) + r0;
+        const int d = 8 * (decltype(want_v)::value ? v_piece<LS>(r, slot) : k_piece<LS>(r, slot));
+        return d;
+    };
+    uint32_t k_off[PER], v_off;                                 // bytes; V pieces do not depend on i
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        const int x = (PER * wave + i) * 64 + lane, r = x / PIECES, c = x % PIECES;
-        const int kd = 8 * k_piece<DP>(r, c), vd = 8 * v_piece<DP>(r, c);
-        k_off[i] = (unsigned)r * (unsigned)a.kr.tok + (kd < a.dim ? kd : 0);
-        v_off[i] = (unsigned)r * (unsigned)a.vr.tok + (vd < a.dim ? vd : 0);
+        const int d = piece(i, std::false_type{});
+        k_off[i] = ((uint32_t)r0 * (uint32_t)a.kr.tok + (d < a.dim ? d : 0)) * (uint32_t)sizeof(T);
     }
-    const auto load = [&](int step) {
+    {
+        const int d = piece(0, std::true_type{});
+        v_off = ((uint32_t)r0 * (uint32_t)a.vr.tok + (d < a.dim ? d : 0)) * (uint32_t)sizeof(T);
+    }
+    const auto load = [&](int step, int parity, auto want_v) {
+        constexpr bool V = decltype(want_v)::value;
         const int j0 = step * kKeys;
-        T *lk = lds + (step & 1) * 2 * TILE + PER * wave * 512, *lv = lk + TILE;
+        const uint32_t dst = lds_address(buffer(parity, V) + PER * wave * 512);
+        const int64_t tok = V ? a.vr.tok : a.kr.tok;
         if (j0 >= keys.sinks && j0 + kKeys <= keys.total) {     // 64 neighbouring keys
-            const T *k0 = kb + (int64_t)keys.key(j0) * a.kr.tok, *v0 = vb + (int64_t)keys.key(j0) * a.vr.tok;
+            const T *x = (V ? v_window : k_window) + (int64_t)(j0 + PER * wave * (64 / PIECES)) * tok;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                copy_to_lds(k0 + k_off[i], lk + 512 * i);
-                copy_to_lds(v0 + v_off[i], lv + 512 * i);
-            }
+            for (int i = 0; i < PER; ++i, x += 64 / PIECES * tok)
+                if (DP == LS || piece(i, want_v) < DP) copy_to_lds(x, V ? v_off : k_off[i], dst + 1024 * i);
         } else {
+            const T *src = V ? vb : kb;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const int r = ((PER * wave + i) * 64 + lane) / PIECES, j = j0 + r;
-                const int64_t key = keys.key(j < keys.total ? j : keys.total - 1);
-                copy_to_lds(kb + (key - r) * a.kr.tok + k_off[i], lk + 512 * i);
-                copy_to_lds(vb + (key - r) * a.vr.tok + v_off[i], lv + 512 * i);
+                const int d = piece(i, want_v), j = j0 + (PER * wave + i) * (64 / PIECES) + r0;
+                const int jc = j < keys.total ? j : keys.total - 1;
+                if (DP == LS || d < DP) copy_to_lds(src + keys.key(jc) * tok + (d < a.dim ? d : 0), dst + 1024 * i);
             }
         }
     };
-    if (s0 < s1) load(s0);
-    __syncthreads();
-    for (int step = s0; step < s1; ++step) {
-        const int j0 = step * kKeys, jz = j0 + kKeys - 1;
-        T *lk = lds + (step & 1) * 2 * TILE, *lv = lk + TILE;
-        const int kmin = keys.key(j0), kmax = keys.key(jz < keys.total ? jz : keys.total - 1);
-        const bool window_only = j0 >= keys.sinks;
-        uint64_t seen = ~0ull;                                 // inside the range and not masked
-        if (mask || jz >= keys.total) {
-            const int j = j0 + lane;
-            const bool in = j < keys.total;
-            seen = __ballot(in && (!mask || mask[keys.key(in ? j : keys.total - 1)] != 0));
-            if (mask && seen != ~0ull) {
+    // Tiles that any row of the wave sees: those of the sinks, below es, and those of the window, ea .. eb - 1; tiles whose keys all
+    // its rows see: f0 .. f1 - 1.  As numbers once, because the loop's scalar instructions are not free.
+    const int to_j = keys.sinks - keys.start;                  // window key + to_j = its index
+    int es = 0, ea = 0, eb = 0, f0 = 0, f1 = 0;
+    if (wp1 >= 0) {
+        const int sinks = a.sinks < (int64_t)wp1 + 1 ? (int)a.sinks : wp1 + 1;
+        es = (sinks + kKeys - 1) / kKeys;
+        ea = (wlo0 + to_j) / kKeys;
+        eb = (wp1 + to_j) / kKeys + 1;
+        const int fa = wlo1 + to_j > keys.sinks ? wlo1 + to_j : keys.sinks, fb = wp0 + to_j + 1 < keys.total ? wp0 + to_j + 1 : keys.total;
+        f0 = (fa + kKeys - 1) / kKeys;
+        f1 = mask || wp0 < 0 ? 0 : fb / kKeys;
+    }
+    // of 64 keys from j0 on, those inside the range and not masked (the same in every wave)
+    const auto seen_keys = [&](int j0) {
+        const int j = j0 + lane;
+        const bool in = j < keys.total;
+        return (uint64_t)__ballot(in && (!mask || mask[keys.key(in ? j : 0)] != 0));
+    };
+    // O^T += V^T P^T, a k-step (16 keys) at a time; its V operands are read a k-step ahead and the next one's exponentials fill
+    // the time of its products.  The order is spelled out for the scheduler, which otherwise puts every LDS read right in front of
+    // the product that waits for it.
+    const auto run_step = [&](int step, auto parity) {
+        constexpr int P = decltype(parity)::value;
+        copies_landed();                                       // this step's tiles are in LDS, the other buffers are free
+        uint64_t seen = ~0ull;
+        if (mask) {
+            seen = seen_keys(step * kKeys);
+            if (seen != ~0ull) {
                 // 0 times what a masked key holds must stay 0
 #pragma unroll
                 for (int i = 0; i < PER; ++i) {
                     const int x = (PER * wave + i) * 64 + lane;
-                    if (!((seen >> (x / PIECES)) & 1)) *reinterpret_cast<u32x4 *>(lv + 8 * x) = u32x4{0, 0, 0, 0};
+                    if (!((seen >> (x / PIECES)) & 1)) *reinterpret_cast<u32x4 *>(buffer(P, 1) + 8 * x) = u32x4{0, 0, 0, 0};
                 }
                 __syncthreads();
             }
         }
-        if (step + 1 < s1) load(step + 1);
-        const bool none = wp1 < 0 || (window_only && (kmin > wp1 || (kmax < wlo0 && kmin >= a.sinks)));
-        if (!none) {
-            f32x16 s[2];
+        if (step + 1 < s1) {
+            load(step + 1, P ^ 1, std::false_type{});
+            load(step + 1, P ^ 1, std::true_type{});
+        }
+        if (!(step < es || (step >= ea && step < eb))) return;
+        const T *lk = buffer(P, 0), *lv = buffer(P, 1);
+        const int i16 = lane & 15;
+        V8 kf[NK], vf[2][ND], pb[4];
+        f32x16 s[2];
+        const auto read_k = [&](int u, int c) {
+            const int kr = 32 * u + n;
+            kf[c] = *reinterpret_cast<const V8 *>(&lk[kr * LS + 8 * k_piece<LS>(kr, 2 * c + h)]);
+        };
+        const auto read_v = [&](int k, int dt) {               // k-step k: 16 keys; 32 features
+            const int vr = 16 * k + 4 * h + (i16 >> 2), d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+            const uint2 x = lds_read_transposed(&lv[vr * LS + 8 * v_piece<LS>(vr, d >> 3) + (d & 7)]);
+            const uint2 y = lds_read_transposed(&lv[(vr + 8) * LS + 8 * v_piece<LS>(vr + 8, d >> 3) + (d & 7)]);
+            vf[k & 1][dt] = __builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y});
+        };
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[0][r] = s[1][r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) read_k(0, c);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            s[0] = Mat<T>::mul32(kf[c], qf[c], s[0]);
+            read_k(1, c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            s[1] = Mat<T>::mul32(kf[c], qf[c], s[1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) read_v(0, dt);
+        if (!(step >= f0 && step < f1)) {                      // scores of what a row does not see
+            const uint64_t vis = sees.bits(step * kKeys) & seen;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
+                const unsigned w = (unsigned)(vis >> (32 * u)) >> (4 * h);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
-#pragma unroll
-                for (int c = 0; c < NK; ++c) {
-                    const int kr = 32 * u + n;
-                    const V8 kf = *reinterpret_cast<const V8 *>(&lk[kr * DP + 8 * k_piece<DP>(kr, 2 * c + h)]);
-                    s[u] = Mat<T>::mul32(kf, qf[c], s[u]);
-                }
-            }
-            // a tile whose keys all rows of the wave see needs no mask: inside the range, unmasked, up to the first row's
-            // position, inside the last row's window
-            const bool full = seen == ~0ull && window_only && kmax <= wp0 && kmin >= wlo1;
-            if (!full) {
-                const uint64_t vis = sees.bits(j0) & seen;
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const unsigned w = (unsigned)(vis >> (32 * u)) >> (4 * h);
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[u][r] = seen_or_inf(w, (r & 3) + 8 * (r >> 2), s[u][r]);
-                }
-            }
-            float top = -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-            top = fmaxf(top, other_half(top));
-            // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
-            const float scaled = top * c2;
-            if (__ballot(scaled > m + 8.f)) {
-                const float mn = scaled > m ? scaled : m;
-                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < ND; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
-                m = mn;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    V8 pb;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        l += s[u][8 * ks + i];
-                        pb[i] = from_f32<T>(s[u][8 * ks + i]);
-                    }
-                    const int i16 = lane & 15, vr = 32 * u + 16 * ks + 4 * h + (i16 >> 2);
-#pragma unroll
-                    for (int dt = 0; dt < ND; ++dt) {
-                        const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-                        const uint2 x = lds_read_transposed(&lv[vr * DP + 8 * v_piece<DP>(vr, d >> 3) + (d & 7)]);
-                        const uint2 y = lds_read_transposed(&lv[(vr + 8) * DP + 8 * v_piece<DP>(vr + 8, d >> 3) + (d & 7)]);
-                        o[dt] = Mat<T>::mul32(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
-                    }
-                }
+                for (int r = 0; r < 16; ++r) s[u][r] = seen_or_inf(w, (r & 3) + 8 * (r >> 2), s[u][r]);
             }
         }
-        __syncthreads();                                       // the next tile has landed, this one is no longer read
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top[r & 3] = fmaxf(fmaxf(top[r & 3], s[0][r]), s[1][r]);
+        top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // the running maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+        const float scaled = fmaxf(top[0], other_half(top[0])) * c2;
+        if (__ballot(scaled > m + 8.f)) {
+            const float mn = scaled > m ? scaled : m;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+            l *= alpha;
+            l2 *= alpha;
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        const auto exponentials = [&](int k, int first, int end) {
+#pragma unroll
+            for (int i = first; i < end; ++i)
+                pb[k][i] = from_f32<T>(__builtin_amdgcn_exp2f(fmaf(s[k >> 1][8 * (k & 1) + i], c2, -base)));
+        };
+        exponentials(0, 0, 8);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int dt = 0; dt < ND; ++dt) {
+                __builtin_amdgcn_sched_barrier(0);
+                o[dt] = Mat<T>::mul32(vf[k & 1][dt], pb[k], o[dt]);
+                if (k < 3) {
+                    read_v(k + 1, dt);
+                    exponentials(k + 1, dt * 8 / ND, (dt + 1) * 8 / ND);
+                }
+                // the sum, of the rounded p that O sums too
+#pragma unroll
+                for (int i = dt * 4 / ND; i < (dt + 1) * 4 / ND; ++i) {
+                    if (k & 1) l2 = Mat<T>::add_pair(pb[k], i, l2);
+                    else l = Mat<T>::add_pair(pb[k], i, l);
+                }
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    if (s0 < s1) {
+        load(s0, 0, std::false_type{});
+        load(s0, 0, std::true_type{});
+        for (int step = s0; step < s1; step += 2) {
+            run_step(step, std::integral_constant<int, 0>{});
+            if (step + 1 < s1) run_step(step + 1, std::integral_constant<int, 1>{});
+        }
     }
+    l += l2;
     l += other_half(l);
     if (splits > 1) {
         // joined by attn_window_join_kernel: this part's maximum, sum and numerators

@@ -112,6 +112,12 @@ template <> struct Mat<_Float16> {
     using V8 = f16x8;
     using V4 = __attribute__((ext_vector_type(4))) _Float16;
     static __device__ __forceinline__ f32x16 mul32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    // c + x[2 i] + x[2 i + 1], products with 1 in fp32
+    static __device__ __forceinline__ float add_pair(V8 x, int i, float c)
+    {
+        using V2 = __attribute__((ext_vector_type(2))) _Float16;
+        return __builtin_amdgcn_fdot2(V2{x[2 * i], x[2 * i + 1]}, V2{(_Float16)1.f, (_Float16)1.f}, c, false);
+    }
     static __device__ __forceinline__ f32x4 mul16(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mul16(V4 a, V4 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 };
@@ -120,6 +126,11 @@ template <> struct Mat<__bf16> {
     using V4 = __attribute__((ext_vector_type(4))) __bf16;
     using S4 = __attribute__((ext_vector_type(4))) short;
     static __device__ __forceinline__ f32x16 mul32(V8 a, V8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ float add_pair(V8 x, int i, float c)
+    {
+        using V2 = __attribute__((ext_vector_type(2))) __bf16;
+        return __builtin_amdgcn_fdot2_f32_bf16(V2{x[2 * i], x[2 * i + 1]}, V2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    }
     static __device__ __forceinline__ f32x4 mul16(V8 a, V8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ f32x4 mul16(V4 a, V4 b, f32x4 c)
     {
