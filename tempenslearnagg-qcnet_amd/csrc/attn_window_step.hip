@@ -73,7 +73,7 @@ struct StepArgs {
 };
 
 // A task is a cache row, a key head, up to 16 of the query heads that share it, and a part of the filled slots.  Its waves take
-// chunks of 32 slots in turn:  S^T (slots x heads) = K Q^T, O^T (features x heads) = V^T P^T with 16 x 16 accumulators, so that a
+// chunks of 32 or 64 slots in turn:  S^T (slots x heads) = K Q^T, O^T (features x heads) = V^T P^T with 16 x 16 accumulators, so that a
 // shared key head is read once for its whole group.
 //
 // HBM-bound: every filled slot is read once.  K goes straight into registers as the A operand (a lane reads 16 bytes of a slot,
@@ -82,12 +82,14 @@ struct StepArgs {
 // The new token is read from the inputs, never from its slot, which another block of this launch is writing.
 template <class T, int DP> struct Step {
     static constexpr bool F32 = sizeof(T) == 4;
-    static constexpr int CHUNK = 32, NT = DP / 16;
+    static constexpr int NU = DP <= 32 ? 4 : 2, CHUNK = 16 * NU;                        // slots of a chunk: narrow heads take 64
     static constexpr int VW = !F32 ? 1 : (DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1));   // float32: features of a lane's V load
     static constexpr int SB = 16 * VW, NSB = DP / SB;
     static constexpr int PIECES = DP / 8;                 // 16-bit: 16-byte pieces of a row
     static constexpr int O_STRIDE = DP + 4;               // floats: a row's pad keeps 16 heads off one bank
-    static constexpr int WAVE_BYTES = 64 * O_STRIDE;      // 32 rows of V, then 16 rows of O
+    static constexpr int V_BYTES = F32 ? 0 : CHUNK * DP * 2, O_BYTES = 64 * O_STRIDE;   // a chunk of V, then 16 rows of O
+    static constexpr int WAVE_BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
+    static constexpr bool V_AHEAD = F32 && DP <= 32;      // float32: V is requested with K where registers allow
 };
 
 // 8 rows x 32 bytes of a transposing read (half a wave) cover all banks
@@ -139,29 +141,42 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
             c = c < t.c1 ? c : t.c1 - 1;
             return c == t.slot ? fresh : cache + c * a.dim;
         };
-        u32x4 kf[2][NQ];
+        u32x4 kf[L::NU][NQ];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < L::NU; ++u) {
             const T *row = row_of(kc, kn, 16 * u + n);
 #pragma unroll
             for (int c = 0; c < NQ; ++c) kf[u][c] = piece(row, L::F32 ? 16 * c + 4 * g : 32 * c + 8 * g);
         }
-        const int64_t cl = j0 + (lane & 31);
-        const bool in = cl < t.c1;
+        const int64_t cl = j0 + lane;
+        const bool in = lane < L::CHUNK && cl < t.c1;
         const bool ok = in && (cl == t.slot ? new_seen : (!mask || mask[in ? cl : t.c1 - 1] != 0));
-        const unsigned seen = (unsigned)__ballot(ok);
-        constexpr int NV = L::F32 ? 1 : (32 * L::PIECES + 63) / 64;
+        constexpr int NV = L::F32 ? 1 : (L::CHUNK * L::PIECES + 63) / 64;
         u32x4 vf[NV];
+        using PV = Pack<T, L::VW>;
+        PV va[L::V_AHEAD ? L::NU : 1][L::NSB][4];
+        const auto load_v = [&](int u, int sb, int r) {        // float32: VW features of slot 16 u + 4 g + r
+            const int d = sb * L::SB + L::VW * n;
+            return *reinterpret_cast<const PV *>(row_of(vc, vn, 16 * u + 4 * g + r) + (d < a.dim ? d : 0));
+        };
         if constexpr (!L::F32) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int x = lane + 64 * i, r = x / L::PIECES;
                 vf[i] = piece(row_of(vc, vn, r), x % L::PIECES * 8);
             }
-        }
-        f32x4 s[2];
+        } else if constexpr (L::V_AHEAD) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < L::NU; ++u)
+#pragma unroll
+                for (int sb = 0; sb < L::NSB; ++sb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) va[u][sb][r] = load_v(u, sb, r);
+        }
+        const uint64_t seen = __ballot(ok);
+        f32x4 s[L::NU];
+#pragma unroll
+        for (int u = 0; u < L::NU; ++u) {
             s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < NQ; ++c) {
@@ -186,12 +201,14 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
         }
         float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < L::NU; ++u) {
+            const unsigned w = (unsigned)(seen >> (16 * u)) >> (4 * g);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                if (!((seen >> (16 * u + 4 * g + r)) & 1)) s[u][r] = -INFINITY;
+                if (!((w >> r) & 1)) s[u][r] = -INFINITY;
                 top = fmaxf(top, s[u][r]);
             }
+        }
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
@@ -206,25 +223,24 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
         }
         const float at = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < L::NU; ++u)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], a.c2, -at));
                 l += s[u][r];
             }
         if constexpr (L::F32) {
-            using PV = Pack<float, L::VW>;
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < L::NU; ++u) {
+                const unsigned w = (unsigned)(seen >> (16 * u)) >> (4 * g);
 #pragma unroll
                 for (int sb = 0; sb < L::NSB; ++sb) {
-                    const int d = sb * L::SB + L::VW * n;
                     PV v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const int c = 16 * u + 4 * g + r;
-                        v[r] = *reinterpret_cast<const PV *>(row_of(vc, vn, c) + (d < a.dim ? d : 0));
-                        if (!((seen >> c) & 1)) v[r] = PV{};
+                        if constexpr (L::V_AHEAD) v[r] = va[u][sb][r];
+                        else v[r] = load_v(u, sb, r);
+                        if (!((w >> r) & 1)) v[r] = PV{};
                     }
 #pragma unroll
                     for (int e = 0; e < L::VW; ++e)
@@ -232,20 +248,24 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
                         for (int r = 0; r < 4; ++r)
                             o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
                 }
+            }
         } else {
             using V8 = typename Mat<T>::V8;
-            V8 pb;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) pb[i] = from_f32<T>(s[i >> 2][i & 3]);
             // the wave's own LDS: its writes above are done in order before these reads; only the compiler is to keep them apart
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            const int i16 = lane & 15, r = 4 * g + (i16 >> 2);
 #pragma unroll
-            for (int dt = 0; dt < DP / 16; ++dt) {
-                const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
-                const uint2 x = lds_read_transposed(lds + (r * L::PIECES + v_piece<DP>(r, c)) * 16 + byte);
-                const uint2 y = lds_read_transposed(lds + ((r + 16) * L::PIECES + v_piece<DP>(r + 16, c)) * 16 + byte);
-                o[dt] = Mat<T>::mul16(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
+            for (int half = 0; half < L::NU / 2; ++half) {
+                V8 pb;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) pb[i] = from_f32<T>(s[2 * half + (i >> 2)][i & 3]);
+                const int i16 = lane & 15, r = 32 * half + 4 * g + (i16 >> 2);
+#pragma unroll
+                for (int dt = 0; dt < DP / 16; ++dt) {
+                    const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
+                    const uint2 x = lds_read_transposed(lds + (r * L::PIECES + v_piece<DP>(r, c)) * 16 + byte);
+                    const uint2 y = lds_read_transposed(lds + ((r + 16) * L::PIECES + v_piece<DP>(r + 16, c)) * 16 + byte);
+                    o[dt] = Mat<T>::mul16(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
+                }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
@@ -270,13 +290,13 @@ __global__ __launch_bounds__(256) void attn_window_step_kernel(StepArgs a, int h
     __shared__ float ml[4][16][2];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t task = WAVES == 4 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
-    const int split = (int)(task % splits);
-    const int64_t r0 = task / splits, r1 = r0 / head_tiles;
-    const int ht = (int)(r0 % head_tiles);
+    const unsigned task = WAVES == 4 ? blockIdx.x : blockIdx.x * 4 + wave;      // below 2^31 + 3
+    const int split = (int)(task % (unsigned)splits);
+    const unsigned r0 = task / (unsigned)splits, r1 = r0 / (unsigned)head_tiles;
+    const int ht = (int)(r0 % (unsigned)head_tiles);
     Part t;
-    t.kvh = (int)(r1 % a.hk);
-    t.b = r1 / a.hk;
+    t.kvh = (int)(r1 % (unsigned)a.hk);
+    t.b = r1 / (unsigned)a.hk;
     if (t.b >= a.batch) return;
     t.heads = a.group - 16 * ht < 16 ? a.group - 16 * ht : 16;
     t.head0 = t.kvh * a.group + 16 * ht;
@@ -351,31 +371,56 @@ __global__ __launch_bounds__(256) void attn_window_step_kernel(StepArgs a, int h
     }
 }
 
-// Joins the parts of a row: a wave per (cache row, query head).
+// Joins the parts of a row: a block per (cache row, query head), its waves take the parts in turn.  All loads of a wave are
+// requested before the first is used: the kernel's time is a few memory latencies, not one per part.
+constexpr int kMaxSplits = 64;
+
 template <class T>
 __global__ __launch_bounds__(256) void attn_window_step_join_kernel(StepArgs a, int splits, const float *__restrict__ part_o,
                                                                     const float *__restrict__ part_ml)
 {
-    const int lane = threadIdx.x & 63;
+    __shared__ float2 acc[4][64];
+    const int lane = threadIdx.x & 63, d = 2 * lane;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-    if (row >= a.batch * a.hq) return;
-    float top = -INFINITY;
-    for (int s = 0; s < splits; ++s) top = fmaxf(top, part_ml[2 * (row * splits + s)]);
-    float sum = 0.f, acc0 = 0.f, acc1 = 0.f;
-    const bool has0 = lane < a.dim, has1 = lane + 64 < a.dim;
-    for (int s = 0; s < splits; ++s) {
-        const float ms = part_ml[2 * (row * splits + s)];
-        if (ms == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ms - top);
-        const float *po = part_o + (row * splits + s) * a.dim;
-        sum = fmaf(f, part_ml[2 * (row * splits + s) + 1], sum);
-        if (has0) acc0 = fmaf(f, po[lane], acc0);
-        if (has1) acc1 = fmaf(f, po[lane + 64], acc1);
+    const int64_t row = blockIdx.x, first = row * splits;
+    const bool has = d < a.dim;
+    const float2 *po = reinterpret_cast<const float2 *>(part_o + first * a.dim + (has ? d : 0));
+    const int64_t stride = a.dim / 2;
+    const float2 own = lane < splits ? reinterpret_cast<const float2 *>(part_ml)[first + lane] : make_float2(-INFINITY, 0.f);
+    float top = own.x;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    // weight of part `lane`; a part that saw nothing has no numerators
+    const float f = own.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(own.x - top);
+    const float sum = wave_sum(f * own.y);
+    constexpr int AHEAD = 8;
+    float x = 0.f, y = 0.f;
+    for (int s0 = wave; s0 < splits; s0 += 4 * AHEAD) {
+        float2 v[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = s0 + 4 * i;
+            v[i] = po[(int64_t)(s < splits ? s : s0) * stride];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const int s = s0 + 4 * i;
+            const float g = __shfl(f, s < splits ? s : 0), mg = __shfl(own.x, s < splits ? s : 0);
+            if (s < splits && mg != -INFINITY) {
+                x = fmaf(g, v[i].x, x);
+                y = fmaf(g, v[i].y, y);
+            }
+        }
     }
-    T *out = reinterpret_cast<T *>(a.out) + row * a.dim;
-    if (has0) out[lane] = from_f32<T>(sum == 0.f ? 0.f : acc0 / sum);
-    if (has1) out[lane + 64] = from_f32<T>(sum == 0.f ? 0.f : acc1 / sum);
+    acc[wave][lane] = make_float2(x, y);
+    __syncthreads();
+    if (wave == 0 && has) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        x = ((acc[0][lane].x + acc[1][lane].x) + (acc[2][lane].x + acc[3][lane].x)) * inv;
+        y = ((acc[0][lane].y + acc[1][lane].y) + (acc[2][lane].y + acc[3][lane].y)) * inv;
+        Pack<T, 2> two = {{from_f32<T>(x), from_f32<T>(y)}};
+        *reinterpret_cast<Pack<T, 2> *>(reinterpret_cast<T *>(a.out) + row * a.dim + d) = two;
+    }
 }
 
 struct Plan {
@@ -392,7 +437,7 @@ Plan plan_step(int64_t batch, int hk, int group, int64_t slots)
         const int64_t tasks = batch * hk * p.head_tiles, want = 4 * (int64_t)qcn_num_cus();
         int64_t s = tasks > 0 ? (want + tasks - 1) / tasks : 1;
         if (s > (slots + 127) / 128) s = (slots + 127) / 128;
-        if (s > 64) s = 64;
+        if (s > kMaxSplits) s = kMaxSplits;
         p.splits = (int)(s < 1 ? 1 : s);
     }
     return p;
@@ -402,7 +447,7 @@ template <class T, int DP>
 int launch_step_dim(const StepArgs &a, const Plan &p, float *ws, hipStream_t s)
 {
     const int64_t tasks = a.batch * a.hk * p.head_tiles * p.splits, blocks = p.waves == 4 ? tasks : (tasks + 3) / 4;
-    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (tasks >= ((int64_t)1 << 31) || blocks >= ((int64_t)1 << 31) || a.batch * a.hq >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
     const int64_t rows = a.batch * a.hq * p.splits;
     float *part_o = ws, *part_ml = ws ? ws + rows * a.dim : nullptr;
     if (p.waves == 4)
@@ -411,7 +456,7 @@ int launch_step_dim(const StepArgs &a, const Plan &p, float *ws, hipStream_t s)
         hipLaunchKernelGGL((attn_window_step_kernel<T, DP, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a, p.head_tiles, p.splits, part_o, part_ml);
     QCN_CHECK_LAUNCH();
     if (p.splits > 1) {
-        hipLaunchKernelGGL(attn_window_step_join_kernel<T>, dim3((unsigned)((a.batch * a.hq + 3) / 4)), dim3(256), 0, s, a, p.splits, part_o, part_ml);
+        hipLaunchKernelGGL(attn_window_step_join_kernel<T>, dim3((unsigned)(a.batch * a.hq)), dim3(256), 0, s, a, p.splits, part_o, part_ml);
         QCN_CHECK_LAUNCH();
     }
     return QCN_OK;
@@ -485,7 +530,7 @@ extern "C" int qcn_attn_window_step(const qcn_attn_window_step_args *args, void 
     const int group = (int)(x.n_q_heads / x.n_kv_heads);
     const Plan plan = plan_step(x.batch, (int)x.n_kv_heads, group, x.window + x.sinks);
     const size_t need = qcn_attn_window_step_workspace_bytes(x.batch, x.n_q_heads, x.n_kv_heads, x.dim, x.window, x.sinks);
-    if (need && (x.workspace_bytes < (int64_t)need || !x.workspace || ((uintptr_t)x.workspace & 3))) return QCN_ERR_WORKSPACE_TOO_SMALL;
+    if (need && (x.workspace_bytes < (int64_t)need || !x.workspace || ((uintptr_t)x.workspace & 7))) return QCN_ERR_WORKSPACE_TOO_SMALL;
     const StepArgs a = {x.q, x.k, x.v, {x.q_strides[0], x.q_strides[1]}, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]},
                         x.lengths, x.key_mask, x.batch, (int)x.n_q_heads, (int)x.n_kv_heads, group, (int)x.dim, x.window, x.sinks,
                         x.window + x.sinks,
