@@ -130,8 +130,9 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // 16 rows per wave, keys straight from memory (float32 of every width; 16-bit types up to 16 features)
 // ---------------------------------------------------------------------------------------------------------------------
 // A wave is on its own: no LDS, no barrier.  For short windows (the agents' 10 steps) every key tile is used by two or three row
-// tiles at most, so staging would cost more than the cache hits it saves; the four waves of a block take neighbouring key heads
-// of the same tokens, whose rows share cache lines.
+// tiles at most, so staging would cost more than the cache hits it saves.  A wave keeps its 16 rows and goes through key heads:
+// where its sequence lies, what its rows see and the rows' offsets are found once, and (narrow heads) the next head's rows are
+// requested while this head's are worked on.
 //
 // v_mfma_f32_16x16x4_f32: contraction index = lane >> 4.  A lane loads 4 neighbouring features (16 bytes) of its key and feeds
 // them to 4 products, so product e of piece c contracts features 16 c + 4 g + e.  V^T tile (sb, e) holds features
@@ -140,200 +141,259 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 template <class T, int DP> struct Direct {
     static constexpr int VW = DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1);
     static constexpr int SB = 16 * VW, NSB = DP / SB, NT = DP / 16;
+    static constexpr int NU = 2, CHUNK = 16 * NU;          // keys of a step
+    static constexpr bool AHEAD = DP <= 32;                // registers for the next step's rows
 };
 
 template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 
-template <class T, int DP>
-__global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t n_tiles)
+// OFF: byte offset inside one of the tensors; 32 bits where every tensor is below 4 GiB (a load then takes a scalar base).
+template <class T, int DP, class OFF>
+__global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t n_tiles, int heads_per_wave, int head_groups)
 {
     using L = Direct<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
-    constexpr int NU = 2;                                  // 16-key tiles per step
+    constexpr int NU = L::NU;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t item = (int64_t)qcn_xcd_remap(blockIdx.x, gridDim.x) * 4 + wave;
-    const int64_t tile = item / a.hk;
-    const int kvh = (int)(item % a.hk);
-    if (tile >= n_tiles) return;
-    const Tile t = find_tile(a, tile, 4, lane);
-    if (t.row0 < 0 || t.row0 >= t.rows) return;
-    const int last = (int)((t.rows - 1 - t.row0) < 15 ? (t.rows - 1 - t.row0) : 15);
-    const int64_t row = t.row0 + (n < last ? n : last);    // lanes past the end repeat the last row and do not store
+    const unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
+    const int64_t tile = item / (unsigned)head_groups;
+    const int h0 = (int)(item % (unsigned)head_groups) * heads_per_wave, h1 = h0 + heads_per_wave < a.hk ? h0 + heads_per_wave : a.hk;
+    const Tile t = find_tile(a, tile, 6, lane);
+    const int64_t row0 = t.row0 + 16 * wave;
+    if (t.row0 < 0 || row0 >= t.rows) return;
+    const int last = (int)((t.rows - 1 - row0) < 15 ? (t.rows - 1 - row0) : 15);
+    const int64_t row = row0 + (n < last ? n : last);      // lanes past the end repeat the last row and do not store
     const int64_t qi = row / a.group;
-    const int head = kvh * a.group + (int)(row % a.group);
+    const int sub = (int)(row % a.group);                  // query head inside the group
     if (t.behind) {
-        if (n <= last) zero_row<T>(a, t.q_beg + qi, head, g, 4);
+        if (n <= last)
+            for (int kvh = h0; kvh < h1; ++kvh) zero_row<T>(a, t.q_beg + qi, kvh * a.group + sub, g, 4);
         return;
     }
     const int p = (int)qi + t.shift;
-    const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
+    const int p0 = (int)(row0 / a.group) + t.shift, p1 = (int)((row0 + last) / a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
     const Sees sees = row_sees(a, keys, p);
     const int lo1 = p1 < 0 ? 0 : window_start(a, p1);
+    const int chunks = (keys.total + L::CHUNK - 1) / L::CHUNK;
 
-    const T *q = reinterpret_cast<const T *>(a.q) + (t.q_beg + qi) * a.qr.tok + head * a.qr.head;
-    const T *kb = reinterpret_cast<const T *>(a.k) + t.k_beg * a.kr.tok + kvh * a.kr.head;
-    const T *vb = reinterpret_cast<const T *>(a.v) + t.k_beg * a.vr.tok + kvh * a.vr.head;
+    constexpr int ES = sizeof(T);
+    const char *qb = reinterpret_cast<const char *>(a.q) + (t.q_beg * a.qr.tok) * ES;
+    const char *kb = reinterpret_cast<const char *>(a.k) + (t.k_beg * a.kr.tok) * ES;
+    const char *vb = reinterpret_cast<const char *>(a.v) + (t.k_beg * a.vr.tok) * ES;
+    char *ob = reinterpret_cast<char *>(a.out) + (t.q_beg * a.hq) * (int64_t)a.dim * ES;
+    const OFF q_off = (OFF)((qi * a.qr.tok + sub * a.qr.head) * ES), o_off = (OFF)((qi * a.hq + sub) * (int64_t)a.dim * ES);
     const uint8_t *mask = a.key_mask ? a.key_mask + t.k_beg : nullptr;
 
     using P4 = Pack<T, 4>;
     using PV = Pack<T, L::VW>;
-    P4 qf[DP / 16];
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-        const int d = 16 * c + 4 * g;
-        qf[c] = *reinterpret_cast<const P4 *>(q + (d < a.dim ? d : 0));
-        if (d >= a.dim) qf[c] = P4{};
-    }
-    f32x4 o[L::NT];
-#pragma unroll
-    for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-    const float c2 = a.c2;
-
-    for (int j0 = 0; j0 < keys.total; j0 += 16 * NU) {
-        f32x4 s[NU];
-        unsigned seen[NU];                                 // bit per key of the tile: inside the range and not masked
+    struct Place {                                         // of a step's keys
+        OFF k[NU], v[NU][4];
+        unsigned seen[NU];                                 // bit per key of a 16-key tile: inside the range and not masked
+    };
+    const auto locate = [&](int j0) {
+        Place x;
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int j = j0 + 16 * u + n;
             const bool in = j < keys.total;
             const int key = keys.key(in ? j : keys.total - 1);
-            const bool ok = in && (!mask || mask[key] != 0);
-            seen[u] = (unsigned)__ballot(ok) & 0xffffu;
-            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-            const T *kr = kb + key * a.kr.tok;
-            P4 kf[DP / 16];
+            x.seen[u] = (unsigned)__ballot(in && (!mask || mask[key] != 0)) & 0xffffu;
+            x.k[u] = (OFF)key * (OFF)(a.kr.tok * ES);
 #pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
-                const int d = 16 * c + 4 * g;
-                kf[c] = *reinterpret_cast<const P4 *>(kr + (d < a.dim ? d : 0));
-                if (d >= a.dim) kf[c] = P4{};
-            }
-#pragma unroll
-            for (int c = 0; c < DP / 16; ++c) {
-                if constexpr (F32) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[c].e[e], qf[c].e[e], s[u], 0, 0, 0);
-                } else {
-                    using V4 = typename Mat<T>::V4;
-                    s[u] = Mat<T>::mul16(__builtin_bit_cast(V4, kf[c]), __builtin_bit_cast(V4, qf[c]), s[u]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                const int jv = j0 + 16 * u + 4 * g + r;
+                x.v[u][r] = (OFF)keys.key(jv < keys.total ? jv : keys.total - 1) * (OFF)(a.vr.tok * ES);
             }
         }
-        // a tile whose keys every row sees needs no mask: inside the range, unmasked, up to the first row's position, inside
-        // the last row's window
-        const int jz = j0 + 16 * NU - 1;
-        const bool full = !mask && j0 >= keys.sinks && jz < keys.total && keys.key(jz) <= p0 && keys.key(j0) >= lo1;
-        if (!full) {
-            const uint64_t vis = sees.bits(j0);
+        return x;
+    };
+    struct Rows16 {                                        // 16-key tiles in registers
+        P4 k[NU][DP / 16];
+        PV v[L::AHEAD ? NU : 1][L::NSB][4];
+    };
+    const auto four = [&](const char *base, OFF off, int c) {   // features 16 c + 4 g ..
+        const int d = 16 * c + 4 * g;
+        P4 x = *reinterpret_cast<const P4 *>(base + (OFF)(off + (OFF)((d < a.dim ? d : 0) * ES)));
+        if (d >= a.dim) x = P4{};
+        return x;
+    };
+    const auto value = [&](const Place &x, int kvh, int u, int sb, int r) {
+        const int d = sb * L::SB + L::VW * n;
+        return *reinterpret_cast<const PV *>(vb + kvh * a.vr.head * ES + (OFF)(x.v[u][r] + (OFF)((d < a.dim ? d : 0) * ES)));
+    };
+    const auto load = [&](const Place &x, int kvh) {
+        Rows16 y;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int c = 0; c < DP / 16; ++c) y.k[u][c] = four(kb + kvh * a.kr.head * ES, x.k[u], c);
+        if constexpr (L::AHEAD) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int sb = 0; sb < L::NSB; ++sb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) y.v[u][sb][r] = value(x, kvh, u, sb, r);
+        }
+        return y;
+    };
+    struct Query { P4 q[DP / 16]; };
+    const auto load_q = [&](int kvh) {
+        Query y;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c) y.q[c] = four(qb + (int64_t)kvh * a.group * a.qr.head * ES, q_off, c);
+        return y;
+    };
+    const float c2 = a.c2;
+
+    Place here = {};
+    Rows16 rows = {};
+    if (chunks) here = locate(0);
+    Query qf = load_q(h0);
+    if (L::AHEAD && chunks) rows = load(here, h0);
+    for (int kvh = h0; kvh < h1; ++kvh) {
+        f32x4 o[L::NT];
+#pragma unroll
+        for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, l = 0.f;
+        Query q_next = qf;
+        for (int step = 0; step < chunks; ++step) {
+            const int j0 = step * L::CHUNK;
+            const bool more = step + 1 < chunks;
+            Place there = here;
+            Rows16 ahead;
+            if (chunks > 1) there = locate(more ? j0 + L::CHUNK : 0);
+            if constexpr (L::AHEAD) {
+                // the next step's rows, or the next head's (the last head's are read again: no branch around loads)
+                const int next_head = more ? kvh : (kvh + 1 < h1 ? kvh + 1 : kvh);
+                ahead = load(there, next_head);
+                if (!more) q_next = load_q(next_head);
+            } else {
+                rows = load(here, kvh);
+            }
+            f32x4 s[NU];
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                const unsigned w = ((unsigned)(vis >> (16 * u)) & seen[u]) >> (4 * g);
+                s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s[u][r] = seen_or_inf(w, r, s[u][r]);
-            }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
-        const float scaled = top * c2;
-        if (__ballot(scaled > m + 8.f)) {
-            const float mn = scaled > m ? scaled : m;
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-            l *= alpha;
-#pragma unroll
-            for (int i = 0; i < L::NT; ++i) o[i] *= alpha;
-            m = mn;
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
-                l += s[u][r];
-            }
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            int64_t at[4];
-            bool ok[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int j = j0 + 16 * u + 4 * g + r;
-                ok[r] = (seen[u] >> (4 * g + r)) & 1;
-                at[r] = keys.key(j < keys.total ? j : keys.total - 1) * a.vr.tok;
-            }
-#pragma unroll
-            for (int sb = 0; sb < L::NSB; ++sb) {
-                const int d = sb * L::SB + L::VW * n;
-                PV v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v[r] = *reinterpret_cast<const PV *>(vb + at[r] + (d < a.dim ? d : 0));
-                    if (!ok[r]) v[r] = PV{};               // 0 times what a masked key holds must stay 0
-                }
-#pragma unroll
-                for (int e = 0; e < L::VW; ++e) {
+                for (int c = 0; c < DP / 16; ++c) {
                     if constexpr (F32) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
+                        for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[u][c].e[e], qf.q[c].e[e], s[u], 0, 0, 0);
                     } else {
-                        typename Mat<T>::V4 va, pb;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
-                        o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                        using V4 = typename Mat<T>::V4;
+                        s[u] = Mat<T>::mul16(__builtin_bit_cast(V4, rows.k[u][c]), __builtin_bit_cast(V4, qf.q[c]), s[u]);
                     }
                 }
             }
-        }
-    }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    bool bad = false;
-    T *out = reinterpret_cast<T *>(a.out) + ((t.q_beg + qi) * a.hq + head) * (int64_t)a.dim;
+            // a step whose keys every row sees needs no mask: inside the range, unmasked, up to the first row's position, inside
+            // the last row's window
+            const int jz = j0 + L::CHUNK - 1;
+            const bool full = !mask && j0 >= keys.sinks && jz < keys.total && keys.key(jz) <= p0 && keys.key(j0) >= lo1;
+            if (!full) {
+                const uint64_t vis = sees.bits(j0);
 #pragma unroll
-    for (int i = 0; i < L::NT; ++i)
+                for (int u = 0; u < NU; ++u) {
+                    const unsigned w = ((unsigned)(vis >> (16 * u)) & here.seen[u]) >> (4 * g);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            o[i][r] *= inv;
-            bad |= !(fabsf(o[i][r]) < INFINITY);
-        }
-    unsigned repair = 0;
-    {
-        const uint64_t b = __ballot(bad && n <= last);
-        repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
-    }
-    if (n <= last && !((repair >> n) & 1)) {
-#pragma unroll
-        for (int sb = 0; sb < L::NSB; ++sb) {
-            const int d = sb * L::SB + 4 * L::VW * g;
-#pragma unroll
-            for (int part = 0; part < L::VW; ++part) {     // 4 features each
-                if (d + 4 * part >= a.dim) break;
-                P4 w;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int f = 4 * part + x;            // feature f of the lane's 4 VW: r = f / VW, e = f % VW
-                    w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW]);
+                    for (int r = 0; r < 4; ++r) s[u][r] = seen_or_inf(w, r, s[u][r]);
                 }
-                *reinterpret_cast<P4 *>(out + d + 4 * part) = w;
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+            const float scaled = top * c2;
+            if (__ballot(scaled > m + 8.f)) {
+                const float mn = scaled > m ? scaled : m;
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < L::NT; ++i) o[i] *= alpha;
+                m = mn;
+            }
+            const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
+                    l += s[u][r];
+                }
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+#pragma unroll
+                for (int sb = 0; sb < L::NSB; ++sb) {
+                    PV v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if constexpr (L::AHEAD) v[r] = rows.v[u][sb][r];
+                        else v[r] = value(here, kvh, u, sb, r);
+                        if (!((here.seen[u] >> (4 * g + r)) & 1)) v[r] = PV{};   // 0 times what a masked key holds must stay 0
+                    }
+#pragma unroll
+                    for (int e = 0; e < L::VW; ++e) {
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
+                        } else {
+                            typename Mat<T>::V4 va, pb;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
+                            o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                        }
+                    }
+                }
+            }
+            here = there;
+            if constexpr (L::AHEAD) rows = ahead;
+        }
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < L::NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                o[i][r] *= inv;
+                bad |= !(fabsf(o[i][r]) < INFINITY);
+            }
+        const uint64_t b = __ballot(bad && n <= last);
+        unsigned repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
+        if (n <= last && !((repair >> n) & 1)) {
+            char *out = ob + (int64_t)kvh * a.group * a.dim * ES;
+#pragma unroll
+            for (int sb = 0; sb < L::NSB; ++sb) {
+                const int d = sb * L::SB + 4 * L::VW * g;
+#pragma unroll
+                for (int part = 0; part < L::VW; ++part) { // 4 features each
+                    if (d + 4 * part >= a.dim) break;
+                    P4 w;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int f = 4 * part + x;        // feature f of the lane's 4 VW: r = f / VW, e = f % VW
+                        w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW]);
+                    }
+                    *reinterpret_cast<P4 *>(out + (OFF)(o_off + (OFF)((d + 4 * part) * ES))) = w;
+                }
             }
         }
-    }
-    // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
-    // Rows that came out not finite are formed again key by key.
-    for (; repair; repair &= repair - 1) {
-        const int64_t r = t.row0 + __builtin_ctz(repair);
-        row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+        // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
+        // Rows that came out not finite are formed again key by key.
+        for (; repair; repair &= repair - 1) {
+            const int64_t r = row0 + __builtin_ctz(repair);
+            row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+        }
+        if constexpr (L::AHEAD) qf = q_next;
+        else if (kvh + 1 < h1) qf = load_q(kvh + 1);
     }
 }
 
@@ -744,9 +804,21 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int split
 template <class T, int DP>
 int launch_direct(const Args &a, hipStream_t s)
 {
-    const int64_t tiles = (a.nq * a.group >> 4) + a.n_seq + 1, blocks = (tiles * a.hk + 3) / 4;
+    const int64_t tiles = (a.nq * a.group >> 6) + a.n_seq + 1;
+    // as many key heads per wave as leave four blocks per CU
+    int hpw = a.hk;
+    while (hpw > 1 && tiles * ((a.hk + hpw - 1) / hpw) < 4 * (int64_t)qcn_num_cus()) hpw = (hpw + 1) / 2;
+    const int groups = (a.hk + hpw - 1) / hpw;
+    const int64_t blocks = tiles * groups;
     if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
-    hipLaunchKernelGGL((attn_window_direct_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles);
+    const int64_t most = (int64_t)1 << 32, es = sizeof(T);
+    const auto bytes = [&](int64_t tokens, int64_t tok, int64_t head, int64_t heads) { return (tokens * tok + heads * head + a.dim) * es; };
+    const bool small = bytes(a.nq, a.qr.tok, a.qr.head, a.hq) < most && bytes(a.nk, a.kr.tok, a.kr.head, a.hk) < most &&
+                       bytes(a.nk, a.vr.tok, a.vr.head, a.hk) < most && a.nq * a.hq * a.dim * es < most;
+    if (small)
+        hipLaunchKernelGGL((attn_window_direct_kernel<T, DP, uint32_t>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles, hpw, groups);
+    else
+        hipLaunchKernelGGL((attn_window_direct_kernel<T, DP, uint64_t>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles, hpw, groups);
     QCN_CHECK_LAUNCH();
     return QCN_OK;
 }
