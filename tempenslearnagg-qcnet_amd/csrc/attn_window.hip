@@ -175,7 +175,6 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     const int p0 = (int)(row0 / a.group) + t.shift, p1 = (int)((row0 + last) / a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
     const Sees sees = row_sees(a, keys, p);
-    const int lo1 = p1 < 0 ? 0 : window_start(a, p1);
     const int chunks = (keys.total + L::CHUNK - 1) / L::CHUNK;
 
     constexpr int ES = sizeof(T);
@@ -190,21 +189,25 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     using PV = Pack<T, L::VW>;
     struct Place {                                         // of a step's keys
         OFF k[NU], v[NU][4];
-        unsigned seen[NU];                                 // bit per key of a 16-key tile: inside the range and not masked
-    };
+        int sees[NU][4], seen[NU][4];                      // all bits or none: whether this lane's row sees the score's key; whether
+    };                                                     // the key is inside the range and not masked
     const auto locate = [&](int j0) {
         Place x;
+        const uint64_t vis = sees.bits(j0);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int j = j0 + 16 * u + n;
             const bool in = j < keys.total;
             const int key = keys.key(in ? j : keys.total - 1);
-            x.seen[u] = (unsigned)__ballot(in && (!mask || mask[key] != 0)) & 0xffffu;
+            const unsigned seen = (unsigned)__ballot(in && (!mask || mask[key] != 0)) >> (4 * g);
+            const unsigned both = seen & (unsigned)(vis >> (16 * u + 4 * g));
             x.k[u] = (OFF)key * (OFF)(a.kr.tok * ES);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int jv = j0 + 16 * u + 4 * g + r;
                 x.v[u][r] = (OFF)keys.key(jv < keys.total ? jv : keys.total - 1) * (OFF)(a.vr.tok * ES);
+                x.sees[u][r] = __builtin_amdgcn_sbfe((int)both, r, 1);
+                x.seen[u][r] = __builtin_amdgcn_sbfe((int)seen, r, 1);
             }
         }
         return x;
@@ -213,10 +216,11 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         P4 k[NU][DP / 16];
         PV v[L::AHEAD ? NU : 1][L::NSB][4];
     };
+    const bool padded = a.dim < DP;
     const auto four = [&](const char *base, OFF off, int c) {   // features 16 c + 4 g ..
         const int d = 16 * c + 4 * g;
         P4 x = *reinterpret_cast<const P4 *>(base + (OFF)(off + (OFF)((d < a.dim ? d : 0) * ES)));
-        if (d >= a.dim) x = P4{};
+        if (padded && d >= a.dim) x = P4{};
         return x;
     };
     const auto value = [&](const Place &x, int kvh, int u, int sb, int r) {
@@ -247,117 +251,82 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         return y;
     };
     const float c2 = a.c2;
-
-    Place here = {};
-    Rows16 rows = {};
-    if (chunks) here = locate(0);
-    Query qf = load_q(h0);
-    if (L::AHEAD && chunks) rows = load(here, h0);
-    for (int kvh = h0; kvh < h1; ++kvh) {
-        f32x4 o[L::NT];
+    // scores, -inf where unseen; returns the largest of the lane's row
+    const auto scores = [&](const Place &x, const Rows16 &rows, const Query &q, f32x4 (&s)[NU]) {
 #pragma unroll
-        for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float m = -INFINITY, l = 0.f;
-        Query q_next = qf;
-        for (int step = 0; step < chunks; ++step) {
-            const int j0 = step * L::CHUNK;
-            const bool more = step + 1 < chunks;
-            Place there = here;
-            Rows16 ahead;
-            if (chunks > 1) there = locate(more ? j0 + L::CHUNK : 0);
-            if constexpr (L::AHEAD) {
-                // the next step's rows, or the next head's (the last head's are read again: no branch around loads)
-                const int next_head = more ? kvh : (kvh + 1 < h1 ? kvh + 1 : kvh);
-                ahead = load(there, next_head);
-                if (!more) q_next = load_q(next_head);
-            } else {
-                rows = load(here, kvh);
-            }
-            f32x4 s[NU];
+        for (int u = 0; u < NU; ++u) {
+            s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < DP / 16; ++c) {
+                if constexpr (F32) {
 #pragma unroll
-                for (int c = 0; c < DP / 16; ++c) {
-                    if constexpr (F32) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[u][c].e[e], qf.q[c].e[e], s[u], 0, 0, 0);
-                    } else {
-                        using V4 = typename Mat<T>::V4;
-                        s[u] = Mat<T>::mul16(__builtin_bit_cast(V4, rows.k[u][c]), __builtin_bit_cast(V4, qf.q[c]), s[u]);
-                    }
+                    for (int e = 0; e < 4; ++e) s[u] = __builtin_amdgcn_mfma_f32_16x16x4f32(rows.k[u][c].e[e], q.q[c].e[e], s[u], 0, 0, 0);
+                } else {
+                    using V4 = typename Mat<T>::V4;
+                    s[u] = Mat<T>::mul16(__builtin_bit_cast(V4, rows.k[u][c]), __builtin_bit_cast(V4, q.q[c]), s[u]);
                 }
             }
-            // a step whose keys every row sees needs no mask: inside the range, unmasked, up to the first row's position, inside
-            // the last row's window
-            const int jz = j0 + L::CHUNK - 1;
-            const bool full = !mask && j0 >= keys.sinks && jz < keys.total && keys.key(jz) <= p0 && keys.key(j0) >= lo1;
-            if (!full) {
-                const uint64_t vis = sees.bits(j0);
+        }
+        float top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < NU; ++u) {
-                    const unsigned w = ((unsigned)(vis >> (16 * u)) & here.seen[u]) >> (4 * g);
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[u][r] = seen_or_inf(w, r, s[u][r]);
-                }
+            for (int r = 0; r < 4; ++r) {
+                const float raw = s[u][r];
+                const int keep = x.sees[u][r];
+                s[u][r] = __builtin_bit_cast(float, (__builtin_bit_cast(int, raw) & keep) | ((int)0xff800000 & ~keep));
+                top = fmaxf(top, s[u][r]);
             }
-            float top = -INFINITY;
+        return quarters_max(top) * c2;
+    };
+    // p in place of the scores; returns the lane's sum
+    const auto softmax = [&](f32x4 (&s)[NU], float m) {
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum = 0.f;
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
+        for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) top = fmaxf(top, s[u][r]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
-            const float scaled = top * c2;
-            if (__ballot(scaled > m + 8.f)) {
-                const float mn = scaled > m ? scaled : m;
-                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
-                l *= alpha;
-#pragma unroll
-                for (int i = 0; i < L::NT; ++i) o[i] *= alpha;
-                m = mn;
+            for (int r = 0; r < 4; ++r) {
+                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
+                sum += s[u][r];
             }
-            const float base = m == -INFINITY ? 0.f : m;
+        return sum;
+    };
+    const auto accumulate = [&](const Place &x, const Rows16 &rows, int kvh, const f32x4 (&s)[NU], f32x4 (&o)[L::NT]) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int sb = 0; sb < L::NSB; ++sb) {
+                PV v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], c2, -base));
-                    l += s[u][r];
-                }
+                    if constexpr (L::AHEAD) v[r] = rows.v[u][sb][r];
+                    else v[r] = value(x, kvh, u, sb, r);
+                    if (mask) {                            // 0 times what a masked key holds must stay 0
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-#pragma unroll
-                for (int sb = 0; sb < L::NSB; ++sb) {
-                    PV v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if constexpr (L::AHEAD) v[r] = rows.v[u][sb][r];
-                        else v[r] = value(here, kvh, u, sb, r);
-                        if (!((here.seen[u] >> (4 * g + r)) & 1)) v[r] = PV{};   // 0 times what a masked key holds must stay 0
-                    }
-#pragma unroll
-                    for (int e = 0; e < L::VW; ++e) {
-                        if constexpr (F32) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
-                        } else {
-                            typename Mat<T>::V4 va, pb;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
-                            o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                        for (int e = 0; e < L::VW; ++e) {
+                            if constexpr (F32) v[r].e[e] = __builtin_bit_cast(float, __builtin_bit_cast(int, v[r].e[e]) & x.seen[u][r]);
+                            else v[r].e[e] = __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(uint16_t, v[r].e[e]) & x.seen[u][r]));
                         }
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < L::VW; ++e) {
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
+                    } else {
+                        typename Mat<T>::V4 va, pb;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
+                        o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                    }
+                }
             }
-            here = there;
-            if constexpr (L::AHEAD) rows = ahead;
-        }
-        l += __shfl_xor(l, 16);
-        l += __shfl_xor(l, 32);
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+    };
+    const auto finish = [&](int kvh, float l, f32x4 (&o)[L::NT]) {
+        const float inv = inverse_sum(quarters_sum(l));
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < L::NT; ++i)
@@ -366,8 +335,8 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 o[i][r] *= inv;
                 bad |= !(fabsf(o[i][r]) < INFINITY);
             }
-        const uint64_t b = __ballot(bad && n <= last);
-        unsigned repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
+        unsigned repair = 0;
+        if (const uint64_t b = __ballot(bad && n <= last)) repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
         if (n <= last && !((repair >> n) & 1)) {
             char *out = ob + (int64_t)kvh * a.group * a.dim * ES;
 #pragma unroll
@@ -392,8 +361,56 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
             const int64_t r = row0 + __builtin_ctz(repair);
             row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
         }
-        if constexpr (L::AHEAD) qf = q_next;
-        else if (kvh + 1 < h1) qf = load_q(kvh + 1);
+    };
+    const auto clear = [&](f32x4 (&o)[L::NT]) {
+#pragma unroll
+        for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+
+    if (L::AHEAD && chunks == 1) {
+        // all keys in one step: found once for all heads; no running maximum; the next head's rows in the other set of registers
+        const Place x = locate(0);
+        Rows16 ra = load(x, h0), rb;
+        Query qa = load_q(h0), qc;
+        const auto head = [&](int kvh, const Rows16 &rows, const Query &q, Rows16 &rows_next, Query &q_next) {
+            const int next = kvh + 1 < h1 ? kvh + 1 : kvh;      // the last head's are read again: no branch around loads
+            rows_next = load(x, next);
+            q_next = load_q(next);
+            f32x4 s[NU], o[L::NT];
+            clear(o);
+            const float m = scores(x, rows, q, s);
+            const float l = softmax(s, m);
+            accumulate(x, rows, kvh, s, o);
+            finish(kvh, l, o);
+        };
+        for (int kvh = h0; kvh < h1; kvh += 2) {
+            head(kvh, ra, qa, rb, qc);
+            if (kvh + 1 < h1) head(kvh + 1, rb, qc, ra, qa);
+        }
+        return;
+    }
+    for (int kvh = h0; kvh < h1; ++kvh) {
+        f32x4 s[NU], o[L::NT];
+        clear(o);
+        float m = -INFINITY, l = 0.f;
+        const Query q = load_q(kvh);
+        for (int step = 0; step < chunks; ++step) {
+            const Place x = locate(step * L::CHUNK);
+            const Rows16 rows = load(x, kvh);
+            // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
+            const float scaled = scores(x, rows, q, s);
+            if (__ballot(scaled > m + 8.f)) {
+                const float mn = scaled > m ? scaled : m;
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
+                l *= alpha;
+#pragma unroll
+                for (int i = 0; i < L::NT; ++i) o[i] *= alpha;
+                m = mn;
+            }
+            l += softmax(s, m);
+            accumulate(x, rows, kvh, s, o);
+        }
+        finish(kvh, l, o);
     }
 }
 
@@ -642,7 +659,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
         for (int r = 0; r < 16; ++r) top[r & 3] = fmaxf(fmaxf(top[r & 3], s[0][r]), s[1][r]);
         top[0] = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         // the running maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
-        const float scaled = fmaxf(top[0], other_half(top[0])) * c2;
+        const float scaled = halves_max(top[0]) * c2;
         if (__ballot(scaled > m + 8.f)) {
             const float mn = scaled > m ? scaled : m;
             const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn);
@@ -688,8 +705,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
             if (step + 1 < s1) run_step(step + 1, std::integral_constant<int, 1>{});
         }
     }
-    l += l2;
-    l += other_half(l);
+    l = halves_sum(l + l2);
     if (splits > 1) {
         // joined by attn_window_join_kernel: this part's maximum, sum and numerators
         const int64_t at = out_row * splits + split;
@@ -705,7 +721,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
         }
         return;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_sum(l);
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < ND; ++i)

@@ -209,8 +209,7 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
                 top = fmaxf(top, s[u][r]);
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
+        top = quarters_max(top);
         // the maximum follows only jumps of more than 2^8: until then p stays below 2^8 and nothing is rescaled
         const float scaled = top * a.c2;
         if (__ballot(scaled > m + 8.f)) {
@@ -270,8 +269,7 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     }
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
+    l = quarters_sum(l);
 }
 
 // features of accumulator element (tile i, register r) of lane group g
@@ -314,7 +312,7 @@ __global__ __launch_bounds__(256) void attn_window_step_kernel(StepArgs a, int h
 
     T *out = reinterpret_cast<T *>(a.out) + t.b * (int64_t)a.hq * a.dim;
     if constexpr (WAVES == 1) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = inverse_sum(l);
         if (n < t.heads) {
 #pragma unroll
             for (int sb = 0; sb < L::NSB; ++sb)

@@ -146,13 +146,29 @@ __device__ __forceinline__ uint2 lds_read_transposed(const void *p)
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) S4 *)p));
 }
 
-// value of the lane in the other half of the wave
-__device__ __forceinline__ float other_half(float v)
+// Largest and sum over lanes l, l ^ 32 (halves), and over l, l ^ 16, l ^ 32, l ^ 48 (quarters).  v_permlane32_swap of a value with
+// itself leaves the low half's value in all lanes of one result and the high half's in the other; v_permlane16_swap likewise
+// for the 16-lane rows of each half.
+struct Pair { float a, b; };
+__device__ __forceinline__ Pair both_halves(float v)
 {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
-    // r[0] = {own low half, low half again}: lanes below 32 need r[1], the others r[0]
-    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+    const unsigned x = r[0], y = r[1];   // (a bit cast of a vector's element in place takes its first element)
+    return {__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
 }
+__device__ __forceinline__ Pair both_rows(float v)
+{
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, v), __builtin_bit_cast(unsigned, v), false, false);
+    const unsigned x = r[0], y = r[1];   // (a bit cast of a vector's element in place takes its first element)
+    return {__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
+}
+__device__ __forceinline__ float halves_max(float v) { const Pair p = both_halves(v); return fmaxf(p.a, p.b); }
+__device__ __forceinline__ float halves_sum(float v) { const Pair p = both_halves(v); return p.a + p.b; }
+__device__ __forceinline__ float quarters_max(float v) { const Pair p = both_rows(halves_max(v)); return fmaxf(p.a, p.b); }
+__device__ __forceinline__ float quarters_sum(float v) { const Pair p = both_rows(halves_sum(v)); return p.a + p.b; }
+
+// 1 / sum of a softmax whose largest term is at least 1 (the running maximum is at most the largest score), 0 for an empty row
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l); }
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
