@@ -62,7 +62,11 @@ struct Tile {
     int64_t q_beg, k_beg;   // first token of the sequence
     int64_t rows, row0;     // rows of the sequence; first row of the tile
     int lk, shift;          // keys of the sequence; position of query i = i + shift
+    int token0, sub0;       // token of the tile's first row (counted in the sequence) and its query head in the group
     bool behind;            // rows behind the last sequence
+    // token and query head of the tile's row r
+    __device__ __forceinline__ int token(int r, int group) const { return group == 1 ? token0 + r : token0 + (int)((unsigned)(sub0 + r) / (unsigned)group); }
+    __device__ __forceinline__ int sub(int r, int group) const { return group == 1 ? 0 : (int)((unsigned)(sub0 + r) % (unsigned)group); }
 };
 
 __device__ __forceinline__ Tile find_tile(const Args &a, int64_t tile, int shift, int lane)
@@ -83,6 +87,8 @@ __device__ __forceinline__ Tile find_tile(const Args &a, int64_t tile, int shift
     t.row0 = (tile - ((t.q_beg * a.group >> shift) + b)) << shift;
     t.lk = (int)(k_end - t.k_beg);
     t.shift = t.lk - (int)(q_end - t.q_beg);
+    t.token0 = (int)(a.group == 1 ? t.row0 : t.row0 / a.group);
+    t.sub0 = a.group == 1 ? 0 : (int)(t.row0 % a.group);
     return t;
 }
 
@@ -163,16 +169,16 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     const int64_t row0 = t.row0 + 16 * wave;
     if (t.row0 < 0 || row0 >= t.rows) return;
     const int last = (int)((t.rows - 1 - row0) < 15 ? (t.rows - 1 - row0) : 15);
-    const int64_t row = row0 + (n < last ? n : last);      // lanes past the end repeat the last row and do not store
-    const int64_t qi = row / a.group;
-    const int sub = (int)(row % a.group);                  // query head inside the group
+    const int r_own = 16 * wave + (n < last ? n : last);   // lanes past the end repeat the last row and do not store
+    const int64_t qi = t.token(r_own, a.group);
+    const int sub = t.sub(r_own, a.group);                 // query head inside the group
     if (t.behind) {
         if (n <= last)
             for (int kvh = h0; kvh < h1; ++kvh) zero_row<T>(a, t.q_beg + qi, kvh * a.group + sub, g, 4);
         return;
     }
     const int p = (int)qi + t.shift;
-    const int p0 = (int)(row0 / a.group) + t.shift, p1 = (int)((row0 + last) / a.group) + t.shift;
+    const int p0 = t.token(16 * wave, a.group) + t.shift, p1 = t.token(16 * wave + last, a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
     const Sees sees = row_sees(a, keys, p);
     const int chunks = (keys.total + L::CHUNK - 1) / L::CHUNK;
@@ -358,8 +364,8 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
         // Rows that came out not finite are formed again key by key.
         for (; repair; repair &= repair - 1) {
-            const int64_t r = row0 + __builtin_ctz(repair);
-            row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+            const int r = 16 * wave + __builtin_ctz(repair), token = t.token(r, a.group);
+            row_by_wave<T>(a, t.k_beg, token + t.shift, t.q_beg + token, kvh * a.group + t.sub(r, a.group), lane);
         }
     };
     const auto clear = [&](f32x4 (&o)[L::NT]) {
@@ -483,9 +489,9 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     const int last = (int)(left < 127 ? left : 127);           // last row of the tile
     const int r_local = wave * 32 + n;
     const bool real = r_local <= last;
-    const int64_t row = t.row0 + (real ? r_local : last);
-    const int64_t qi = row / a.group;
-    const int head = kvh * a.group + (int)(row % a.group);
+    const int r_own = real ? r_local : last;
+    const int64_t qi = t.token(r_own, a.group);
+    const int head = kvh * a.group + t.sub(r_own, a.group);
     const int64_t out_row = (t.q_beg + qi) * a.hq + head;
     if (t.behind) {
         if (splits > 1) {
@@ -493,16 +499,16 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
             return;
         }
         for (int r = wave; r <= last; r += 4)
-            zero_row<T>(a, t.q_beg + (t.row0 + r) / a.group, kvh * a.group + (int)((t.row0 + r) % a.group), lane, 64);
+            zero_row<T>(a, t.q_beg + t.token(r, a.group), kvh * a.group + t.sub(r, a.group), lane, 64);
         return;
     }
     const int p = (int)qi + t.shift;
-    const int p0 = (int)(t.row0 / a.group) + t.shift, p1 = (int)((t.row0 + last) / a.group) + t.shift;
+    const int p0 = t.token0 + t.shift, p1 = t.token(last, a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
     const Sees sees = row_sees(a, keys, p);
     // the wave's own rows
     const int wa = wave * 32 < last ? wave * 32 : last, wz = wave * 32 + 31 < last ? wave * 32 + 31 : last;
-    const int wp0 = (int)((t.row0 + wa) / a.group) + t.shift, wp1 = (int)((t.row0 + wz) / a.group) + t.shift;
+    const int wp0 = t.token(wa, a.group) + t.shift, wp1 = t.token(wz, a.group) + t.shift;
     const int wlo0 = wp0 < 0 ? 0 : window_start(a, wp0), wlo1 = wp1 < 0 ? 0 : window_start(a, wp1);
 
     const T *q = reinterpret_cast<const T *>(a.q) + (t.q_beg + qi) * a.qr.tok + head * a.qr.head;
@@ -758,8 +764,8 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
     // Rows that came out not finite are formed again key by key.
     for (; repair; repair &= repair - 1) {
-        const int64_t r = t.row0 + wave * 32 + __builtin_ctz(repair);
-        row_by_wave<T>(a, t.k_beg, r / a.group + t.shift, t.q_beg + r / a.group, kvh * a.group + (int)(r % a.group), lane);
+        const int r = wave * 32 + __builtin_ctz(repair), token = t.token(r, a.group);
+        row_by_wave<T>(a, t.k_beg, token + t.shift, t.q_beg + token, kvh * a.group + t.sub(r, a.group), lane);
     }
 }
 
