@@ -69,24 +69,21 @@ struct Tile {
     __device__ __forceinline__ int sub(int r, int group) const { return group == 1 ? 0 : (int)((unsigned)(sub0 + r) % (unsigned)group); }
 };
 
-__device__ __forceinline__ Tile find_tile(const Args &a, int64_t tile, int shift, int lane)
+__device__ __forceinline__ Tile find_tile(const Args &a, int64_t tile, int64_t n_tiles, int shift, int lane)
 {
     Tile t;
-    const int64_t b = find_seq(a.cu_q, a.n_seq, a.nq, a.group, shift, tile, lane);
-    t.behind = b == a.n_seq;
-    int64_t q_end, k_end;
-    if (t.behind) {
-        t.q_beg = clamp64(a.cu_q[b], 0, a.nq);
-        q_end = a.nq;
-        t.k_beg = k_end = 0;
-    } else {
-        seq_range(a.cu_q, b, a.nq, t.q_beg, q_end);
-        seq_range(a.cu_k, b, a.nk, t.k_beg, k_end);
-    }
-    t.rows = (q_end - t.q_beg) * a.group;
-    t.row0 = (tile - ((t.q_beg * a.group >> shift) + b)) << shift;
+    const Found f = find_seq(a.cu_q, a.n_seq, a.nq, a.group, shift, tile, n_tiles, lane);
+    t.behind = f.b == a.n_seq;
+    t.q_beg = f.beg;
+    int64_t k_end = f.end;
+    t.k_beg = f.beg;
+    if (t.behind) t.k_beg = k_end = 0;
+    else if (a.cu_k != a.cu_q) seq_range(a.cu_k, f.b, a.nk, t.k_beg, k_end);
+    else if (k_end > a.nk) { t.k_beg = t.k_beg < a.nk ? t.k_beg : a.nk; k_end = a.nk; }
+    t.rows = (f.end - f.beg) * a.group;
+    t.row0 = (tile - ((f.beg * a.group >> shift) + f.b)) << shift;
     t.lk = (int)(k_end - t.k_beg);
-    t.shift = t.lk - (int)(q_end - t.q_beg);
+    t.shift = t.lk - (int)(f.end - f.beg);
     t.token0 = (int)(a.group == 1 ? t.row0 : t.row0 / a.group);
     t.sub0 = a.group == 1 ? 0 : (int)(t.row0 % a.group);
     return t;
@@ -165,7 +162,7 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     const unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
     const int64_t tile = item / (unsigned)head_groups;
     const int h0 = (int)(item % (unsigned)head_groups) * heads_per_wave, h1 = h0 + heads_per_wave < a.hk ? h0 + heads_per_wave : a.hk;
-    const Tile t = find_tile(a, tile, 6, lane);
+    const Tile t = find_tile(a, tile, n_tiles, 6, lane);
     const int64_t row0 = t.row0 + 16 * wave;
     if (t.row0 < 0 || row0 >= t.rows) return;
     const int last = (int)((t.rows - 1 - row0) < 15 ? (t.rows - 1 - row0) : 15);
@@ -483,7 +480,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     item /= (unsigned)splits;
     const int64_t tile = item % (unsigned)n_tiles;
     const int kvh = (int)(item / (unsigned)n_tiles);
-    const Tile t = find_tile(a, tile, kRowShift, lane);
+    const Tile t = find_tile(a, tile, n_tiles, kRowShift, lane);
     if (t.row0 < 0 || t.row0 >= t.rows) return;
     const int64_t left = t.rows - 1 - t.row0;
     const int last = (int)(left < 127 ? left : 127);           // last row of the tile

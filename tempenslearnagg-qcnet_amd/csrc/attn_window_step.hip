@@ -31,13 +31,12 @@ struct AppendArgs {
 template <class T>
 __global__ __launch_bounds__(256) void window_cache_append_kernel(AppendArgs a)
 {
-    const int64_t b = find_seq(a.cu, a.n_seq, a.n, 1, kAppendShift, blockIdx.x, threadIdx.x & 63);
-    if (b == a.n_seq) return;                               // behind the last sequence: left as they are
-    int64_t beg, end;
-    seq_range(a.cu, b, a.n, beg, end);
+    const Found f = find_seq(a.cu, a.n_seq, a.n, 1, kAppendShift, blockIdx.x, gridDim.x, threadIdx.x & 63);
+    if (f.b == a.n_seq) return;                             // behind the last sequence: left as they are
+    const int64_t b = f.b, beg = f.beg, end = f.end;
     const int64_t first = ((int64_t)blockIdx.x - ((beg >> kAppendShift) + b)) << kAppendShift;
     const int64_t old = a.lengths[b];
-    if (first >= end - beg || old < 0) return;
+    if (first < 0 || first >= end - beg || old < 0) return;
     const int64_t total = old + (end - beg);
     const int64_t ntok = end - beg - first < (1 << kAppendShift) ? end - beg - first : (1 << kAppendShift);
     constexpr int kPiece = 16 / (int)sizeof(T);

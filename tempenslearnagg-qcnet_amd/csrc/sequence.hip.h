@@ -46,27 +46,59 @@ __device__ __forceinline__ void seq_range(const int64_t *__restrict__ cu, int64_
 }
 
 // Ragged tiles without a host round trip: sequence b owns the tile numbers  start(b) .. start(b + 1) - 1  with
-// start(b) = (cu[b] * rows >> shift) + b, tiles of 2^shift rows.  That is at least ceil(len * rows / tile) numbers for every sequence (the floor of a sum
-// is at least the sum of the floors), at most one too many, and start() needs no prefix sum.  The whole wave searches:
-// 64 probes per step, so 4096 sequences take two dependent loads.  Returns the last b in [0, n_seq] with start(b) <= tile;
-// n_seq itself stands for the rows behind the last sequence.
-__device__ __forceinline__ int64_t find_seq(const int64_t *__restrict__ cu, int64_t n_seq, int64_t n, int64_t rows, int shift,
-                                            int64_t tile, int lane)
+// start(b) = (cu[b] * rows >> shift) + b, tiles of 2^shift rows.  That is at least ceil(len * rows / tile) numbers for every
+// sequence (the floor of a sum is at least the sum of the floors), at most one too many, and start() needs no prefix sum.
+// Number n_seq stands for the rows behind the last sequence.
+//
+// The wave looks for the last b in [0, n_seq] with start(b) <= tile, 64 candidates at a time: first around where b would be if
+// all sequences were of one length (mostly right, so one dependent load), else by narrowing 64-fold.  The boundaries of b come
+// with the last look: beg = cu[b], end = cu[b + 1] (n for n_seq), forced into range as in seq_range.
+struct Found {
+    int64_t b, beg, end;
+};
+__device__ __forceinline__ int64_t wave_get(int64_t v, int lane)
 {
-    int64_t lo = 0, count = n_seq + 1;   // candidates lo .. lo + count - 1; lo always satisfies start(lo) <= tile
-    while (count > 1) {
-        const int64_t step = (count + 63) / 64;
-        const int64_t b = lo + (int64_t)lane * step;
-        const bool in = (int64_t)lane * step < count;
-        const bool ok = in && (clamp64(cu[in ? b : lo], 0, n) * rows >> shift) + b <= tile;
-        const uint64_t hits = __ballot(ok) | 1ull;
-        const int last = 63 - __builtin_clzll(hits);
-        const int64_t next = lo + (int64_t)last * step;
-        const int64_t left = lo + count - next;
-        lo = next;
-        count = left < step ? left : step;
+    const unsigned lo = __builtin_amdgcn_readlane((int)(v & 0xffffffff), lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ Found find_seq(const int64_t *__restrict__ cu, int64_t n_seq, int64_t n, int64_t rows, int shift, int64_t tile,
+                                          int64_t n_tiles, int lane)
+{
+    int64_t lo = 0, count = n_seq + 1;   // candidates lo .. lo + count - 1
+    int64_t base = 0, value = 0;
+    uint64_t hits = 0;
+    const auto look = [&](int64_t from) {
+        const int64_t c = from + lane < n_seq ? from + lane : n_seq;
+        base = from;
+        value = clamp64(cu[c], 0, n);
+        hits = __ballot(from + lane < lo + count && (value * rows >> shift) + c <= tile);
+    };
+    bool found = false;
+    if (count > 64) {
+        int64_t guess = (int64_t)((float)tile * ((float)n_seq / (float)n_tiles)) - 31;
+        guess = clamp64(guess, 0, n_seq - 63);
+        look(guess);
+        if (!(hits & 1) && guess > 0) count = guess;                              // it lies in front
+        else if (hits == ~0ull && guess + 64 <= n_seq) { lo = guess + 63; count = n_seq + 1 - lo; }   // or behind
+        else found = true;
+        while (!found && count > 64) {
+            const int64_t step = (count + 63) / 64, b = lo + (int64_t)lane * step;
+            const bool in = (int64_t)lane * step < count;
+            const bool ok = in && (clamp64(cu[in ? b : lo], 0, n) * rows >> shift) + b <= tile;
+            const int last = 63 - __builtin_clzll(__ballot(ok) | 1ull);
+            const int64_t next = lo + (int64_t)last * step, left = lo + count - next;
+            lo = next;
+            count = left < step ? left : step;
+        }
     }
-    return lo;
+    if (!found) look(lo);
+    const int last = 63 - __builtin_clzll(hits | 1ull);
+    Found f;
+    f.b = base + last;
+    f.beg = wave_get(value, last);
+    f.end = f.b >= n_seq ? n : (last < 63 ? wave_get(value, last + 1) : clamp64(cu[f.b + 1], 0, n));
+    if (f.end < f.beg) f.end = f.beg;
+    return f;
 }
 
 // slot of position p in a cache of `sinks` first tokens and a ring of `window`
