@@ -132,20 +132,24 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // ---------------------------------------------------------------------------------------------------------------------
 // 16 rows per wave, keys straight from memory (float32 of every width; 16-bit types up to 16 features)
 // ---------------------------------------------------------------------------------------------------------------------
-// A wave is on its own: no LDS, no barrier.  For short windows (the agents' 10 steps) every key tile is used by two or three row
+// A wave is on its own: no barrier.  For short windows (the agents' 10 steps) every key tile is used by two or three row
 // tiles at most, so staging would cost more than the cache hits it saves.  A wave keeps its 16 rows and goes through key heads:
 // where its sequence lies, what its rows see and the rows' offsets are found once, and (narrow heads) the next head's rows are
 // requested while this head's are worked on.
 //
 // v_mfma_f32_16x16x4_f32: contraction index = lane >> 4.  A lane loads 4 neighbouring features (16 bytes) of its key and feeds
 // them to 4 products, so product e of piece c contracts features 16 c + 4 g + e.  V^T tile (sb, e) holds features
-// sb SB + VW m + e (m = 0 .. 15): a lane loads VW neighbouring features of a key and ends with 4 VW neighbouring features of
-// its query.
+// sb SB + VW m + e (m = 0 .. 15): a lane ends with 4 VW neighbouring features of its query.  Wide heads load VW neighbouring
+// features of a key for it; of narrow ones that would be loads of 4 or 8 bytes, four times as many instructions as the bytes
+// need, so their V comes like K and is turned in a few hundred bytes of LDS of the wave's own.
 template <class T, int DP> struct Direct {
     static constexpr int VW = DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1);
     static constexpr int SB = 16 * VW, NSB = DP / SB, NT = DP / 16;
     static constexpr int NU = 2, CHUNK = 16 * NU;          // keys of a step
-    static constexpr bool AHEAD = DP <= 32;                // registers for the next step's rows
+    static constexpr bool NARROW = DP <= 32;               // V through LDS; registers for the next step's rows
+    static constexpr int V_STRIDE = DP + 16 / sizeof(T);   // LDS row: the pad spreads the rows of a read over the banks
+    static constexpr int HP = NARROW ? 128 / (DP * (int)sizeof(T)) : 1;                // heads of 128 bytes
+    static constexpr int HEAD_ELEMS = 80 * V_STRIDE, WAVE_ELEMS = NARROW ? HP * HEAD_ELEMS : 4;
 };
 
 template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
@@ -157,6 +161,7 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     using L = Direct<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int NU = L::NU;
+    __shared__ __attribute__((aligned(16))) T turn[4 * L::WAVE_ELEMS];
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
@@ -190,10 +195,11 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
 
     using P4 = Pack<T, 4>;
     using PV = Pack<T, L::VW>;
+    constexpr int NS = L::NARROW ? 1 : 4;                  // V loads of a lane per tile come from its own key, or from four
     struct Place {                                         // of a step's keys
-        OFF k[NU], v[NU][4];
-        int sees[NU][4], seen[NU][4];                      // all bits or none: whether this lane's row sees the score's key; whether
-    };                                                     // the key is inside the range and not masked
+        OFF k[NU], v[NU][NS];
+        int sees[NU][4], seen[NU][NS];                     // all bits or none: whether this lane's row sees the score's key; whether
+    };                                                     // the key of a V load is inside the range and not masked
     const auto locate = [&](int j0) {
         Place x;
         const uint64_t vis = sees.bits(j0);
@@ -202,22 +208,28 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
             const int j = j0 + 16 * u + n;
             const bool in = j < keys.total;
             const int key = keys.key(in ? j : keys.total - 1);
-            const unsigned seen = (unsigned)__ballot(in && (!mask || mask[key] != 0)) >> (4 * g);
+            const bool ok = in && (!mask || mask[key] != 0);
+            const unsigned seen = (unsigned)__ballot(ok) >> (4 * g);
             const unsigned both = seen & (unsigned)(vis >> (16 * u + 4 * g));
             x.k[u] = (OFF)key * (OFF)(a.kr.tok * ES);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int jv = j0 + 16 * u + 4 * g + r;
-                x.v[u][r] = (OFF)keys.key(jv < keys.total ? jv : keys.total - 1) * (OFF)(a.vr.tok * ES);
-                x.sees[u][r] = __builtin_amdgcn_sbfe((int)both, r, 1);
-                x.seen[u][r] = __builtin_amdgcn_sbfe((int)seen, r, 1);
+            for (int r = 0; r < 4; ++r) x.sees[u][r] = __builtin_amdgcn_sbfe((int)both, r, 1);
+            if constexpr (L::NARROW) {
+                x.v[u][0] = (OFF)key * (OFF)(a.vr.tok * ES);
+                x.seen[u][0] = ok ? -1 : 0;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int jv = j0 + 16 * u + 4 * g + r;
+                    x.v[u][r] = (OFF)keys.key(jv < keys.total ? jv : keys.total - 1) * (OFF)(a.vr.tok * ES);
+                    x.seen[u][r] = __builtin_amdgcn_sbfe((int)seen, r, 1);
+                }
             }
         }
         return x;
     };
     struct Rows16 {                                        // 16-key tiles in registers
-        P4 k[NU][DP / 16];
-        PV v[L::AHEAD ? NU : 1][L::NSB][4];
+        P4 k[NU][DP / 16], v[L::NARROW ? NU : 1][DP / 16];
     };
     const bool padded = a.dim < DP;
     const auto four = [&](const char *base, OFF off, int c) {   // features 16 c + 4 g ..
@@ -236,13 +248,11 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         for (int u = 0; u < NU; ++u)
 #pragma unroll
             for (int c = 0; c < DP / 16; ++c) y.k[u][c] = four(kb + kvh * a.kr.head * ES, x.k[u], c);
-        if constexpr (L::AHEAD) {
+        if constexpr (L::NARROW) {
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
-                for (int sb = 0; sb < L::NSB; ++sb)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) y.v[u][sb][r] = value(x, kvh, u, sb, r);
+                for (int c = 0; c < DP / 16; ++c) y.v[u][c] = four(vb + kvh * a.vr.head * ES, x.v[u][0], c);
         }
         return y;
     };
@@ -295,7 +305,12 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
             }
         return sum;
     };
-    const auto accumulate = [&](const Place &x, const Rows16 &rows, int kvh, const f32x4 (&s)[NU], f32x4 (&o)[L::NT]) {
+    // bits of x where the key counts, else 0: 0 times what a masked key holds must stay 0
+    const auto keep = [&](T x, int bits) {
+        if constexpr (F32) return __builtin_bit_cast(float, __builtin_bit_cast(int, x) & bits);
+        else return __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(uint16_t, x) & bits));
+    };
+    const auto accumulate = [&](const Place &x, int kvh, const f32x4 (&s)[NU], f32x4 (&o)[L::NT], const T *turned) {
 #pragma unroll
         for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -303,13 +318,13 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 PV v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    if constexpr (L::AHEAD) v[r] = rows.v[u][sb][r];
-                    else v[r] = value(x, kvh, u, sb, r);
-                    if (mask) {                            // 0 times what a masked key holds must stay 0
+                    if constexpr (L::NARROW) {
+                        v[r] = *reinterpret_cast<const PV *>(turned + (16 * u + 4 * g + r) * L::V_STRIDE + sb * L::SB + L::VW * n);
+                    } else {
+                        v[r] = value(x, kvh, u, sb, r);
+                        if (mask) {
 #pragma unroll
-                        for (int e = 0; e < L::VW; ++e) {
-                            if constexpr (F32) v[r].e[e] = __builtin_bit_cast(float, __builtin_bit_cast(int, v[r].e[e]) & x.seen[u][r]);
-                            else v[r].e[e] = __builtin_bit_cast(T, (uint16_t)(__builtin_bit_cast(uint16_t, v[r].e[e]) & x.seen[u][r]));
+                            for (int e = 0; e < L::VW; ++e) v[r].e[e] = keep(v[r].e[e], x.seen[u][r]);
                         }
                     }
                 }
@@ -328,6 +343,8 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 }
             }
     };
+    // LDS of the wave's own: its accesses are done in order; only the compiler is to keep them apart
+    const auto in_order = [&]() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
     const auto finish = [&](int kvh, float l, f32x4 (&o)[L::NT]) {
         const float inv = inverse_sum(quarters_sum(l));
         bool bad = false;
@@ -370,27 +387,89 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
         for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
     };
 
-    if (L::AHEAD && chunks == 1) {
-        // all keys in one step: found once for all heads; no running maximum; the next head's rows in the other set of registers
-        const Place x = locate(0);
-        Rows16 ra = load(x, h0), rb;
-        Query qa = load_q(h0), qc;
-        const auto head = [&](int kvh, const Rows16 &rows, const Query &q, Rows16 &rows_next, Query &q_next) {
-            const int next = kvh + 1 < h1 ? kvh + 1 : kvh;      // the last head's are read again: no branch around loads
-            rows_next = load(x, next);
-            q_next = load_q(next);
-            f32x4 s[NU], o[L::NT];
-            clear(o);
-            const float m = scores(x, rows, q, s);
-            const float l = softmax(s, m);
-            accumulate(x, rows, kvh, s, o);
-            finish(kvh, l, o);
-        };
-        for (int kvh = h0; kvh < h1; kvh += 2) {
-            head(kvh, ra, qa, rb, qc);
-            if (kvh + 1 < h1) head(kvh + 1, rb, qc, ra, qa);
+    if constexpr (L::NARROW) {
+        if (chunks == 1) {
+            // All keys in one step: found once for all heads, and no running maximum.  A load covers 128 bytes of 8 rows, that is
+            // as many heads as that takes: with 64 bytes of 16 rows (the operands' own layout) each request fills half a cache
+            // line, and the number of requests in flight is what such a wave is short of.  LDS turns rows into operands; the next
+            // heads' rows are requested as soon as these are in LDS.
+            constexpr int PPH = DP * ES / 16, HP = L::HP, E16 = 16 / ES;     // 16-byte pieces of a head's row, heads, elements
+            const int lr = lane >> 3, hp = (lane & 7) / PPH, d = (lane & 7) % PPH * E16;
+            const bool past = padded && d >= a.dim;
+            const uint64_t vis = sees.bits(0);
+            const int jc = lane < keys.total ? lane : keys.total - 1;
+            const unsigned seen = (unsigned)__ballot(lane < keys.total && (!mask || mask[keys.key(jc)] != 0));
+            Place x = {};
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x.sees[u][r] = __builtin_amdgcn_sbfe((int)((seen & (unsigned)vis) >> (16 * u + 4 * g)), r, 1);
+            OFF qo[2], ko[4], vo[4];
+            int counts[4];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = lr + 8 * i, own = 16 * wave + (r < last ? r : last);
+                qo[i] = (OFF)((t.token(own, a.group) * a.qr.tok + t.sub(own, a.group) * a.qr.head + (past ? 0 : d)) * ES);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int j = lr + 8 * i, key = keys.key(j < keys.total ? j : keys.total - 1);
+                ko[i] = (OFF)key * (OFF)(a.kr.tok * ES) + (OFF)((past ? 0 : d) * ES);
+                vo[i] = (OFF)key * (OFF)(a.vr.tok * ES) + (OFF)((past ? 0 : d) * ES);
+                counts[i] = (seen >> j) & 1 ? -1 : 0;
+            }
+            u32x4 qx[2], kx[4], vx[4];
+            const auto request = [&](int first) {
+                const int kvh = first + hp < h1 ? first + hp : h1 - 1;
+                const OFF qh = (OFF)((int64_t)kvh * a.group * a.qr.head * ES), kh = (OFF)(kvh * a.kr.head * ES), vh = (OFF)(kvh * a.vr.head * ES);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) qx[i] = *reinterpret_cast<const u32x4 *>(qb + (OFF)(qo[i] + qh));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kx[i] = *reinterpret_cast<const u32x4 *>(kb + (OFF)(ko[i] + kh));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vx[i] = *reinterpret_cast<const u32x4 *>(vb + (OFF)(vo[i] + vh));
+            };
+            T *mine = turn + wave * L::WAVE_ELEMS;             // [head][16 rows of q, 32 of k, 32 of v][V_STRIDE]
+            request(h0);
+            for (int first = h0; first < h1; first += HP) {
+                T *to = mine + hp * L::HEAD_ELEMS + d;
+                const u32x4 none = {0, 0, 0, 0};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4 *>(to + (lr + 8 * i) * L::V_STRIDE) = past ? none : qx[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<u32x4 *>(to + (16 + lr + 8 * i) * L::V_STRIDE) = past ? none : kx[i];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    u32x4 y = vx[i];
+                    if (mask) y &= (uint32_t)counts[i];        // 0 times what a masked key holds must stay 0
+                    *reinterpret_cast<u32x4 *>(to + (48 + lr + 8 * i) * L::V_STRIDE) = y;
+                }
+                in_order();
+                if (first + HP < h1) request(first + HP);
+#pragma unroll
+                for (int i = 0; i < HP; ++i) {
+                    const int kvh = first + i;
+                    if (kvh >= h1) break;
+                    const T *own = mine + i * L::HEAD_ELEMS;
+                    Rows16 rows;
+                    Query q;
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c) {
+                        q.q[c] = *reinterpret_cast<const P4 *>(own + n * L::V_STRIDE + 16 * c + 4 * g);
+#pragma unroll
+                        for (int u = 0; u < NU; ++u) rows.k[u][c] = *reinterpret_cast<const P4 *>(own + (16 + 16 * u + n) * L::V_STRIDE + 16 * c + 4 * g);
+                    }
+                    f32x4 s[NU], o[L::NT];
+                    clear(o);
+                    const float m = scores(x, rows, q, s);
+                    const float l = softmax(s, m);
+                    accumulate(x, kvh, s, o, own + 48 * L::V_STRIDE);
+                    finish(kvh, l, o);
+                }
+                in_order();
+            }
+            return;
         }
-        return;
     }
     for (int kvh = h0; kvh < h1; ++kvh) {
         f32x4 s[NU], o[L::NT];
@@ -411,7 +490,23 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 m = mn;
             }
             l += softmax(s, m);
-            accumulate(x, rows, kvh, s, o);
+            T *mine = turn + wave * L::WAVE_ELEMS;
+            if constexpr (L::NARROW) {
+#pragma unroll
+                for (int u = 0; u < NU; ++u)
+#pragma unroll
+                    for (int c = 0; c < DP / 16; ++c) {
+                        P4 y = rows.v[u][c];
+                        if (mask) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) y.e[e] = keep(y.e[e], x.seen[u][0]);
+                        }
+                        *reinterpret_cast<P4 *>(mine + (16 * u + n) * L::V_STRIDE + 16 * c + 4 * g) = y;
+                    }
+                in_order();
+            }
+            accumulate(x, kvh, s, o, mine);
+            if constexpr (L::NARROW) in_order();
         }
         finish(kvh, l, o);
     }
