@@ -345,7 +345,9 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
     };
     // LDS of the wave's own: its accesses are done in order; only the compiler is to keep them apart
     const auto in_order = [&]() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
-    const auto finish = [&](int kvh, float l, f32x4 (&o)[L::NT]) {
+    // o / l; a bit for each row that did not come out finite.  A value that is not finite, of a key that some rows of the tile see
+    // and others do not, reaches the others as 0 * inf: such rows are formed again key by key.
+    const auto divide = [&](float l, f32x4 (&o)[L::NT]) {
         const float inv = inverse_sum(quarters_sum(l));
         bool bad = false;
 #pragma unroll
@@ -355,32 +357,40 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 o[i][r] *= inv;
                 bad |= !(fabsf(o[i][r]) < INFINITY);
             }
-        unsigned repair = 0;
-        if (const uint64_t b = __ballot(bad && n <= last)) repair = (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
-        if (n <= last && !((repair >> n) & 1)) {
-            char *out = ob + (int64_t)kvh * a.group * a.dim * ES;
-#pragma unroll
-            for (int sb = 0; sb < L::NSB; ++sb) {
-                const int d = sb * L::SB + 4 * L::VW * g;
-#pragma unroll
-                for (int part = 0; part < L::VW; ++part) { // 4 features each
-                    if (d + 4 * part >= a.dim) break;
-                    P4 w;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int f = 4 * part + x;        // feature f of the lane's 4 VW: r = f / VW, e = f % VW
-                        w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW]);
-                    }
-                    *reinterpret_cast<P4 *>(out + (OFF)(o_off + (OFF)((d + 4 * part) * ES))) = w;
-                }
-            }
-        }
-        // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
-        // Rows that came out not finite are formed again key by key.
-        for (; repair; repair &= repair - 1) {
-            const int r = 16 * wave + __builtin_ctz(repair), token = t.token(r, a.group);
+        const uint64_t b = __ballot(bad && n <= last);
+        return (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
+    };
+    const auto again = [&](int kvh, unsigned rows) {
+        for (; rows; rows &= rows - 1) {
+            const int r = 16 * wave + __builtin_ctz(rows), token = t.token(r, a.group);
             row_by_wave<T>(a, t.k_beg, token + t.shift, t.q_beg + token, kvh * a.group + t.sub(r, a.group), lane);
         }
+    };
+    // the lane's 4 VW neighbouring features per sb, four at a time, to to(feature)
+    const auto write = [&](const f32x4 (&o)[L::NT], auto to) {
+#pragma unroll
+        for (int sb = 0; sb < L::NSB; ++sb) {
+            const int d = sb * L::SB + 4 * L::VW * g;
+#pragma unroll
+            for (int part = 0; part < L::VW; ++part) {
+                if (d + 4 * part >= a.dim) break;
+                P4 w;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int f = 4 * part + x;            // feature f of the lane's 4 VW: r = f / VW, e = f % VW
+                    w.e[x] = from_f32<T>(o[sb * L::VW + f % L::VW][f / L::VW]);
+                }
+                *reinterpret_cast<P4 *>(to(d + 4 * part)) = w;
+            }
+        }
+    };
+    const auto finish = [&](int kvh, float l, f32x4 (&o)[L::NT]) {
+        const unsigned bad = divide(l, o);
+        if (n <= last && !((bad >> n) & 1)) {
+            char *out = ob + (int64_t)kvh * a.group * a.dim * ES;
+            write(o, [&](int d) { return out + (OFF)(o_off + (OFF)(d * ES)); });
+        }
+        again(kvh, bad);
     };
     const auto clear = [&](f32x4 (&o)[L::NT]) {
 #pragma unroll
@@ -404,12 +414,13 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
             for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) x.sees[u][r] = __builtin_amdgcn_sbfe((int)((seen & (unsigned)vis) >> (16 * u + 4 * g)), r, 1);
-            OFF qo[2], ko[4], vo[4];
+            OFF qo[2], oo[2], ko[4], vo[4];
             int counts[4];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = lr + 8 * i, own = 16 * wave + (r < last ? r : last);
                 qo[i] = (OFF)((t.token(own, a.group) * a.qr.tok + t.sub(own, a.group) * a.qr.head + (past ? 0 : d)) * ES);
+                oo[i] = (OFF)((((int64_t)t.token(own, a.group) * a.hq + t.sub(own, a.group)) * a.dim + d) * ES);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -446,6 +457,7 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                 }
                 in_order();
                 if (first + HP < h1) request(first + HP);
+                unsigned bad[HP] = {};
 #pragma unroll
                 for (int i = 0; i < HP; ++i) {
                     const int kvh = first + i;
@@ -464,9 +476,26 @@ __global__ __launch_bounds__(256) void attn_window_direct_kernel(Args a, int64_t
                     const float m = scores(x, rows, q, s);
                     const float l = softmax(s, m);
                     accumulate(x, kvh, s, o, own + 48 * L::V_STRIDE);
-                    finish(kvh, l, o);
+                    bad[i] = divide(l, o);
+                    // rows go out as they came in, through the place of q
+                    in_order();
+                    write(o, [&](int f) { return mine + i * L::HEAD_ELEMS + n * L::V_STRIDE + f; });
                 }
                 in_order();
+                if (first + hp < h1 && !past) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (lr + 8 * i <= last)
+                            *reinterpret_cast<u32x4 *>(ob + (OFF)(oo[i] + (OFF)((first + hp) * a.group * a.dim * ES))) =
+                                *reinterpret_cast<const u32x4 *>(to + (lr + 8 * i) * L::V_STRIDE);
+                }
+                in_order();
+#pragma unroll
+                for (int i = 0; i < HP; ++i)
+                    if (bad[i]) {
+                        __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): behind the stores above
+                        again(first + i, bad[i]);
+                    }
             }
             return;
         }
