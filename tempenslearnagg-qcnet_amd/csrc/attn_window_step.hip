@@ -77,18 +77,20 @@ struct StepArgs {
 //
 // HBM-bound: every filled slot is read once.  K goes straight into registers as the A operand (a lane reads 16 bytes of a slot,
 // four lanes 64).  V has to be transposed: 16-bit rows pass through LDS that belongs to the wave alone (no barrier) and come
-// back by transposing reads; float32 needs no transposition, a lane reads the features it multiplies.
+// back by transposing reads.  Of float32 a lane reads the features it multiplies: straight from memory where a row is 256 bytes or
+// more, through LDS where that would be loads of 4 or 8 bytes.
 // The new token is read from the inputs, never from its slot, which another block of this launch is writing.
 template <class T, int DP> struct Step {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NU = DP <= 32 ? 4 : 2, CHUNK = 16 * NU;                        // slots of a chunk: narrow heads take 64
     static constexpr int VW = !F32 ? 1 : (DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1));   // float32: features of a lane's V load
     static constexpr int SB = 16 * VW, NSB = DP / SB;
-    static constexpr int PIECES = DP / 8;                 // 16-bit: 16-byte pieces of a row
+    static constexpr bool TURN = !F32 || DP <= 32;         // V passes through LDS
+    static constexpr int PIECES = DP * (int)sizeof(T) / 16, PIECE = 16 / (int)sizeof(T);   // 16-byte pieces of a row, elements of one
     static constexpr int O_STRIDE = DP + 4;               // floats: a row's pad keeps 16 heads off one bank
-    static constexpr int V_BYTES = F32 ? 0 : CHUNK * DP * 2, O_BYTES = 64 * O_STRIDE;   // a chunk of V, then 16 rows of O
+    static constexpr int V_ROW = F32 ? O_STRIDE * 4 : DP * 2;                           // bytes of a V row in LDS
+    static constexpr int V_BYTES = TURN ? CHUNK * V_ROW : 0, O_BYTES = 64 * O_STRIDE;   // a chunk of V, then 16 rows of O
     static constexpr int WAVE_BYTES = V_BYTES > O_BYTES ? V_BYTES : O_BYTES;
-    static constexpr bool V_AHEAD = F32 && DP <= 32;      // float32: V is requested with K where registers allow
 };
 
 // 8 rows x 32 bytes of a transposing read (half a wave) cover all banks
@@ -150,27 +152,15 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
         const int64_t cl = j0 + lane;
         const bool in = lane < L::CHUNK && cl < t.c1;
         const bool ok = in && (cl == t.slot ? new_seen : (!mask || mask[in ? cl : t.c1 - 1] != 0));
-        constexpr int NV = L::F32 ? 1 : (L::CHUNK * L::PIECES + 63) / 64;
+        constexpr int NV = L::TURN ? (L::CHUNK * L::PIECES + 63) / 64 : 1;
         u32x4 vf[NV];
         using PV = Pack<T, L::VW>;
-        PV va[L::V_AHEAD ? L::NU : 1][L::NSB][4];
-        const auto load_v = [&](int u, int sb, int r) {        // float32: VW features of slot 16 u + 4 g + r
-            const int d = sb * L::SB + L::VW * n;
-            return *reinterpret_cast<const PV *>(row_of(vc, vn, 16 * u + 4 * g + r) + (d < a.dim ? d : 0));
-        };
-        if constexpr (!L::F32) {
+        if constexpr (L::TURN) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int x = lane + 64 * i, r = x / L::PIECES;
-                vf[i] = piece(row_of(vc, vn, r), x % L::PIECES * 8);
+                vf[i] = piece(row_of(vc, vn, r), x % L::PIECES * L::PIECE);
             }
-        } else if constexpr (L::V_AHEAD) {
-#pragma unroll
-            for (int u = 0; u < L::NU; ++u)
-#pragma unroll
-                for (int sb = 0; sb < L::NSB; ++sb)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) va[u][sb][r] = load_v(u, sb, r);
         }
         const uint64_t seen = __ballot(ok);
         f32x4 s[L::NU];
@@ -189,14 +179,16 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
                 }
             }
         }
-        if constexpr (!L::F32) {
+        if constexpr (L::TURN) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int x = lane + 64 * i, r = x / L::PIECES;
+                const int x = lane + 64 * i, r = x / L::PIECES, c = x % L::PIECES;
                 // 0 times what a masked slot holds must stay 0
                 const u32x4 v = (seen >> r) & 1 ? vf[i] : u32x4{0, 0, 0, 0};
-                *reinterpret_cast<u32x4 *>(lds + (r * L::PIECES + v_piece<DP>(r, x % L::PIECES)) * 16) = v;
+                *reinterpret_cast<u32x4 *>(lds + r * L::V_ROW + (L::F32 ? c : v_piece<DP>(r, c)) * 16) = v;
             }
+            // the wave's own LDS: these writes are done in order before the reads below; only the compiler is to keep them apart
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         float top = -INFINITY;
 #pragma unroll
@@ -236,9 +228,13 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
                     PV v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        if constexpr (L::V_AHEAD) v[r] = va[u][sb][r];
-                        else v[r] = load_v(u, sb, r);
-                        if (!((w >> r) & 1)) v[r] = PV{};
+                        const int d = sb * L::SB + L::VW * n, c = 16 * u + 4 * g + r;
+                        if constexpr (L::TURN) {
+                            v[r] = *reinterpret_cast<const PV *>(lds + c * L::V_ROW + d * (int)sizeof(T));
+                        } else {
+                            v[r] = *reinterpret_cast<const PV *>(row_of(vc, vn, c) + (d < a.dim ? d : 0));
+                            if (!((w >> r) & 1)) v[r] = PV{};
+                        }
                     }
 #pragma unroll
                     for (int e = 0; e < L::VW; ++e)
@@ -249,8 +245,6 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
             }
         } else {
             using V8 = typename Mat<T>::V8;
-            // the wave's own LDS: its writes above are done in order before these reads; only the compiler is to keep them apart
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int half = 0; half < L::NU / 2; ++half) {
                 V8 pb;
@@ -260,13 +254,13 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
 #pragma unroll
                 for (int dt = 0; dt < DP / 16; ++dt) {
                     const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
-                    const uint2 x = lds_read_transposed(lds + (r * L::PIECES + v_piece<DP>(r, c)) * 16 + byte);
-                    const uint2 y = lds_read_transposed(lds + ((r + 16) * L::PIECES + v_piece<DP>(r + 16, c)) * 16 + byte);
+                    const uint2 x = lds_read_transposed(lds + r * L::V_ROW + v_piece<DP>(r, c) * 16 + byte);
+                    const uint2 y = lds_read_transposed(lds + (r + 16) * L::V_ROW + v_piece<DP>(r + 16, c) * 16 + byte);
                     o[dt] = Mat<T>::mul16(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+        if constexpr (L::TURN) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
     l = quarters_sum(l);
 }

@@ -28,6 +28,7 @@ _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}            # QCN
 MAX_HEAD_DIM = 128
 _MOST = (1 << 62) - 1
 _MOST_TOK = 1 << 24      # token stride in elements
+_NO_SECTIONS = (0,) * 8
 
 # the argument structs of include/qcnet_hip.h (8-byte fields: no padding)
 _ROTARY_ARGS = struct.Struct('=27q').pack
@@ -76,11 +77,12 @@ def _in_place(t: torch.Tensor):
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:
-    if not torch.is_tensor(t):
+    if not isinstance(t, torch.Tensor):
         raise TypeError('%s must be a tensor' % name)
-    if t.dtype not in _DTYPES:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
         raise TypeError('%s has dtype %s, expected float32, float16 or bfloat16' % (name, t.dtype))
-    return _DTYPES[t.dtype]
+    return code
 
 
 def _on_device(index: int, fn, *args):
@@ -93,7 +95,11 @@ def _on_device(index: int, fn, *args):
 
 def _launch(index: int, what: str, args: bytes) -> None:
     """A launch on the tensors' own device and its current stream."""
-    status = _on_device(index, getattr(_lib.lib(), what), args, torch._C._cuda_getCurrentRawStream(index))
+    fn = getattr(_lib.lib(), what)
+    if torch._C._cuda_getDevice() == index:
+        status = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        status = _on_device(index, fn, args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, what)
 
@@ -141,40 +147,43 @@ def _even_rows(t):
            _rotary_embed_fake, SEQUENCE_OP_NAMES)
 def _rotary_embed(q, k, pos, freqs, sections, interleaved, inverse):
     code = _dtype_code(q, 'q')
-    _rows(q, 'q', q.dtype, q.device)
-    n, hq, dim = q.shape
-    index = q.get_device()
+    dtype, index, shape = q.dtype, q.get_device(), q.shape
+    if index < 0 or len(shape) != 3:
+        _rows(q, 'q', dtype, q.device)
+    n, hq, dim = shape
     if dim % 2 or not 2 <= dim <= 256:
         raise _lib.QcnError('head dim %d is not supported (even, 2 .. 256)' % dim)
     pairs, axes = sum(sections), len(sections)
     if not 1 <= axes <= 8 or min(sections) < 0 or pairs < 1 or 2 * pairs > dim:
         raise ValueError('sections %s: one to eight axes, at least one pair, at most dim / 2 = %d pairs' % (list(sections), dim // 2))
-    if not torch.is_tensor(pos) or pos.dtype not in _POS_TYPES:
+    pos_type = _POS_TYPES.get(pos.dtype) if isinstance(pos, torch.Tensor) else None
+    if pos_type is None:
         raise TypeError('pos must be a float32, int32 or int64 tensor')
     if not _is(pos, pos.dtype, index, (n, axes)):
         _require(pos, 'pos', pos.dtype, q.device, (n, axes))
     if not _is(freqs, torch.float32, index, (pairs,)):
         _require(freqs, 'freqs', torch.float32, q.device, (pairs,))
-    hk = 0
+    q, qs = _even_rows(q)
+    q_out = q.new_empty(shape)
+    hk = kp = ks0 = ks1 = k_out_ptr = 0
+    outs = [q_out]
     if k is not None:
-        _rows(k, 'k', q.dtype, q.device)
-        hk = k.size(1)
-        if k.size(0) != n or k.size(2) != dim:
+        if not (isinstance(k, torch.Tensor) and k.dtype is dtype and k.get_device() == index and k.dim() == 3):
+            _rows(k, 'k', dtype, q.device)
+        nk, hk, dk = k.shape
+        if nk != n or dk != dim:
             raise ValueError('k has shape %s, expected (%d, heads, %d)' % (tuple(k.shape), n, dim))
         if hk == 0:
             raise ValueError('k has no heads: pass None')
-    q, qs = _even_rows(q)
-    outs = [q.new_empty((n, hq, dim))]
-    kp = ks0 = ks1 = k_out = 0
-    if hk:
         k, (ks0, ks1, _) = _even_rows(k)
         kp = k.data_ptr()
-        outs.append(q.new_empty((n, hk, dim)))
-        k_out = outs[1].data_ptr()
+        k_out = q.new_empty((n, hk, dim))
+        k_out_ptr = k_out.data_ptr()
+        outs.append(k_out)
     if n and (hq or hk):
         _launch(index, 'qcn_rotary_embed', _ROTARY_ARGS(
-            q.data_ptr(), qs[0], qs[1], hq, kp, ks0, ks1, hk, n, dim, code, pos.data_ptr(), _POS_TYPES[pos.dtype], axes,
-            *sections, *([0] * (8 - axes)), freqs.data_ptr(), interleaved, inverse, outs[0].data_ptr(), k_out))
+            q.data_ptr(), qs[0], qs[1], hq, kp, ks0, ks1, hk, n, dim, code, pos.data_ptr(), pos_type, axes,
+            *sections, *_NO_SECTIONS[axes:], freqs.data_ptr(), interleaved, inverse, q_out.data_ptr(), k_out_ptr))
     return outs
 
 
