@@ -12,6 +12,7 @@ whose features are contiguous and 16-byte aligned are read in place, anything el
 are float32 and every output is rounded once.  All of them launch on torch's current stream of the tensors' device, allocate
 their outputs with torch, never synchronise, and can be captured into graphs.
 """
+import functools
 import math
 import struct
 from typing import List, Optional, Sequence, Tuple
@@ -102,6 +103,18 @@ def _launch(index: int, what: str, args: bytes) -> None:
         status = _on_device(index, fn, args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _lib.check(status, what)
+
+
+@functools.lru_cache(maxsize=1024)
+def _step_workspace(index, batch, hq, hk, dim, window, sinks) -> int:
+    """Bytes that a step of these sizes needs on this device; a serving loop asks for the same sizes every time."""
+    return _on_device(index, _lib.lib().qcn_attn_window_step_workspace_bytes, batch, hq, hk, dim, window, sinks)
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_workspace(index, code, n_seq, nq, nk, hq, hk, dim, window, sinks) -> int:
+    args = _WINDOW_ARGS(*[0] * 12, n_seq, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), 0.0, 0, 0, 0)
+    return _on_device(index, _lib.lib().qcn_attn_window_workspace_bytes, args)
 
 
 def _scale(scale: Optional[float], dim: int) -> float:
@@ -262,12 +275,13 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
     if nq:
         args = (q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
                 n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr())
-        packed = _WINDOW_ARGS(*args, 0, 0)
-        ws_bytes = _on_device(index, _lib.lib().qcn_attn_window_workspace_bytes, packed)
-        if ws_bytes:
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=k.device)
-            packed = _WINDOW_ARGS(*args, ws.data_ptr(), ws_bytes)
-        _launch(index, 'qcn_attn_window', packed)
+        ws_ptr = ws_bytes = 0
+        if code:                                            # 16-bit types: keys split over blocks when query tokens are few
+            ws_bytes = _window_workspace(index, code, n_cu - 1, nq, nk, hq, hk, dim, window, sinks)
+            if ws_bytes:
+                ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
+                ws_ptr = ws.data_ptr()
+        _launch(index, 'qcn_attn_window', _WINDOW_ARGS(*args, ws_ptr, ws_bytes))
     return out
 
 
@@ -378,8 +392,8 @@ def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_
     v, vs = _in_place(v)
     out = q.new_empty((batch, hq, dim))
     if batch:
-        ws_bytes = _on_device(index, _lib.lib().qcn_attn_window_step_workspace_bytes, batch, hq, hk, dim, window, sinks)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=k.device) if ws_bytes else None
+        ws_bytes = _step_workspace(index, batch, hq, hk, dim, window, sinks)
+        ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         _launch(index, 'qcn_attn_window_step', _STEP_ARGS(
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], lengths.data_ptr(), mask_ptr, batch, hq,
             hk, dim, code, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache_ptr, out.data_ptr(),
