@@ -456,16 +456,16 @@ __global__ __launch_bounds__(256) void gru_pair_kernel(const float *__restrict__
     f32x16 aAr, aAz, aAn, aBr = {}, aBz = {}, aBn = {};   // (B's are first written by Y(0); X(0) only names them)
     phase(on, off, 0, aAr, aAz, aAn, 1, 0, aBr, aBz, aBn, hB);            // X(0): nothing to put under it
     phase_barrier();                                                      // Y(0) rewrites the image X(0) has read
+    // The last X is a whole phase too, its products unused (they run under the gates): without it the loop's two phases are all
+    // the code there is.  Peeled off the end, two more copies of them cost 72 bytes of spills, and the compiler (ROCm 7.2, no
+    // packed fp32 instructions) brought one spilled weight fragment back by three of its four registers.
 #pragma unroll 1
-    for (int t = 0; t < n_steps - 1; ++t) {
+    for (int t = 0; t < n_steps; ++t) {
         phase(on, on, 1, aBr, aBz, aBn, 0, t, aAr, aAz, aAn, hA);         // Y(t)
         phase_barrier();
-        phase(on, on, 0, aAr, aAz, aAn, 1, t, aBr, aBz, aBn, hB);         // X(t + 1)
+        phase(on, on, 0, aAr, aAz, aAn, 1, t, aBr, aBz, aBn, hB);         // X(t + 1); past the last step only its gates count
         phase_barrier();
     }
-    phase(on, on, 1, aBr, aBz, aBn, 0, n_steps - 1, aAr, aAz, aAn, hA);   // Y(n_steps - 1)
-    phase_barrier();
-    phase(off, on, 0, aAr, aAz, aAn, 1, n_steps - 1, aBr, aBz, aBn, hB);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                      // no copy may land after the workgroup has gone
 
 #pragma unroll
