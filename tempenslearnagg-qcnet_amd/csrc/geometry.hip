@@ -5,8 +5,10 @@
 //   r  = [ |dp|_2,  atan2(c x dp, c . dp) with c = (cos, sin)(head_dst[dst]),  wrap(head_src[src] - head_dst[dst]) (, extra) ]
 // One thread per edge; HBM-bound on the index and output streams (16 B of indices + 12-16 B out per edge; the gathered
 // positions / headings are cache-served).  Every operation is the individually rounded fp32 operation of the reference's
-// elementwise form (no fma contraction), and the dot product keeps the reference's reduction form 0 + a + b: for a zero
-// dp the products can be -0 and (-0) + (-0) = -0 would turn atan2(0, .) from 0 into pi.
+// elementwise form (contraction off by pragma: HIP's __fmul_rn and __fadd_rn are the plain operators, which hipcc contracts,
+// and a cross product that should be 0 then keeps the residue of one product: atan2 turns its sign into + or - pi), and the
+// dot product keeps the reference's reduction form 0 + a + b: for a zero dp the products can be -0 and (-0) + (-0) = -0 would
+// turn atan2(0, .) from 0 into pi.
 #include "common.hip.h"
 
 namespace {
@@ -18,23 +20,24 @@ __global__ __launch_bounds__(256) void rel_geometry_kernel(const float *__restri
                                                            const int64_t *__restrict__ extra, int64_t n_edges, int pos_stride_src,
                                                            int pos_stride_dst, float *__restrict__ out)
 {
+#pragma clang fp contract(off)
     const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (e >= n_edges) return;
     const int64_t j = src[e], i = dst[e];
-    const float dx = __fsub_rn(pos_src[j * pos_stride_src], pos_dst[i * pos_stride_dst]);
-    const float dy = __fsub_rn(pos_src[j * pos_stride_src + 1], pos_dst[i * pos_stride_dst + 1]);
+    const float dx = pos_src[j * pos_stride_src] - pos_dst[i * pos_stride_dst];
+    const float dy = pos_src[j * pos_stride_src + 1] - pos_dst[i * pos_stride_dst + 1];
     const float hd = head_dst[i];
     const float cx = cosf(hd), cy = sinf(hd);
-    const float dist = sqrtf(__fadd_rn(__fmul_rn(dx, dx), __fmul_rn(dy, dy)));
-    const float cross = __fsub_rn(__fmul_rn(cx, dy), __fmul_rn(cy, dx));
-    const float dot = __fadd_rn(__fadd_rn(0.0f, __fmul_rn(cx, dx)), __fmul_rn(cy, dy));
+    const float dist = sqrtf(dx * dx + dy * dy);
+    const float cross = cx * dy - cy * dx;
+    const float dot = (0.0f + cx * dx) + cy * dy;
     const float ang = atan2f(cross, dot);
     // wrap_angle: remainder(a + pi, 2 pi) - pi with the floor-mod of torch.remainder
     const float kPi = 3.14159265358979323846f, kTwoPi = 6.28318530717958647692f;
-    const float a = __fadd_rn(__fsub_rn(head_src[j], hd), kPi);
+    const float a = (head_src[j] - hd) + kPi;
     float m = fmodf(a, kTwoPi);
-    if (m != 0.0f && m < 0.0f) m = __fadd_rn(m, kTwoPi);
-    const float wrapped = __fadd_rn(m, -kPi);
+    if (m != 0.0f && m < 0.0f) m = m + kTwoPi;
+    const float wrapped = m + -kPi;
     if (extra != nullptr) {
         float4 o = make_float4(dist, ang, wrapped, (float)extra[e]);
         *reinterpret_cast<float4 *>(out + 4 * e) = o;
