@@ -495,7 +495,7 @@ int qcn_nms_select_f32(const float *traj, const float *conf, const float *gt, in
  * (modules/qcnet_agent_encoder.py:129-140: a causal band of time_span steps) for token sequences of any width.
  *
  * Row tensors are [tokens, heads, dim] with strides in ELEMENTS; the features of a head are contiguous and rows start on
- * 16-byte boundaries (rotary: on multiples of any access width, it adapts).  dim: a multiple of 8, 8 .. 128 (rotary: even,
+ * 16-byte boundaries (rotary: on multiples of any access width, it adapts).  Strides are not negative.  dim: a multiple of 8, 8 .. 128 (rotary: even,
  * 2 .. 256).  Outputs are contiguous.  Boundaries `cu` are int64 [n_seq + 1], ascending, cu[0] = 0.  Accumulation, softmax
  * statistics and rotations are fp32, angles fp64; each output is rounded once.
  */
@@ -560,8 +560,8 @@ int qcn_attn_window(const qcn_attn_window_args *args, void *stream);
 /* The cache of that attention: [n_seq, n_kv_heads, sinks + window, dim] contiguous; position p in slot p (p < sinks) or
  * sinks + (p - sinks) % window; mask_cache uint8 [n_seq, sinks + window] (NULL: every token is visible).
  * append: sequence b brings cu[b + 1] - cu[b] tokens behind the lengths[b] (int64) it has; lengths is not changed (several
- * layers share it).  Tokens that fall out of the window within the call are not written; sequences with lengths[b] < 0 and
- * rows behind cu[n_seq] are left alone.  key_mask uint8 [n_tokens] (NULL: 1) goes into mask_cache. */
+ * layers share it).  Tokens that fall out of the window within the call are not written; sequences with lengths[b] < 0 (or
+ * above 2^62) and rows behind cu[n_seq] are left alone.  key_mask uint8 [n_tokens] (NULL: 1) goes into mask_cache. */
 typedef struct {
     const void *k;
     int64_t k_strides[2];
@@ -577,7 +577,8 @@ typedef struct {
 int qcn_window_cache_append(const qcn_window_cache_append_args *args, void *stream);
 
 /* One new token per sequence: k / v [batch, n_kv_heads, dim] go into the cache at position lengths[b], q [batch, n_q_heads,
- * dim] attends to what that position sees.  lengths[b] < 0: the row is not in use, its output is 0 and its cache untouched.
+ * dim] attends to what that position sees.  lengths[b] < 0 (or above 2^62): the row is not in use, its output is 0 and its cache
+ * untouched.
  * lengths is not changed.  key_mask uint8 [batch]: whether the new token is visible.  The workspace's contents do not outlive
  * the call's work on its stream. */
 typedef struct {

@@ -564,7 +564,7 @@ template <int LS> __device__ __forceinline__ int v_piece(int row, int piece)
     return piece ^ (LS == 128 ? (row & 3) << 2 : LS == 64 ? ((row >> 1) & 1) << 2 : 0);
 }
 
-constexpr int64_t kMost = ((int64_t)1 << 31) - 1;   // positions are 32-bit
+constexpr int64_t kMost = ((int64_t)1 << 31) - 256;   // positions, and the end of a tile behind the last, are 32-bit
 constexpr int kRowShift = 7, kKeys = 64, kMaxSplits = 8;
 
 // 64 x 16 bytes, lane's own source, to LDS bytes dst .. dst + 1023 (dst the same in the wave).  Written out, and not as the builtin:
@@ -572,11 +572,11 @@ constexpr int kRowShift = 7, kKeys = 64, kMaxSplits = 8;
 // of a step belong to the NEXT step's tiles, and copies_landed() at that step's barrier is the wait they need.
 __device__ __forceinline__ void copy_to_lds(const void *base, uint32_t offset, uint32_t dst)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(dst) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(dst) : "memory", "m0");
 }
 __device__ __forceinline__ void copy_to_lds(const void *src, uint32_t dst)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
 }
 
 __device__ __forceinline__ void copies_landed()
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     const int64_t out_row = (t.q_beg + qi) * a.hq + head;
     if (t.behind) {
         if (splits > 1) {
-            if (real && h == 0) part_ml[2 * (out_row * splits + split)] = -INFINITY;
+            if (real && h == 0) { part_ml[2 * (out_row * splits + split)] = -INFINITY; part_ml[2 * (out_row * splits + split) + 1] = 0.f; }
             return;
         }
         for (int r = wave; r <= last; r += 4)
@@ -913,7 +913,10 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int split
     float sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
     for (int s = 0; s < kMaxSplits; ++s) {
-        if (ms[s] == -INFINITY) continue;                      // a part that saw nothing has no numerators
+        if (ms[s] == -INFINITY) {                              // a part that saw nothing has no numerators; its sum is 0, or NaN
+            if (s < splits) sum = fmaf(0.f, ls[s], sum);       // where every score was
+            continue;
+        }
         const float f = __builtin_amdgcn_exp2f(ms[s] - top);
         sum = fmaf(f, ls[s], sum);
         x = fmaf(f, ov[s].x, x);

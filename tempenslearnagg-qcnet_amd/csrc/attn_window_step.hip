@@ -13,6 +13,7 @@ namespace {
 using namespace qcn_seq;
 
 constexpr int kAppendShift = 4;   // tokens of a block: 16
+constexpr int64_t kMaxLength = (int64_t)1 << 62;   // a length above it is no length: positions behind it stay in 64 bits
 
 struct AppendArgs {
     const void *k, *v;
@@ -36,7 +37,7 @@ __global__ __launch_bounds__(256) void window_cache_append_kernel(AppendArgs a)
     const int64_t b = f.b, beg = f.beg, end = f.end;
     const int64_t first = ((int64_t)blockIdx.x - ((beg >> kAppendShift) + b)) << kAppendShift;
     const int64_t old = a.lengths[b];
-    if (first < 0 || first >= end - beg || old < 0) return;
+    if (first < 0 || first >= end - beg || old < 0 || old > kMaxLength) return;
     const int64_t total = old + (end - beg);
     const int64_t ntok = end - beg - first < (1 << kAppendShift) ? end - beg - first : (1 << kAppendShift);
     // nothing of the tile stays (the sinks are the first positions, the window the last)
@@ -296,6 +297,7 @@ __global__ __launch_bounds__(256, WAVES == 1 && DP <= 16 ? 6 : 1) void attn_wind
     t.heads = a.group - 16 * ht < 16 ? a.group - 16 * ht : 16;
     t.head0 = t.kvh * a.group + 16 * ht;
     t.p = a.lengths[t.b];
+    if (t.p > kMaxLength) t.p = -1;
     t.n = t.p < 0 ? 0 : (t.p < a.slots ? t.p + 1 : a.slots);
     t.slot = t.p < 0 ? -1 : cache_slot(t.p, a.sinks, a.window);
     // equal parts of what is filled, in whole block strides

@@ -170,7 +170,7 @@ extern "C" int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream)
         if (dim % n || (!interleaved && a.pairs % n)) return false;
         for (int i = 0; i < 2; ++i) {
             if (!a.heads[i]) continue;
-            if (a.rows[i].tok % n || a.rows[i].head % n) return false;
+            if (a.rows[i].tok < 0 || a.rows[i].head < 0 || a.rows[i].tok % n || a.rows[i].head % n) return false;
             if (((uintptr_t)a.in[i] | (uintptr_t)a.out[i]) & (uintptr_t)(n * es - 1)) return false;
         }
         return true;

@@ -28,11 +28,11 @@ struct Rows {
 constexpr int64_t kMaxHeads = 32767;            // of one tensor
 constexpr int64_t kMaxTokStride = (int64_t)1 << 24;   // elements: 64 rows' offsets are 32-bit
 
-// rows are loaded in 16-byte pieces
+// rows are loaded in 16-byte pieces, and strides do not point backwards
 static inline bool rows_aligned(const void *p, int64_t tok, int64_t head, int64_t dtype)
 {
     const int64_t piece = 16 / (int64_t)dtype_bytes(dtype);
-    return ((uintptr_t)p & 15) == 0 && tok % piece == 0 && head % piece == 0;
+    return ((uintptr_t)p & 15) == 0 && tok >= 0 && head >= 0 && tok % piece == 0 && head % piece == 0;
 }
 
 __device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) { return x < lo ? lo : (x > hi ? hi : x); }

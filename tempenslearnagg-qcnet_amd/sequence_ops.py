@@ -304,8 +304,8 @@ def _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batc
     kp, vp = k_cache.data_ptr(), v_cache.data_ptr()
     if (kp | vp) % 16:
         raise ValueError('the caches must start on 16-byte boundaries')
-    if batch and kp == vp:
-        raise ValueError('k_cache and v_cache are the same memory')
+    if abs(kp - vp) < k_cache.numel() * k_cache.element_size():
+        raise ValueError('k_cache and v_cache share memory')
     if not _is(lengths, torch.int64, index, (batch,)):
         _require(lengths, 'lengths', torch.int64, k.device, (batch,))
     if mask_cache is not None:

@@ -240,6 +240,47 @@ def test_window_split_over_blocks_with_rows_behind_and_unseen_infinities(dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lens,extra,hq,hk,dim,win', [([40, 23], None, 4, 2, 16, 50), ([150, 70], None, 4, 2, 64, 120),
+                                                      ([20, 6], [2500, 1100], 2, 1, 64, 2200)])
+def test_window_nan_reaches_the_rows_that_see_it(lens, extra, hq, hk, dim, win, dtype):
+    """A NaN in a query makes that row NaN and no other; a stretch of NaN keys, longer than what one block of a split works on, every
+    row that sees it."""
+    q, k, v, cu_q, cu_k, _ = _case(lens, extra, hq, hk, dim, dtype, False, seed=13)
+    cuk = None if extra is None else cu_k.to(DEV)
+    want = ref.window(q, k, v, cu_q, win, 1, cu_k)
+    tol = ref.tolerance(dtype, dim, *want, float(v.double().abs().max()))
+    qq = q.clone()
+    qq[3, 1, 5] = float('nan')
+    got = ops.attn_window(*_dev(qq, k, v, cu_q), win, 1, cu_k=cuk).cpu().double()
+    assert bool(got[3, 1].isnan().all())
+    got[3, 1] = want[0][3, 1]
+    assert bool(((got - want[0]).abs() <= tol).all())
+    kk = k.clone()
+    kk[: lens[0] - 5 if extra is None else 1300] = float('nan')    # the sink and more, of the first sequence: all its rows see some
+    got = ops.attn_window(*_dev(q, kk, v, cu_q), win, 1, cu_k=cuk).cpu().double()
+    n0 = lens[0]
+    assert bool(got[:n0].isnan().all())
+    assert bool(((got - want[0]).abs() <= tol)[n0:].all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim', [16, 64])
+def test_window_rows_more_than_4_gib_apart(dim, dtype):
+    """Token strides just below the limit: offsets of 80 tokens pass 32 bits, in bytes for float32 and in signed elements for all."""
+    n, h, tok = 80, 2, (1 << 24) - 16
+    q, k, v, cu, _, mask = _case([50, 30], None, h, h, dim, dtype, True, seed=14)
+    room = torch.empty(n * tok, dtype=dtype, device=DEV)
+    views = [room.as_strided((n, h, dim), (tok, 4096, 1), 65536 * i) for i in range(3)]      # interleaved in one stretch of memory
+    for view, x in zip(views, (q, k, v)):
+        view.copy_(x)
+    got = ops.attn_window(*views, cu.to(DEV), 20, 2, key_mask=mask.to(DEV))
+    _check(got, ref.window(q, k, v, cu, 20, 2, key_mask=mask), dtype, dim, v)
+    tq, tk = ops.rotary_embed(views[0], views[1], torch.arange(n, device=DEV).view(n, 1), torch.ones(dim // 2, device=DEV), [dim // 2])
+    sq, sk = ops.rotary_embed(q.to(DEV), k.to(DEV), torch.arange(n, device=DEV).view(n, 1), torch.ones(dim // 2, device=DEV), [dim // 2])
+    assert torch.equal(tq, sq) and torch.equal(tk, sk)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_window_all_masked_and_large_scores(dtype):
     q, k, v, cu, _, _ = _case([45, 30], None, 4, 2, 32, dtype, False, seed=6)
     none = torch.zeros(75, dtype=torch.bool)
@@ -358,6 +399,63 @@ def test_step_ignores_what_masked_slots_hold(dtype):
     assert bool((got == 0).all())
 
 
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
+def test_cache_rows_beyond_4_gib(dtype):
+    """The second row of a cache whose rows are more than 4 GiB each: prompt and step land there and read there, and a length that
+    has gone round the ring comes back to its start."""
+    hk, dim, sinks = 1, 128, 2
+    slots = (1 << 32) // (dim * torch.finfo(dtype).bits // 8) + 70
+    kc, vc = (torch.empty(2, hk, slots, dim, dtype=dtype, device=DEV) for _ in range(2))
+    g = _gen(15)
+    n = 40
+    k, v = _rand(g, n, hk, dim, dtype=dtype), _rand(g, n, hk, dim, dtype=dtype)
+    q, k1, v1 = _rand(g, 2, 2, dim, dtype=dtype), _rand(g, 2, hk, dim, dtype=dtype), _rand(g, 2, hk, dim, dtype=dtype)
+    lengths = torch.tensor([-1, 0])
+    ops.window_cache_append(*_dev(k, v), torch.tensor([0, 0, n], device=DEV), lengths.to(DEV), kc, vc, sinks)
+    assert torch.equal(kc[1, 0, :n].cpu(), k[:, 0]) and torch.equal(vc[1, 0, :n].cpu(), v[:, 0])
+    lengths[1] = n
+    got = ops.attn_window_step(*_dev(q, k1, v1, lengths), kc, vc, sinks)
+    assert torch.equal(kc[1, 0, n].cpu(), k1[1, 0]) and torch.equal(vc[1, 0, n].cpu(), v1[1, 0])
+    allk, allv = torch.cat([k, k1[1:]]), torch.cat([v, v1[1:]])
+    want = ref.window(torch.cat([torch.zeros(n, 2, dim, dtype=dtype), q[1:]]), allk, allv, torch.tensor([0, n + 1]), slots, sinks)
+    assert bool((got[0] == 0).all())
+    _check(got[1:], [x[n:] for x in want], dtype, dim, allv)
+    ops.window_cache_append(*_dev(k, v), torch.tensor([0, 0, n], device=DEV), torch.tensor([-1, slots - 7], device=DEV), kc, vc, sinks)
+    assert torch.equal(kc[1, 0, slots - 7:].cpu(), k[:7, 0]) and torch.equal(vc[1, 0, sinks:sinks + n - 7].cpu(), v[7:, 0])
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('win', [20, 700])
+def test_step_nan_query(win, dtype):
+    q, k, v, lengths, kc, vc, _, _ = _step_case([900, 90], 4, 2, 64, win, 3, False, dtype, seed=16)
+    want = ref.step(q, k, v, lengths, kc.clone(), vc.clone(), 3)
+    qq = q.clone()
+    qq[0, 2, 9] = float('nan')
+    got = ops.attn_window_step(*_dev(qq, k, v, lengths, kc, vc), 3).cpu().double()
+    assert bool(got[0, 2].isnan().all())
+    got[0, 2] = want[0][0, 2]
+    assert bool(((got - want[0]).abs() <= ref.tolerance(dtype, 64, *want, float(vc.double().abs().max()))).all())
+
+
+def test_lengths_out_of_range_are_rows_not_in_use():
+    q, k, v, _, kc, vc, _, _ = _step_case([5, 5], 4, 2, 64, 20, 3, False, torch.bfloat16, seed=17)
+    lengths = torch.tensor([(1 << 63) - 1, (1 << 62) + 1], device=DEV)
+    dq, dk, dv, dkc, dvc = _dev(q, k, v, kc, vc)
+    assert bool((ops.attn_window_step(dq, dk, dv, lengths, dkc, dvc, 3) == 0).all())
+    ops.window_cache_append(dk, dv, torch.tensor([0, 1, 2], device=DEV), lengths, dkc, dvc, 3)
+    assert torch.equal(dkc.cpu(), kc) and torch.equal(dvc.cpu(), vc)
+
+
+def test_caches_that_share_memory_are_refused():
+    room = torch.zeros(3, 1, 8, 16, device=DEV)
+    x, n = torch.zeros(2, 1, 16, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+    for a, b in ((room[:2], room[:2]), (room[:2], room[1:])):
+        with pytest.raises(ValueError, match='share memory'):
+            ops.attn_window_step(x, x, x, n, a, b, 1)
+        with pytest.raises(ValueError, match='share memory'):
+            ops.window_cache_append(x, x, torch.tensor([0, 1, 2], device=DEV), n, a, b, 1)
+
+
 # ------------------------------------------------------------------------------------------------
 # together
 # ------------------------------------------------------------------------------------------------
@@ -438,6 +536,53 @@ def test_steps_in_a_graph_on_another_stream():
         assert torch.equal(out, eager[i]), i
         ops.attn_window_step(tokens[0, :, :hq], tokens[0, :, hq:hq + hk], tokens[0, :, hq + hk:], start, kc0.clone(), vc0.clone(), sinks)
     assert torch.equal(gk, kc) and torch.equal(gv, vc) and torch.equal(gl, lengths)
+
+
+@pytest.mark.parametrize('lens,extra,win', [([300, 45], None, 60), ([20, 6], [2500, 1100], 2200)])
+def test_prefill_in_a_graph(lens, extra, win):
+    """Rotation, attention (in one pass and split over blocks) and append, captured once and replayed on other data, with eager calls in
+    between, equal the eager calls."""
+    hq, hk, dim, sinks, dtype = 4, 2, 64, 2, torch.bfloat16
+    cases = [_case(lens, extra, hq, hk, dim, dtype, True, seed=20 + i) for i in range(3)]
+    cu_q, cu_k = _dev(cases[0][3], cases[0][4] if extra is not None else cases[0][3])
+    nq, nk = cases[0][0].size(0), cases[0][1].size(0)
+    freqs, pos = torch.rand(dim // 2, generator=_gen(21)).to(DEV), torch.arange(nq, device=DEV).view(nq, 1)
+    lengths = torch.tensor([3, 0], device=DEV)
+
+    def one(q, k, v, mask, kc, vc, mc):
+        q = ops.rotary_embed(q, None, pos, freqs, [dim // 2])[0]
+        out = ops.attn_window(q, k, v, cu_q, win, sinks, cu_k=cu_k, key_mask=mask)
+        ops.window_cache_append(k, v, cu_k, lengths, kc, vc, sinks, key_mask=mask, mask_cache=mc)
+        return out
+
+    def cache():
+        return (torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV), torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV),
+                torch.zeros(2, win + sinks, dtype=torch.bool, device=DEV))
+
+    data = [_dev(c[0], c[1], c[2], c[5]) for c in cases]
+    wants = []
+    for d in data:
+        c = cache()
+        wants.append((one(*d, *c).clone(), c))
+    held, kept = [x.clone() for x in data[0]], cache()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one(*held, *kept)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = one(*held, *kept)
+    for _ in range(2):
+        for d, (want, c) in zip(data, wants):
+            for a, b in zip(held, d):
+                a.copy_(b)
+            for x in kept:
+                x.zero_()
+            graph.replay()
+            one(*data[0], *cache())
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(kept, c))
 
 
 def test_window_on_two_streams_is_the_same_every_time():

@@ -95,6 +95,25 @@ def test_rotary_entry_point_refusals():
     assert lib.qcn_rotary_embed(None, None) == INVALID
 
 
+def test_strides_that_point_backwards_and_sizes_past_32_bits_are_refused():
+    lib = _lib.lib()
+    window = dict(q=FAKE, qs=(32, 16), k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu_q=FAKE, cu_k=FAKE, mask=0, n_seq=1, nq=4, nk=4, hq=2,
+                  hk=2, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE, ws=0, ws_bytes=0)
+    for bad in (dict(qs=(-32, 16)), dict(ks=(32, -16)), dict(vs=(-32, -16))):
+        assert _call(lib, 'qcn_attn_window', '21qd3q', window, **bad) == INVALID, bad
+    for bad in (dict(nq=(1 << 31) - 1), dict(nk=(1 << 31) - 200)):
+        assert _call(lib, 'qcn_attn_window', '21qd3q', window, **bad) == UNSUPPORTED, bad
+    step = dict(q=FAKE, qs=(512, 64), k=FAKE, ks=(512, 64), v=FAKE, vs=(512, 64), lengths=FAKE, key_mask=0, batch=2, hq=4, hk=2, dim=64,
+                dtype=2, window=4, sinks=1, scale=1.0, kc=FAKE, vc=FAKE, mc=0, out=FAKE, ws=0, ws_bytes=0)
+    append = dict(k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu=FAKE, lengths=FAKE, key_mask=0, n_seq=1, n=4, hk=2, dim=16, dtype=0, window=3,
+                  sinks=0, kc=FAKE, vc=FAKE, mc=0)
+    rotary = dict(q=FAKE, qs=(-32, 16), hq=2, k=0, ks=(0, 0), hk=0, n=4, dim=16, dtype=0, pos=FAKE, pos_type=0, axes=1,
+                  sections=(8,) + (0,) * 7, freqs=FAKE, interleaved=0, inverse=0, q_out=FAKE, k_out=0)
+    assert _call(lib, 'qcn_attn_window_step', '18qd6q', step, ks=(-512, 64)) == INVALID
+    assert _call(lib, 'qcn_window_cache_append', '19q', append, vs=(32, -16)) == INVALID
+    assert _call(lib, 'qcn_rotary_embed', '27q', rotary) == INVALID
+
+
 def test_the_cache_holds_what_a_position_sees():
     """step() over the cache equals window() over the whole sequence, for every position (float64, no kernel)."""
     g = torch.Generator().manual_seed(0)
