@@ -569,14 +569,15 @@ constexpr int kRowShift = 7, kKeys = 64, kMaxSplits = 8;
 
 // 64 x 16 bytes, lane's own source, to LDS bytes dst .. dst + 1023 (dst the same in the wave).  Written out, and not as the builtin:
 // the compiler takes every transposing read for a possible reader of every copy in flight and waits for all of them; the copies
-// of a step belong to the NEXT step's tiles, and copies_landed() at that step's barrier is the wait they need.
+// of a step belong to the NEXT step's tiles, and copies_landed() at that step's barrier is the wait they need.  (m0 is a reserved
+// register: the compiler sets it in front of each instruction of its own that reads it and keeps nothing there.)
 __device__ __forceinline__ void copy_to_lds(const void *base, uint32_t offset, uint32_t dst)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(dst) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(dst) : "memory");
 }
 __device__ __forceinline__ void copy_to_lds(const void *src, uint32_t dst)
 {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst) : "memory");
 }
 
 __device__ __forceinline__ void copies_landed()
