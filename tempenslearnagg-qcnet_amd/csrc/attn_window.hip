@@ -155,10 +155,13 @@ template <class T, int DP> struct Direct {
 template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 
 // OFF: byte offset inside one of the tensors; 32 bits where every tensor is below 4 GiB (a load then takes a scalar base).
-// Rows of 16 float32 ask for four waves per SIMD (128 registers; the compiler's own 139 leave three): 1600 x 59 agent steps 54.3
-// -> 51 us, 8 x 2000 steps with a window of 500 86 -> 77 us.  16-bit rows are faster with three and no spills (34.0 against 35.8 us).
+// Waves per SIMD asked for, against the compiler's own choice (8 x 2000 float32 steps x 8 heads, window 500; us): 16 features four
+// (76.5, own 85), 32 four (119.7, own 123.5), 64 four (183, own 196), 96 its own (390; three: 445), 128 two (371, own 388).  1600 x
+// 59 agent steps of 16 float32: 54.3 -> 51 us.  16-bit rows are faster with the compiler's three and no spills (34.0, four: 35.8).
+template <class T, int DP> constexpr int direct_waves() { return sizeof(T) == 2 || DP == 96 ? 1 : DP <= 64 ? 4 : 2; }
+
 template <class T, int DP, class OFF>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP <= 16 ? 4 : 1) void attn_window_direct_kernel(Args a, int64_t n_tiles, int heads_per_wave, int head_groups)
+__global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_direct_kernel(Args a, int64_t n_tiles, int heads_per_wave, int head_groups)
 {
     using L = Direct<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
