@@ -4,6 +4,13 @@
 // It sees key j when  0 <= j <= p  and  (j > p - window  or  j < sinks)  and key_mask[j]:
 //   o = sum_j softmax_j(scale q . k_j) v_j,   o = 0 for a row that sees nothing.
 // Hkv key heads are shared by Hq / Hkv query heads each.
+//
+// The work is 4 dim operations per visible (query, key) pair and head; q, k, v and o pass memory once.  Short windows (an agent's
+// 10 steps of 16 features) are bound by memory and its latency, long ones by the matrix units, so there are two kernels:
+//   direct  16 rows per wave, operands straight from memory, no barrier: float32, and 16-bit rows of up to 16 features (up to 32
+//           where the window is short)
+//   tile    128 rows per block, 64-key tiles through LDS: wider 16-bit rows
+// Both keep one running maximum and sum per row, in float32, and go over the keys once.
 #include "sequence.hip.h"
 
 #include <type_traits>
@@ -130,7 +137,7 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// 16 rows per wave, keys straight from memory (float32 of every width; 16-bit types up to 16 features)
+// 16 rows per wave, keys straight from memory (float32 of every width; narrow rows of the 16-bit types)
 // ---------------------------------------------------------------------------------------------------------------------
 // A wave is on its own: no barrier.  For short windows (the agents' 10 steps) every key tile is used by two or three row
 // tiles at most, so staging would cost more than the cache hits it saves.  A wave keeps its 16 rows and goes through key heads:
@@ -142,6 +149,12 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // sb SB + VW m + e (m = 0 .. 15): a lane ends with 4 VW neighbouring features of its query.  Wide heads load VW neighbouring
 // features of a key for it; of narrow ones that would be loads of 4 or 8 bytes, four times as many instructions as the bytes
 // need, so their V comes like K and is turned in a few hundred bytes of LDS of the wave's own.
+//
+// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 50 us, 3.9 TB/s, bound by
+// the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
+// 80 Tflop/s of the 154 that a library product reaches (8 x 2000 steps, 8 heads of 64 or 128, window 500: 183 and 371 us); the L1
+// cache is what bounds them (73 % of its cycles serve a request, against 57 % of the matrix units'): a load of 16 keys serves 16 rows.
+// Whole steps with scalar addresses and no masks did not help (183 -> 202 us at 64 features), 32 rows per wave are left.
 template <class T, int DP> struct Direct {
     static constexpr int VW = DP % 64 == 0 ? 4 : (DP % 32 == 0 ? 2 : 1);
     static constexpr int SB = 16 * VW, NSB = DP / SB, NT = DP / 16;
@@ -559,13 +572,22 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // in flight while the matrix units work on this one, one barrier per tile.  v_mfma_f32_32x32x16: A = 32 keys (S^T) or 32 features
 // (O^T), B = 32 rows.  With the accumulator's row order, k-step t of key half-tile u contracts keys
 // 32 u + 16 t + {4 h .. 4 h + 3, 8 + 4 h ..}  in lane half h: V^T is fetched in that order by two transposing LDS reads, P^T is the
-// S^T registers rounded to 16 bits.
+// S^T registers rounded to 16 bits: a relative error of at most half a step of the type per weight (bfloat16 2^-9), below the
+// rounding of the output and averaged over the keys; the sum takes the rounded weights, so that they still add up to one.  A second
+// product with the remainders would cost half as much again of what bounds the kernel.
 //
 // LDS rows are swizzled in 16-byte pieces so that 16 neighbouring keys' pieces (K) and the 4 x 64 bytes of a transposing read
 // (V) cover all 64 banks; the copies write LDS in order and permute their source addresses.
 //
 // With few blocks (a short chunk of queries behind a long prefix) the key tiles are split over blocks as well and joined by a
 // second kernel.
+//
+// Bound by the matrix units and the vector instructions around them, which two or three waves per SIMD do not fully overlap
+// (timed with parts left out, 16384 x 16 heads of 128, window 1024: all 177 us, no products 109, no LDS reads 151, no exponentials
+// 167, no copies 175).  Measured: that case 165 us, 810 Tflop/s of the 1130 that a large library product reaches; 24 ragged
+// prompts up to 2500 x 12 heads of 64, window 512, float16: 90 us, 440 Tflop/s counting visible pairs only (32 rows see 9 or 10
+// tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32
+// heads of 128 behind 7000 keys each, window 4096: 100 us + 16 for the join, 620 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
@@ -902,7 +924,7 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     }
 }
 
-// Joins the parts of a row: a wave per (token, query head).
+// Joins the parts of a row: a wave per (token, query head).  Bound by memory: 34 144 rows of 128 in four parts, 79 MB in 16 us.
 template <class T>
 __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int splits, const float *__restrict__ part_o,
                                                                const float *__restrict__ part_ml)
@@ -984,7 +1006,8 @@ int launch_direct(const Args &a, hipStream_t s)
 }
 
 // Blocks of the 128-row kernel for one part of the keys, and the parts: 2 blocks fit a CU, and a launch wants several rounds of
-// them.  A part keeps at least 8 key tiles.  Sizes only: lengths are on the device.
+// them (1067 queries x 8 key heads, window 4096: 304 blocks undivided, 1216 in four parts).  A part keeps at least 8 key tiles:
+// below that its setup and its share of the join cost more than the emptier card.  Sizes only: lengths are on the device.
 int plan_splits(const Args &a)
 {
     if (a.dim <= 16) return 1;
@@ -1026,6 +1049,9 @@ int launch(const Args &a, void *ws, int64_t ws_bytes, hipStream_t s)
         return launch_direct<T, 128>(a, s);
     } else {
         if (a.dim <= 16) return launch_direct<T, 16>(a, s);
+        // 16 rows and all their keys in one step of the direct form: 800 x 59 steps x 8 heads of 32, window 10 + 1, 29 us against the
+        // tile kernel's 50; window 30: 53 against 48.  Of 64 features and more the tile kernel is faster there too (37 against 42 us).
+        if (a.dim <= 32 && a.window + a.sinks <= 17) return launch_direct<T, 32>(a, s);
         if (a.dim <= 32) return launch_tile<T, 32>(a, ws, ws_bytes, s);
         if (a.dim <= 64) return launch_tile<T, 64>(a, ws, ws_bytes, s);
         if (a.dim <= 96) return launch_tile<T, 96>(a, ws, ws_bytes, s);

@@ -437,6 +437,40 @@ def test_step_nan_query(win, dtype):
     assert bool(((got - want[0]).abs() <= ref.tolerance(dtype, 64, *want, float(vc.double().abs().max()))).all())
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('dim,hq,hk,win,sinks', [(8, 5, 5, 10, 1), (24, 6, 2, 16, 1), (32, 8, 8, 10, 1), (32, 3, 3, 17, 0), (32, 12, 4, 1, 16),
+                                                 (32, 7, 1, 18, 0), (24, 4, 4, 1, 0)])
+def test_window_narrow_heads_and_short_windows(dim, hq, hk, win, sinks, dtype):
+    """Windows on both sides of what one step of 32 keys holds, heads that do not fill a 128-byte line, masked keys that hold NaN."""
+    q, k, v, cu, _, mask = _case([59, 1, 0, 16, 130, 17], None, hq, hk, dim, dtype, True, seed=30)
+    kk, vv = k.clone(), v.clone()
+    kk[~mask], vv[~mask] = float('nan'), float('inf')
+    got = ops.attn_window(*_dev(q, kk, vv, cu), win, sinks, key_mask=mask.to(DEV))
+    _check(got, ref.window(q, k, v, cu, win, sinks, None, mask), dtype, dim, v)
+    _check(ops.attn_window(*_dev(q, k, v, cu), win, sinks), ref.window(q, k, v, cu, win, sinks), dtype, dim, v)
+    vv = v.clone()
+    vv[70] = float('inf')                                      # seen by some rows of a tile only
+    got = ops.attn_window(*_dev(q, k, vv, cu), win, sinks).cpu().double()
+    r = ref.window(q, k, v, cu, win, sinks)
+    tol = ref.tolerance(dtype, dim, *r, float(v.double().abs().max()))
+    at = torch.arange(223)
+    sees = (at >= 70) & (at < 76) & (at < 70 + win) if 70 - 60 >= sinks else (at >= 70) & (at < 76)
+    assert not bool(torch.isfinite(got[sees]).any())
+    assert bool(((got - r[0]).abs() <= tol)[~sees].all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('slots', [240, 256, 257])
+@pytest.mark.parametrize('batch,hq,hk,dim', [(3, 8, 2, 64), (70, 8, 8, 16)])
+def test_step_around_the_size_that_one_wave_takes(batch, hq, hk, dim, slots, dtype):
+    ages = [(37 * i) % (2 * slots) for i in range(batch)]
+    q, k, v, lengths, kc, vc, km, mc = _step_case(ages, hq, hk, dim, slots - 2, 2, True, dtype, seed=31)
+    dkc, dvc, dmc = _dev(kc, vc, mc)
+    got = ops.attn_window_step(*_dev(q, k, v, lengths), dkc, dvc, 2, key_mask=km.to(DEV), mask_cache=dmc)
+    _check(got, ref.step(q, k, v, lengths, kc, vc, 2, km, mc), dtype, dim, vc)
+    assert torch.equal(dkc.cpu(), kc) and torch.equal(dvc.cpu(), vc) and torch.equal(dmc.cpu(), mc)
+
+
 def test_lengths_out_of_range_are_rows_not_in_use():
     q, k, v, _, kc, vc, _, _ = _step_case([5, 5], 4, 2, 64, 20, 3, False, torch.bfloat16, seed=17)
     lengths = torch.tensor([(1 << 63) - 1, (1 << 62) + 1], device=DEV)
