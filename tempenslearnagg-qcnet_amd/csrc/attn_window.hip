@@ -150,7 +150,7 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // features of a key for it; of narrow ones that would be loads of 4 or 8 bytes, four times as many instructions as the bytes
 // need, so their V comes like K and is turned in a few hundred bytes of LDS of the wave's own.
 //
-// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 50 us, 3.9 TB/s, bound by
+// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48 us, 4.0 TB/s, bound by
 // the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
 // 80 Tflop/s of the 154 that a library product reaches (8 x 2000 steps, 8 heads of 64 or 128, window 500: 183 and 371 us); the L1
 // cache is what bounds them (73 % of its cycles serve a request, against 57 % of the matrix units'): a load of 16 keys serves 16 rows.

