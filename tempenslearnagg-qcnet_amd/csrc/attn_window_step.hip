@@ -89,8 +89,8 @@ struct StepArgs {
 //
 // Weights meet 16-bit V rounded to its type (relative error at most half a step; the output is rounded to the same type); a second
 // product with what the rounding left makes a step of 64 x 8 key heads x 4100 slots 1.9 % slower (183 against 179.6 us, both in two parts).
-// Measured: that step (64 requests x 32 heads of 128 in bfloat16) 168 us, 984 MB at 5.9 TB/s; one request 9.2 +
-// 4.6 us (two launches, three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21 us, 4 TB/s.
+// Measured: that step (64 requests x 32 heads of 128 in bfloat16) 168 us, 984 MB at 5.9 TB/s; one request 9.8 + 4.1
+// us (two launches, three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21 us, 4 TB/s.
 template <class T, int DP> struct Step {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NU = DP <= 32 ? 4 : 2, CHUNK = 16 * NU;                        // slots of a chunk: narrow heads take 64
@@ -377,7 +377,7 @@ __global__ __launch_bounds__(256, WAVES == 1 && DP <= 16 ? 6 : 1) void attn_wind
 }
 
 // Joins the parts of a row: a block per (cache row, query head), its waves take the parts in turn.  All loads of a wave are
-// requested before the first is used: the kernel's time is a few memory latencies, not one per part (32 rows in 33 parts: 4.6 us).
+// requested before the first is used: the kernel's time is a few memory latencies, not one per part (32 rows in 33 parts: 4.1 us).
 constexpr int kMaxSplits = 64;
 
 template <class T>
