@@ -41,7 +41,7 @@ _STEP_ARGS = struct.Struct('=18qd6q').pack
 def _plain(*tensors) -> bool:
     """Whether the call can go to the implementation directly: plain tensors, nothing tracing, nothing to differentiate.  The
     dispatcher costs 5 us a call, as much as everything else the host does for a decoding step."""
-    if torch._C._len_torch_dispatch_stack() or torch.compiler.is_compiling():
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
         return False
     grad = torch.is_grad_enabled()
     for t in tensors:
@@ -75,6 +75,10 @@ def _in_place(t: torch.Tensor):
         return t, strides
     t = t.clone(memory_format=torch.contiguous_format)
     return t, t.stride()
+
+
+# a contiguous tensor of the same shape and type (two thirds of new_empty's time, and a call for few tokens is the host's time)
+_out_like = functools.partial(torch.empty_like, memory_format=torch.contiguous_format)
 
 
 def _dtype_code(t: torch.Tensor, name: str) -> int:
@@ -177,7 +181,7 @@ def _rotary_embed(q, k, pos, freqs, sections, interleaved, inverse):
     if not _is(freqs, torch.float32, index, (pairs,)):
         _require(freqs, 'freqs', torch.float32, q.device, (pairs,))
     q, qs = _even_rows(q)
-    q_out = q.new_empty(shape)
+    q_out = _out_like(q)
     hk = kp = ks0 = ks1 = k_out_ptr = 0
     outs = [q_out]
     if k is not None:
@@ -190,7 +194,7 @@ def _rotary_embed(q, k, pos, freqs, sections, interleaved, inverse):
             raise ValueError('k has no heads: pass None')
         k, (ks0, ks1, _) = _even_rows(k)
         kp = k.data_ptr()
-        k_out = q.new_empty((n, hk, dim))
+        k_out = _out_like(k)
         k_out_ptr = k_out.data_ptr()
         outs.append(k_out)
     if n and (hq or hk):
@@ -271,7 +275,7 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
     q, qs = _in_place(q)
     k, ks = _in_place(k)
     v, vs = _in_place(v)
-    out = q.new_empty((nq, hq, dim))
+    out = _out_like(q)
     if nq:
         args = (q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
                 n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr())
@@ -390,7 +394,7 @@ def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_
     q, qs = _in_place(q)
     k, ks = _in_place(k)
     v, vs = _in_place(v)
-    out = q.new_empty((batch, hq, dim))
+    out = _out_like(q)
     if batch:
         ws_bytes = _step_workspace(index, batch, hq, hk, dim, window, sinks)
         ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None

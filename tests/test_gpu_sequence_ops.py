@@ -703,6 +703,31 @@ def test_refusals():
         ops.rotary_embed(q, None, pos, f(0), [0, 0])
 
 
+def test_a_traced_step_is_one_graph():
+    """torch.compile (no code generation: backend aot_eager) takes rotation, prefill, append and step in one graph, with the caches
+    written in place, and gives what the eager calls give."""
+    hq, hk, dim, win, sinks, dtype = 4, 2, 64, 24, 2, torch.bfloat16
+    q, k, v, cu, _, mask = _case([30, 17], None, hq, hk, dim, dtype, True, seed=40)
+    dq, dk, dv, dcu, dm = _dev(q, k, v, cu, mask)
+    pos, freqs = torch.arange(47, device=DEV).view(47, 1), torch.rand(dim // 2, generator=_gen(41)).to(DEV)
+    lengths = torch.tensor([30, 17], device=DEV)
+
+    def run(q, k, v, kc, vc, mc):
+        q, k = ops.rotary_embed(q, k, pos, freqs, [dim // 2])
+        out = ops.attn_window(q, k, v, dcu, win, sinks, key_mask=dm)
+        ops.window_cache_append(k, v, dcu, torch.zeros_like(lengths), kc, vc, sinks, key_mask=dm, mask_cache=mc)
+        return out, ops.attn_window_step(q[:2], k[:2], v[:2], lengths, kc, vc, sinks, key_mask=dm[:2], mask_cache=mc)
+
+    def cache():
+        return (torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV), torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV),
+                torch.zeros(2, win + sinks, dtype=torch.bool, device=DEV))
+
+    a, b = cache(), cache()
+    want = run(dq, dk, dv, *a)
+    got = torch.compile(run, backend='aot_eager', fullgraph=True)(dq, dk, dv, *b)
+    assert all(torch.equal(x, y) for x, y in zip(got + b, want + a))
+
+
 def test_sequence_ops_trace_under_fake_tensors():
     from torch._subclasses.fake_tensor import FakeTensorMode
     with FakeTensorMode():
