@@ -587,7 +587,7 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // 167, no copies 175).  Measured: that case 165 us, 810 Tflop/s of the 1130 that a large library product reaches; 24 ragged
 // prompts up to 2500 x 12 heads of 64, window 512, float16: 90 us, 440 Tflop/s counting visible pairs only (32 rows see 9 or 10
 // tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32
-// heads of 128 behind 7000 keys each, window 4096: 100 us + 16 for the join, 620 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
+// heads of 128 behind 7000 keys each, window 4096, in three parts: 115 us with the join, 620 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
@@ -924,7 +924,8 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     }
 }
 
-// Joins the parts of a row: a wave per (token, query head).  Bound by memory: 34 144 rows of 128 in four parts, 79 MB in 16 us.
+// Joins the parts of a row: a wave per (token, query head).  Bound by memory: 34 144 rows of 128 in four parts, 79 MB in
+// 16 us.
 template <class T>
 __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int splits, const float *__restrict__ part_o,
                                                                const float *__restrict__ part_ml)
@@ -1005,13 +1006,14 @@ int launch_direct(const Args &a, hipStream_t s)
     return QCN_OK;
 }
 
-// Blocks of the 128-row kernel for one part of the keys, and the parts: 2 blocks fit a CU, and a launch wants several rounds of
-// them (1067 queries x 8 key heads, window 4096: 304 blocks undivided, 1216 in four parts).  A part keeps at least 8 key tiles:
+// Parts of the keys: as many as bring the launch to three blocks of the 128-row kernel per CU (two or three fit at once).  Measured at
+// two, three, four and six per CU, us: 1067 queries x 8 key heads of 128 behind 7000 keys each, window 4096 (304 blocks undivided) 140,
+// 128, 133, 140; 500 x 8 behind 8000: three 65, four 70; 64 x 8 behind 8000: three 23.4, four 22.9.  A part keeps at least 8 key tiles:
 // below that its setup and its share of the join cost more than the emptier card.  Sizes only: lengths are on the device.
 int plan_splits(const Args &a)
 {
     if (a.dim <= 16) return 1;
-    const int64_t blocks = ((a.nq * a.group >> kRowShift) + a.n_seq + 1) * a.hk, want = 4 * (int64_t)qcn_num_cus();
+    const int64_t blocks = ((a.nq * a.group >> kRowShift) + a.n_seq + 1) * a.hk, want = 3 * (int64_t)qcn_num_cus();
     int64_t reach = a.window + a.sinks + 128 / a.group;
     if (reach > a.nk) reach = a.nk;
     int64_t s = (want + blocks - 1) / blocks;
