@@ -587,7 +587,7 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // 167, no copies 175).  Measured: that case 165 us, 810 Tflop/s of the 1130 that a large library product reaches; 24 ragged
 // prompts up to 2500 x 12 heads of 64, window 512, float16: 90 us, 440 Tflop/s counting visible pairs only (32 rows see 9 or 10
 // tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32
-// heads of 128 behind 7000 keys each, window 4096, in three parts: 115 us with the join, 620 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
+// heads of 128 behind 7000 keys each, window 4096, in three parts: 107 us with the join, 670 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
@@ -924,46 +924,67 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
     }
 }
 
-// Joins the parts of a row: a wave per (token, query head).  Bound by memory: 34 144 rows of 128 in four parts, 79 MB in
-// 16 us.
-template <class T>
+// Joins the parts of a row, all requested before the first is used: half a wave per (token, query head) and 16 bytes of a part per
+// lane where there are up to four parts, a wave and 8 bytes where there are up to eight.  Bound by memory and its latency: 34 144 rows
+// of 128 in three parts, 61 MB.  (With a wave each they took 4 us more of 124 for the whole call; 2048 rows in eight parts take 2 us
+// more of 23 with half a wave each.)
+template <int PARTS> constexpr int join_features() { return PARTS <= 4 ? 4 : 2; }
+
+template <class T, int PARTS>
 __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int splits, const float *__restrict__ part_o,
                                                                const float *__restrict__ part_ml)
 {
+    constexpr int VE = join_features<PARTS>(), LANES = kMaxDim / VE, ROWS = 64 / LANES;   // of a lane, of a row, of a wave
+    using Vec = __attribute__((ext_vector_type(VE))) float;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = (int64_t)blockIdx.x * 4 + wave;
-    if (row >= a.nq * a.hq) return;
-    const int d = 2 * lane;
-    float ms[kMaxSplits], ls[kMaxSplits], top = -INFINITY;
-    float2 ov[kMaxSplits];
+    const int64_t rows = a.nq * a.hq, row0 = ((int64_t)blockIdx.x * 4 + wave) * ROWS;
+    if (row0 >= rows) return;
+    const bool real = row0 + lane / LANES < rows;
+    const int64_t row = real ? row0 + lane / LANES : row0;
+    const int d = VE * (lane % LANES);
+    const bool has = d < a.dim;
+    float2 ml[PARTS];
+    Vec ov[PARTS];
+    float top = -INFINITY;
 #pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s) {
+    for (int s = 0; s < PARTS; ++s) {
         const int64_t at = row * splits + (s < splits ? s : 0);
-        ms[s] = s < splits ? part_ml[2 * at] : -INFINITY;
-        ls[s] = part_ml[2 * at + 1];
-        ov[s] = *reinterpret_cast<const float2 *>(part_o + at * a.dim + (d < a.dim ? d : 0));
-        top = fmaxf(top, ms[s]);
+        ml[s] = reinterpret_cast<const float2 *>(part_ml)[at];
+        if (s >= splits) ml[s] = make_float2(-INFINITY, 0.f);
+        ov[s] = *reinterpret_cast<const Vec *>(part_o + at * a.dim + (has ? d : 0));
+        top = fmaxf(top, ml[s].x);
     }
-    float sum = 0.f, x = 0.f, y = 0.f;
+    float sum = 0.f;
+    Vec x = {};
 #pragma unroll
-    for (int s = 0; s < kMaxSplits; ++s) {
-        if (ms[s] == -INFINITY) {                              // a part that saw nothing has no numerators; its sum is 0, or NaN
-            if (s < splits) sum = fmaf(0.f, ls[s], sum);       // where every score was
-            continue;
-        }
-        const float f = __builtin_amdgcn_exp2f(ms[s] - top);
-        sum = fmaf(f, ls[s], sum);
-        x = fmaf(f, ov[s].x, x);
-        y = fmaf(f, ov[s].y, y);
+    for (int s = 0; s < PARTS; ++s) {
+        const bool saw = ml[s].x != -INFINITY;                 // a part that saw nothing has no numerators; its sum is 0, or NaN
+        const float f = saw ? __builtin_amdgcn_exp2f(ml[s].x - top) : 0.f;   // where every score was
+        sum = fmaf(f, ml[s].y, sum);
+#pragma unroll
+        for (int e = 0; e < VE; ++e) x[e] = saw ? fmaf(f, ov[s][e], x[e]) : x[e];
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    x *= inv;
-    y *= inv;
-    const int64_t token = row / a.hq;
-    const int head = (int)(row % a.hq);
-    if (__ballot(d < a.dim && !(fabsf(x) < INFINITY && fabsf(y) < INFINITY))) {   // see the end of the tile kernel
-        int64_t lo = 0, hi = a.n_seq;                                             // last sequence that starts at or before token
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) {
+        x[e] *= inv;
+        bad |= !(fabsf(x[e]) < INFINITY);
+    }
+    const uint64_t again = __ballot(bad && has && real);       // see the end of the tile kernel
+    const auto of_row = [&](int r) { return LANES == 64 ? again : (uint64_t)(unsigned)(again >> (LANES * r)); };
+    if (has && real && !of_row(lane / LANES)) {
+        Pack<T, VE> y;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) y.e[e] = from_f32<T>(x[e]);
+        *reinterpret_cast<Pack<T, VE> *>(reinterpret_cast<T *>(a.out) + row * a.dim + d) = y;
+    }
+    for (int half = 0; half < ROWS; ++half) {
+        if (!of_row(half)) continue;
+        const int64_t token = (row0 + half) / a.hq;
+        const int head = (int)((row0 + half) % a.hq);
+        int64_t lo = 0, hi = a.n_seq;                          // last sequence that starts at or before token
         while (lo + 1 < hi) {
             const int64_t mid = (lo + hi) / 2;
             if (clamp64(a.cu_q[mid], 0, a.nq) <= token) lo = mid;
@@ -974,11 +995,6 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int split
         seq_range(a.cu_k, lo, a.nk, k_beg, k_end);
         if (token >= q_beg && token < q_end)
             row_by_wave<T>(a, k_beg, token - q_beg + (k_end - k_beg) - (q_end - q_beg), token, head, lane);
-        return;
-    }
-    if (d < a.dim) {
-        Pack<T, 2> two = {{from_f32<T>(x), from_f32<T>(y)}};
-        *reinterpret_cast<Pack<T, 2> *>(reinterpret_cast<T *>(a.out) + row * a.dim + d) = two;
     }
 }
 
@@ -1034,7 +1050,12 @@ int launch_tile(const Args &a, void *workspace, int64_t workspace_bytes, hipStre
     hipLaunchKernelGGL((attn_window_tile_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles, splits, part_o, part_ml);
     QCN_CHECK_LAUNCH();
     if (splits > 1) {
-        hipLaunchKernelGGL(attn_window_join_kernel<T>, dim3((unsigned)((a.nq * a.hq + 3) / 4)), dim3(256), 0, s, a, splits, part_o, part_ml);
+        const int64_t joined = a.nq * a.hq;
+        if (splits <= 4)
+            hipLaunchKernelGGL((attn_window_join_kernel<T, 4>), dim3((unsigned)((joined + 7) / 8)), dim3(256), 0, s, a, splits, part_o, part_ml);
+        else
+            hipLaunchKernelGGL((attn_window_join_kernel<T, kMaxSplits>), dim3((unsigned)((joined + 3) / 4)), dim3(256), 0, s, a, splits, part_o,
+                               part_ml);
         QCN_CHECK_LAUNCH();
     }
     return QCN_OK;

@@ -281,6 +281,29 @@ def test_window_rows_more_than_4_gib_apart(dim, dtype):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('win', [1100, 1700, 4000])
+@pytest.mark.parametrize('dim', [24, 40, 128])
+def test_window_split_into_few_and_many_parts_of_an_odd_number_of_rows(dim, win, dtype):
+    """81 rows in two, three and seven parts of the keys (the join takes one or two rows per wave); an infinity that two rows of three
+    heads see makes them, and only them, infinite or NaN."""
+    lens, extra, hq = [21, 6], [4000, 900], 3
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hq, dim, dtype, True, seed=50)
+    want = ref.window(q, k, v, cu_q, win, 2, cu_k, mask)
+    tol = ref.tolerance(dtype, dim, *want, float(v.double().abs().max()))
+    args = _dev(q, k, v, cu_q)
+    got = ops.attn_window(*args, win, 2, cu_k=cu_k.to(DEV), key_mask=mask.to(DEV)).cpu().double()
+    assert bool(((got - want[0]).abs() <= tol).all())
+    vv, seen = v.clone(), mask.clone()
+    vv[int(cu_k[1]) - 2] = float('inf')                        # the first sequence's last two queries reach it
+    seen[int(cu_k[1]) - 2] = True
+    got = ops.attn_window(args[0], args[1], vv.to(DEV), args[3], win, 2, cu_k=cu_k.to(DEV), key_mask=seen.to(DEV)).cpu().double()
+    assert not bool(torch.isfinite(got[19:21]).any())
+    keep = torch.ones(27, dtype=torch.bool)
+    keep[19:21] = False
+    assert bool(((got - want[0]).abs() <= tol)[keep].all())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_window_all_masked_and_large_scores(dtype):
     q, k, v, cu, _, _ = _case([45, 30], None, 4, 2, 32, dtype, False, seed=6)
     none = torch.zeros(75, dtype=torch.bool)
