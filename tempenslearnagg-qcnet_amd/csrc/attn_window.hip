@@ -584,8 +584,8 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 //
 // Bound by the matrix units and the vector instructions around them, which two or three waves per SIMD do not fully overlap
 // (timed with parts left out, 16384 x 16 heads of 128, window 1024: all 177 us, no products 109, no LDS reads 151, no exponentials
-// 167, no copies 175).  Measured: that case 165 us, 810 Tflop/s of the 1130 that a large library product reaches; 24 ragged
-// prompts up to 2500 x 12 heads of 64, window 512, float16: 90 us, 440 Tflop/s counting visible pairs only (32 rows see 9 or 10
+// 167, no copies 175).  Measured: that case 160 us, 840 Tflop/s of the 1130 that a large library product reaches; 24 ragged
+// prompts up to 2500 x 12 heads of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10
 // tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32
 // heads of 128 behind 7000 keys each, window 4096, in three parts: 107 us with the join, 670 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
