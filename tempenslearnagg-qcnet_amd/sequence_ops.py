@@ -18,6 +18,7 @@ import struct
 from typing import List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _as_u8, _op, _register, _require
@@ -38,14 +39,24 @@ _APPEND_ARGS = struct.Struct('=19q').pack
 _STEP_ARGS = struct.Struct('=18qd6q').pack
 
 
+# (names of this module: an attribute of a torch module costs as much as the question itself)
+_Tensor = torch.Tensor
+_compiling = torch.compiler.is_compiling
+_grad_enabled = torch.is_grad_enabled
+_dispatch_modes = torch._C._len_torch_dispatch_stack
+_recording = torch._C._is_tracing
+_transform = torch._C._functorch.peek_interpreter_stack
+
+
 def _plain(*tensors) -> bool:
-    """Whether the call can go to the implementation directly: plain tensors, nothing tracing, nothing to differentiate.  The
-    dispatcher costs 5 us a call, as much as everything else the host does for a decoding step."""
-    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack():
+    """Whether the call can go to the implementation directly: plain tensors, nothing tracing, no function transform (its wrappers
+    are of the plain type), nothing to differentiate in either direction.  The dispatcher costs 5 us a call, as much as everything
+    else the host does for a decoding step; all of the above have to see the operator, and a launch past it is nothing to them."""
+    if _compiling() or _dispatch_modes() or _recording() or _transform() is not None or forward_ad._current_level >= 0:
         return False
-    grad = torch.is_grad_enabled()
+    grad = _grad_enabled()
     for t in tensors:
-        if t is not None and (type(t) is not torch.Tensor or (grad and t.requires_grad)):
+        if t is not None and (type(t) is not _Tensor or (grad and t.requires_grad)):
             return False
     return True
 

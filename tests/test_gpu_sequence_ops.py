@@ -761,3 +761,46 @@ def test_sequence_ops_trace_under_fake_tensors():
         assert o.shape == (40, 8, 64) and o.dtype == torch.bfloat16
         c = torch.empty(40, 2, 9, 64, device=DEV, dtype=torch.bfloat16)
         assert ops.attn_window_step(q, k, k, torch.empty(40, dtype=torch.int64, device=DEV), c, c.clone(), 1).shape == (40, 8, 64)
+
+
+def test_a_recorded_function_runs_the_operators_again():
+    """torch.jit.trace records the four operators: run on other inputs, the recorded function gives what the eager calls give and
+    writes its caches."""
+    hq, hk, dim, win, sinks, dtype = 4, 2, 64, 24, 2, torch.bfloat16
+    freqs = torch.rand(dim // 2, generator=_gen(61)).to(DEV)
+    pos, lengths, zero = torch.arange(47, device=DEV).view(47, 1), torch.tensor([30, 17], device=DEV), torch.tensor([0, 0], device=DEV)
+
+    def run(q, k, v, cu, kc, vc):
+        q, k = ops.rotary_embed(q, k, pos, freqs, [dim // 2])
+        out = ops.attn_window(q, k, v, cu, win, sinks)
+        ops.window_cache_append(k, v, cu, zero, kc, vc, sinks)
+        return out, ops.attn_window_step(q[:2], k[:2], v[:2], lengths, kc, vc, sinks)
+
+    def inputs(seed):
+        q, k, v, cu, _, _ = _case([30, 17], None, hq, hk, dim, dtype, False, seed=seed)
+        cache = [torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV) for _ in range(2)]
+        return tuple(_dev(q, k, v, cu)) + tuple(cache)
+
+    again = torch.jit.trace(run, inputs(60), check_trace=False)
+    kinds = [n.kind() for n in again.graph.nodes()]
+    assert all('qcnet_hip::' + name in kinds for name in ops.SEQUENCE_OP_NAMES), kinds
+    for seed in (62, 63):
+        a, b = inputs(seed), inputs(seed)
+        want, got = run(*a), again(*b)
+        assert all(torch.equal(x, y) for x, y in zip(got + b, want + a))
+
+
+def test_function_transforms_see_the_operators():
+    """vmap over a batch equals the loop where the dispatcher can loop (an operator that returns one tensor) and is refused as an
+    operator without a batching rule where it cannot; dual numbers reach the operator, which has no forward derivative."""
+    g = _gen(64)
+    q, k, v = (_rand(g, 3, 10, 2, 16).to(DEV) for _ in range(3))
+    cu = torch.tensor([0, 4, 10], device=DEV)
+    attend = lambda q, k, v: ops.attn_window(q, k, v, cu, 3, 1)
+    assert torch.equal(torch.vmap(attend)(q, k, v), torch.stack([attend(*x) for x in zip(q, k, v)]))
+    pos, freqs = torch.arange(10, device=DEV).view(10, 1), torch.rand(8, generator=g).to(DEV)
+    with pytest.raises(RuntimeError, match='Batching rule not implemented for qcnet_hip::rotary_embed'):
+        torch.vmap(lambda t: ops.rotary_embed(t, None, pos, freqs, [8])[0])(q)
+    with torch.autograd.forward_ad.dual_level():
+        got = attend(torch.autograd.forward_ad.make_dual(q[0], q[1]), k[0], v[0])
+        assert torch.equal(torch.autograd.forward_ad.unpack_dual(got).primal, attend(q[0], k[0], v[0]))

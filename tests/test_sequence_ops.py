@@ -137,3 +137,40 @@ def test_rotary_form_keeps_lengths_and_turns_back():
         y = ref.rotary(x, pos, freqs, [5, 3], interleaved)
         assert torch.allclose(y.norm(dim=-1), x.double().norm(dim=-1))
         assert torch.allclose(ref.rotary(y, pos, freqs, [5, 3], interleaved, inverse=True), x.double())
+
+
+def test_calls_go_past_the_dispatcher_only_where_nothing_has_to_see_them():
+    """Plain eager tensors may; under a tracer, a function transform, a dual level or a dispatch mode, and with something to
+    differentiate, the call has to be an operator."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from tempenslearnagg_qcnet_amd import sequence_ops
+    seen = []
+
+    def f(t):
+        seen.append(sequence_ops._plain(t, None))
+        return t * 2
+
+    class Watching(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x = torch.ones(3, 2)
+    f(x)
+    with torch.no_grad():
+        f(x.clone().requires_grad_())
+    assert seen == [True, False] or seen == [True, True]       # no_grad: nothing to differentiate, either way is right
+    seen.clear()
+    torch.jit.trace(f, (x,), check_trace=False)
+    torch.vmap(f)(x)
+    torch.func.jvp(f, (x,), (x,))
+    torch.func.grad(lambda t: f(t).sum())(x)
+    torch.func.functionalize(f)(x)
+    with torch.autograd.forward_ad.dual_level():
+        f(torch.autograd.forward_ad.make_dual(x, x))
+    with Watching():
+        f(x)
+    f(x.clone().requires_grad_())
+    assert len(seen) == 8 and not any(seen), seen
+    seen.clear()
+    f(x)
+    assert seen == [True]
