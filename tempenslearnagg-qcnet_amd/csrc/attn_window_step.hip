@@ -87,8 +87,9 @@ struct StepArgs {
 // more, through LDS where that would be loads of 4 or 8 bytes.
 // The new token is read from the inputs, never from its slot, which another block of this launch is writing.
 //
-// Weights meet 16-bit V rounded to its type (relative error at most half a step; the output is rounded to the same type); a second
-// product with what the rounding left makes a step of 64 x 8 key heads x 4100 slots 1.9 % slower (183 against 179.6 us, both in two parts).
+// Weights meet 16-bit V in two products: rounded to its type, and with what that rounding left (16 bits of bfloat16, 22 of float16
+// together), so the output's rounding is the only one to 16 bits.  The kernel waits for memory, and the second product hardly shows: 64 x 8
+// key heads x 4100 slots 168.5 us against 168.2 with one product, one request 17.5 (17.6), 1600 agents x 51 slots in bfloat16 19.1 (18.4).
 // Measured: that step (64 requests x 32 heads of 128 in bfloat16) 168 us, 984 MB at 5.9 TB/s; one request 9.8 + 4.1
 // us (two launches, three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21 us, 4 TB/s.
 template <class T, int DP> struct Step {
@@ -258,16 +259,22 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
             using V8 = typename Mat<T>::V8;
 #pragma unroll
             for (int half = 0; half < L::NU / 2; ++half) {
-                V8 pb;
+                V8 hi, lo;                                     // p = hi + lo
 #pragma unroll
-                for (int i = 0; i < 8; ++i) pb[i] = from_f32<T>(s[2 * half + (i >> 2)][i & 3]);
+                for (int i = 0; i < 8; ++i) {
+                    const float p = s[2 * half + (i >> 2)][i & 3];
+                    hi[i] = from_f32<T>(p);
+                    lo[i] = from_f32<T>(p - to_f32(hi[i]));
+                }
                 const int i16 = lane & 15, r = 32 * half + 4 * g + (i16 >> 2);
 #pragma unroll
                 for (int dt = 0; dt < DP / 16; ++dt) {
                     const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
                     const uint2 x = lds_read_transposed(lds + r * L::V_ROW + v_piece<DP>(r, c) * 16 + byte);
                     const uint2 y = lds_read_transposed(lds + (r + 16) * L::V_ROW + v_piece<DP>(r + 16, c) * 16 + byte);
-                    o[dt] = Mat<T>::mul16(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), pb, o[dt]);
+                    const V8 vt = __builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y});
+                    o[dt] = Mat<T>::mul16(vt, hi, o[dt]);
+                    o[dt] = Mat<T>::mul16(vt, lo, o[dt]);
                 }
             }
         }

@@ -804,3 +804,37 @@ def test_function_transforms_see_the_operators():
     with torch.autograd.forward_ad.dual_level():
         got = attend(torch.autograd.forward_ad.make_dual(q[0], q[1]), k[0], v[0])
         assert torch.equal(torch.autograd.forward_ad.unpack_dual(got).primal, attend(q[0], k[0], v[0]))
+
+
+# ------------------------------------------------------------------------------------------------
+# weights of the 16-bit types
+# ------------------------------------------------------------------------------------------------
+HALVES = [torch.bfloat16, torch.float16]
+
+
+def _full_tolerance(dtype, dim, r, v_max):
+    """tolerance() of a form whose weights meet V as the sum of two numbers of the type.  With h half a step of the type, the rest of a
+    weight p after its rounding is at most h p, and that is rounded by at most h of itself: h^2 p is lost; float16 also loses up to half
+    of its smallest step (2^-25) of a rest, p relative to a sum of at least 1.  The output's rounding is the only one of size h."""
+    o, mag, reach, count = r
+    h = torch.finfo(dtype).eps / 2
+    tol = ref.tolerance(torch.float32, dim, *r, v_max) + h * o.abs() * 1.01 + h * h * 1.01 * mag
+    if dtype == torch.float16:
+        tol = tol + (count.unsqueeze(-1) + 1) * 2.0 ** -25 * v_max
+    return tol
+
+
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('ages,hq,hk,dim,win,sinks', [([1, 5, 0, 30], 8, 8, 16, 50, 1), ([1, 300, 2], 8, 2, 64, 200, 4),
+                                                      ([700, 1], 4, 1, 128, 600, 2), ([9000], 8, 1, 96, 2500, 0), ([3, 90], 3, 1, 32, 40, 0)])
+def test_step_weights_keep_their_bits(ages, hq, hk, dim, win, sinks, dtype):
+    q, k, v, lengths, kc, vc, km, mc = _step_case(ages, hq, hk, dim, win, sinks, False, dtype, seed=70)
+    got = ops.attn_window_step(*_dev(q, k, v, lengths, kc, vc), sinks).cpu().double()
+    r = ref.step(q, k, v, lengths, kc, vc, sinks)
+    tol = _full_tolerance(dtype, dim, r, float(vc.double().abs().max()))
+    assert bool(((got - r[0]).abs() <= tol).all()), float(((got - r[0]).abs() / tol).max())
+    # a mean of equal values is that value: before the rounding it is off by h^2 (2^-16 or less) and by what float32 sums of at most about
+    # 200 terms (one accumulator's) round, 2 x 200 x 2^-24, together less than 2^-14; half a step below 1 is 2^-9 or 2^-12
+    one = torch.ones_like(v), torch.ones_like(vc)
+    got = ops.attn_window_step(*_dev(q, k, one[0], lengths, kc, one[1]), sinks)
+    assert bool((got == 1).all()), got[got != 1]
