@@ -150,6 +150,10 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // features of a key for it; of narrow ones that would be loads of 4 or 8 bytes, four times as many instructions as the bytes
 // need, so their V comes like K and is turned in a few hundred bytes of LDS of the wave's own.
 //
+// Weights meet 16-bit V in two products, rounded to its type and with what that left (16 bits of bfloat16, 22 of float16 together):
+// these rows wait for memory and for each other's results, not for the matrix units (bfloat16, one product and two: 1600 agents x 59 steps x
+// 8 heads of 16 33.7 and 36 us, 8 x 2000 steps of 16 62.5 and 63, float16 800 x 59 of 32 28.6 and 29.3).
+//
 // Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48 us, 4.0 TB/s, bound by
 // the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
 // 80 Tflop/s of the 154 that a library product reaches (8 x 2000 steps, 8 heads of 64 or 128, window 500: 183 and 371 us); the L1
@@ -353,10 +357,15 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                         for (int r = 0; r < 4; ++r)
                             o[sb * L::VW + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[r].e[e], s[u][r], o[sb * L::VW + e], 0, 0, 0);
                     } else {
-                        typename Mat<T>::V4 va, pb;
+                        typename Mat<T>::V4 va, hi, lo;        // p = hi + lo
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) { va[r] = v[r].e[e]; pb[r] = from_f32<T>(s[u][r]); }
-                        o[sb * L::VW + e] = Mat<T>::mul16(va, pb, o[sb * L::VW + e]);
+                        for (int r = 0; r < 4; ++r) {
+                            va[r] = v[r].e[e];
+                            hi[r] = from_f32<T>(s[u][r]);
+                            lo[r] = from_f32<T>(s[u][r] - to_f32(hi[r]));
+                        }
+                        o[sb * L::VW + e] = Mat<T>::mul16(va, hi, o[sb * L::VW + e]);
+                        o[sb * L::VW + e] = Mat<T>::mul16(va, lo, o[sb * L::VW + e]);
                     }
                 }
             }

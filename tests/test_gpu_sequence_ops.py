@@ -838,3 +838,30 @@ def test_step_weights_keep_their_bits(ages, hq, hk, dim, win, sinks, dtype):
     one = torch.ones_like(v), torch.ones_like(vc)
     got = ops.attn_window_step(*_dev(q, k, one[0], lengths, kc, one[1]), sinks)
     assert bool((got == 1).all()), got[got != 1]
+
+
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('lens,hq,hk,dim,win,sinks', [([59, 1, 0, 16], 8, 8, 16, 10, 1), ([200, 17], 4, 2, 8, 90, 2), ([70, 40], 6, 2, 24, 10, 3),
+                                                      ([59, 30], 8, 8, 32, 16, 1), ([130], 7, 1, 16, 1000, 0)])
+def test_window_weights_of_narrow_heads_keep_their_bits(lens, hq, hk, dim, win, sinks, dtype):
+    q, k, v, cu, _, _ = _case(lens, None, hq, hk, dim, dtype, False, seed=71)
+    got = ops.attn_window(*_dev(q, k, v, cu), win, sinks).cpu().double()
+    r = ref.window(q, k, v, cu, win, sinks)
+    tol = _full_tolerance(dtype, dim, r, float(v.double().abs().max()))
+    assert bool(((got - r[0]).abs() <= tol).all()), float(((got - r[0]).abs() / tol).max())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('lens,extra,hq,hk,dim,win,sinks', [
+    ([59, 1, 0, 16], None, 8, 8, 16, 10, 1), ([150, 17], None, 4, 2, 16, 90, 2), ([59, 30], None, 8, 8, 32, 16, 1), ([59, 30], None, 8, 8, 32, 60, 1),
+    ([150, 70], None, 4, 2, 64, 120, 2), ([90, 3], None, 4, 1, 128, 50, 0), ([20, 6], [2500, 1100], 2, 1, 64, 2200, 2)])
+def test_window_weights_add_up_to_one(lens, extra, hq, hk, dim, win, sinks, dtype):
+    """A mean of equal values is that value.  The sum is either of the rounded weights that V meets or V meets all but h^2 of them; the rest
+    is what float32 sums of at most 700 terms (one part's, of the longest case) round, 2 x 700 x 2^-24 = 2^-13.5.  Half a step below 1 is
+    2^-9 or 2^-12 in 16 bits; float32 shows the rounding itself."""
+    q, k, v, cu_q, cu_k, _ = _case(lens, extra, hq, hk, dim, dtype, False, seed=72)
+    got = ops.attn_window(*_dev(q, k, torch.ones_like(v), cu_q), win, sinks, cu_k=None if extra is None else cu_k.to(DEV)).cpu().double()
+    if dtype == torch.float32:
+        assert float((got - 1).abs().max()) <= 2 * 2300 * 2.0 ** -24
+    else:
+        assert bool((got == 1).all()), got[got != 1]
