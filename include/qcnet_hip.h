@@ -535,7 +535,7 @@ int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream);
  * (j > p - window or j < sinks) and key_mask[j] (uint8 [n_k_tokens], NULL: all).  out [n_q_tokens, n_q_heads, dim] =
  * softmax(scale q.k) v over what it sees; rows that see nothing and rows behind cu_q[n_seq] are 0.  Masked keys and values may
  * hold anything, NaN and infinities among it.  Query head h reads key head h / (n_q_heads / n_kv_heads).
- * scale: finite, >= 0.  Token strides of k and v below 2^24 elements.  The workspace's contents do not outlive the call's work
+ * scale: 0 .. 2.35e38 (times log2(e) it has to be a float).  Token strides of k and v below 2^24 elements.  The workspace's contents do not outlive the call's work
  * on its stream. */
 typedef struct {
     const void *q;
@@ -579,7 +579,7 @@ int qcn_window_cache_append(const qcn_window_cache_append_args *args, void *stre
 /* One new token per sequence: k / v [batch, n_kv_heads, dim] go into the cache at position lengths[b], q [batch, n_q_heads,
  * dim] attends to what that position sees.  lengths[b] < 0 (or above 2^62): the row is not in use, its output is 0 and its cache
  * untouched.
- * lengths is not changed.  key_mask uint8 [batch]: whether the new token is visible.  The workspace's contents do not outlive
+ * lengths is not changed.  scale as above.  key_mask uint8 [batch]: whether the new token is visible.  The workspace's contents do not outlive
  * the call's work on its stream. */
 typedef struct {
     const void *q;

@@ -1110,7 +1110,7 @@ extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
     if (!args) return QCN_ERR_INVALID_ARGUMENT;
     const qcn_attn_window_args &x = *args;
     if (x.n_seq < 0 || x.n_q_tokens < 0 || x.n_k_tokens < 0 || x.n_q_heads < 1 || x.n_kv_heads < 1 || x.n_q_heads % x.n_kv_heads ||
-        x.window < 1 || x.sinks < 0 || !(x.scale >= 0.) || x.scale > 3.0e38 || !dtype_known(x.dtype))
+        x.window < 1 || x.sinks < 0 || !(x.scale >= 0.) || x.scale > kMaxScale || !dtype_known(x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
     const int64_t most = kMost;
     if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.n_q_tokens > most || x.n_k_tokens > most || x.n_seq > most ||

@@ -533,7 +533,7 @@ extern "C" int qcn_attn_window_step(const qcn_attn_window_step_args *args, void 
     if (!args) return QCN_ERR_INVALID_ARGUMENT;
     const qcn_attn_window_step_args &x = *args;
     if (x.batch < 0 || x.n_q_heads < 1 || x.n_kv_heads < 1 || x.n_q_heads % x.n_kv_heads || !cache_shape_ok(x.window, x.sinks) ||
-        !(x.scale >= 0.) || x.scale > 3.0e38 || !dtype_known(x.dtype) || (x.key_mask && !x.mask_cache))
+        !(x.scale >= 0.) || x.scale > kMaxScale || !dtype_known(x.dtype) || (x.key_mask && !x.mask_cache))
         return QCN_ERR_INVALID_ARGUMENT;
     if (x.dim < 8 || x.dim > kMaxDim || x.dim % 8 || x.n_q_heads > kMaxHeads || x.batch >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
     if (x.batch == 0) return QCN_OK;

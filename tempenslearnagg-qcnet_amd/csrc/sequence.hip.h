@@ -203,5 +203,6 @@ __device__ __forceinline__ float quarters_sum(float v) { const Pair p = both_row
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l); }
 
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kMaxScale = 2.35e38;   // times log2(e) it is still a float: an infinite one would make NaN of a score of 0
 
 }  // namespace qcn_seq

@@ -13,7 +13,6 @@ are float32 and every output is rounded once.  All of them launch on torch's cur
 their outputs with torch, never synchronise, and can be captured into graphs.
 """
 import functools
-import math
 import struct
 from typing import List, Optional, Sequence, Tuple
 
@@ -30,6 +29,7 @@ _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}            # QCN
 MAX_HEAD_DIM = 128
 _MOST = (1 << 62) - 1
 _MOST_TOK = 1 << 24      # token stride in elements
+_MAX_SCALE = 2.35e38      # times log2(e) it is still a float32
 _NO_SECTIONS = (0,) * 8
 
 # the argument structs of include/qcnet_hip.h (8-byte fields: no padding)
@@ -136,8 +136,8 @@ def _scale(scale: Optional[float], dim: int) -> float:
     if scale is None:
         return max(dim, 1) ** -0.5
     scale = float(scale)
-    if not (math.isfinite(scale) and 0 <= scale <= 3e38):
-        raise ValueError('scale must be finite and not negative, got %r' % scale)
+    if not 0 <= scale <= _MAX_SCALE:                          # (NaN is neither)
+        raise ValueError('scale must be 0 .. %g, got %r' % (_MAX_SCALE, scale))
     return scale
 
 

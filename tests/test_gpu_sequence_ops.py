@@ -865,3 +865,15 @@ def test_window_weights_add_up_to_one(lens, extra, hq, hk, dim, win, sinks, dtyp
         assert float((got - 1).abs().max()) <= 2 * 2300 * 2.0 ** -24
     else:
         assert bool((got == 1).all()), got[got != 1]
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_the_largest_scale(dtype):
+    """Equal scores of 0 stay a plain mean at every scale that is taken."""
+    q, k, v, cu, _, _ = _case([40, 9], None, 4, 2, 64, dtype, False, seed=73)
+    q = torch.zeros_like(q)
+    got = ops.attn_window(*_dev(q, k, v, cu), 12, 1, scale=2.35e38)
+    _check(got, ref.window(q, k, v, cu, 12, 1), dtype, 64, v)
+    _, _, _, lengths, kc, vc, _, _ = _step_case([30, 4], 4, 2, 64, 20, 1, False, dtype, seed=73)
+    got = ops.attn_window_step(*_dev(q[:2], k[:2], v[:2], lengths, kc, vc), 1, scale=2.35e38)
+    _check(got, ref.step(q[:2], k[:2], v[:2], lengths, kc, vc, 1), dtype, 64, vc)

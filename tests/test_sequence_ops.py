@@ -174,3 +174,21 @@ def test_calls_go_past_the_dispatcher_only_where_nothing_has_to_see_them():
     seen.clear()
     f(x)
     assert seen == [True]
+
+
+def test_scales_whose_base_2_form_is_no_float_are_refused():
+    """scale * log2(e) overflows float32 above 2.358e38, and an infinite factor makes NaN of a score of 0."""
+    lib = _lib.lib()
+    window = dict(q=FAKE, qs=(32, 16), k=FAKE, ks=(32, 16), v=FAKE, vs=(32, 16), cu_q=FAKE, cu_k=FAKE, mask=0, n_seq=1, nq=0, nk=4, hq=2,
+                  hk=2, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE, ws=0, ws_bytes=0)
+    step = dict(q=FAKE, qs=(512, 64), k=FAKE, ks=(512, 64), v=FAKE, vs=(512, 64), lengths=FAKE, key_mask=0, batch=0, hq=4, hk=2, dim=64,
+                dtype=2, window=4, sinks=1, scale=1.0, kc=FAKE, vc=FAKE, mc=0, out=FAKE, ws=0, ws_bytes=0)
+    for name, fmt, fields in (('qcn_attn_window', '21qd3q', window), ('qcn_attn_window_step', '18qd6q', step)):
+        assert _call(lib, name, fmt, fields, scale=2.35e38) == 0                # no tokens: nothing to do
+        for bad in (2.4e38, 2.9e38, 3.0e38):
+            assert _call(lib, name, fmt, fields, scale=bad) == INVALID, (name, bad)
+    x, n, c = torch.zeros(4, 2, 16), torch.zeros(4, dtype=torch.int64), torch.zeros(4, 2, 6, 16)
+    with pytest.raises(ValueError, match='scale'):
+        ops.attn_window(x, x, x, torch.tensor([0, 4]), 3, scale=2.4e38)
+    with pytest.raises(ValueError, match='scale'):
+        ops.attn_window_step(x, x, x, n, c, c.clone(), 1, scale=2.9e38)
