@@ -5,7 +5,7 @@ set -e
 cd "$(dirname "$0")/../../tempenslearnagg-qcnet_amd/csrc"
 OUT=../../scripts/dbg/exp
 mkdir -p $OUT/obj_$1
-FL="-O3 -std=c++17 -fPIC --offload-arch=gfx950 -Wno-unused-result -Wno-unused-value -I../../include -I. $2"
+FL="$(make -s flags) $2"
 for f in *.hip; do
   X=""; [ $f = fourier.hip ] && X="-fno-slp-vectorize"
   /opt/rocm/bin/hipcc $FL $X -c $f -o $OUT/obj_$1/${f%.hip}.o &
