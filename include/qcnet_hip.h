@@ -496,7 +496,8 @@ int qcn_nms_select_f32(const float *traj, const float *conf, const float *gt, in
  *
  * Row tensors are [tokens, heads, dim] with strides in ELEMENTS; the features of a head are contiguous and rows start on
  * 16-byte boundaries (rotary: on multiples of any access width, it adapts).  Strides are not negative.  dim: a multiple of 8, 8 .. 128 (rotary: even,
- * 2 .. 256).  Outputs are contiguous.  Boundaries `cu` are int64 [n_seq + 1], ascending, cu[0] = 0.  Accumulation, softmax
+ * 2 .. 256).  Sizes that take 2^24 blocks or more (2^28 appended tokens, 2^30 rows of a key head, 2^26 cache rows times key heads) are
+ * QCN_ERR_UNSUPPORTED.  Outputs are contiguous.  Boundaries `cu` are int64 [n_seq + 1], ascending, cu[0] = 0.  Accumulation, softmax
  * statistics and rotations are fp32, angles fp64; each output is rounded once.
  */
 #define QCN_DTYPE_F32 0

@@ -1018,7 +1018,7 @@ int launch_direct(const Args &a, hipStream_t s)
     while (hpw > 1 && tiles * ((a.hk + hpw - 1) / hpw) < 8 * (int64_t)qcn_num_cus()) hpw = (hpw + 1) / 2;
     const int groups = (a.hk + hpw - 1) / hpw;
     const int64_t blocks = tiles * groups;
-    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (blocks > kMaxBlocks) return QCN_ERR_UNSUPPORTED;
     const int64_t most = (int64_t)1 << 32, es = sizeof(T);
     const auto bytes = [&](int64_t tokens, int64_t tok, int64_t head, int64_t heads) { return (tokens * tok + heads * head + a.dim) * es; };
     const bool small = bytes(a.nq, a.qr.tok, a.qr.head, a.hq) < most && bytes(a.nk, a.kr.tok, a.kr.head, a.hk) < most &&
@@ -1054,7 +1054,7 @@ int launch_tile(const Args &a, void *workspace, int64_t workspace_bytes, hipStre
     const int64_t rows = a.nq * a.hq * splits;
     if (splits > 1 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < rows * (a.dim + 2) * 4)) return QCN_ERR_WORKSPACE_TOO_SMALL;
     const int64_t tiles = (a.nq * a.group >> kRowShift) + a.n_seq + 1, blocks = tiles * a.hk * splits;
-    if (blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (blocks > kMaxBlocks) return QCN_ERR_UNSUPPORTED;
     float *part_o = reinterpret_cast<float *>(workspace), *part_ml = splits > 1 ? part_o + rows * a.dim : nullptr;
     hipLaunchKernelGGL((attn_window_tile_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), 0, s, a, tiles, splits, part_o, part_ml);
     QCN_CHECK_LAUNCH();

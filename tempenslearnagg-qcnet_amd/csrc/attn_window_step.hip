@@ -462,7 +462,7 @@ template <class T, int DP>
 int launch_step_dim(const StepArgs &a, const Plan &p, float *ws, hipStream_t s)
 {
     const int64_t tasks = a.batch * a.hk * p.head_tiles * p.splits, blocks = p.waves == 4 ? tasks : (tasks + 3) / 4;
-    if (tasks >= ((int64_t)1 << 31) || blocks >= ((int64_t)1 << 31) || a.batch * a.hq >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (tasks >= ((int64_t)1 << 31) || blocks > kMaxBlocks || (p.splits > 1 && a.batch * a.hq > kMaxBlocks)) return QCN_ERR_UNSUPPORTED;
     const int64_t rows = a.batch * a.hq * p.splits;
     float *part_o = ws, *part_ml = ws ? ws + rows * a.dim : nullptr;
     if (p.waves == 4)
@@ -505,7 +505,7 @@ extern "C" int qcn_window_cache_append(const qcn_window_cache_append_args *args,
         !rows_aligned(x.k_cache, 0, 0, x.dtype) || !rows_aligned(x.v_cache, 0, 0, x.dtype))
         return QCN_ERR_INVALID_ARGUMENT;
     const int64_t blocks = (x.n_tokens >> kAppendShift) + x.n_seq + 1;
-    if (x.n_tokens >= ((int64_t)1 << 40) || x.n_seq >= ((int64_t)1 << 31) || blocks >= ((int64_t)1 << 31)) return QCN_ERR_UNSUPPORTED;
+    if (x.n_tokens >= ((int64_t)1 << 40) || x.n_seq >= ((int64_t)1 << 31) || blocks > kMaxBlocks) return QCN_ERR_UNSUPPORTED;
     const AppendArgs a = {x.k, x.v, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]}, x.cu, x.lengths, x.key_mask,
                           x.n_seq, x.n_tokens, (int)x.n_kv_heads, (int)x.dim, (int)x.dim * (int)dtype_bytes(x.dtype) / 16, x.window,
                           x.sinks, x.window + x.sinks, x.k_cache, x.v_cache, x.mask_cache};

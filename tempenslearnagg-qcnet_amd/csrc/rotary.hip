@@ -192,6 +192,7 @@ extern "C" int qcn_rotary_embed(const qcn_rotary_embed_args *args, void *stream)
     while (tpb > 1 && (x.n_tokens + tpb - 1) / tpb < 4 * cus) tpb /= 2;
     int hpb = heads;
     while (hpb > 4 && (x.n_tokens + tpb - 1) / tpb * ((heads + hpb - 1) / hpb) < 2 * cus) hpb = (hpb + 1) / 2;
+    if ((x.n_tokens + tpb - 1) / tpb > kMaxBlocks) return QCN_ERR_UNSUPPORTED;
     a.tokens_per_block = tpb;
     a.heads_per_block = hpb;
     const dim3 grid((unsigned)((x.n_tokens + tpb - 1) / tpb), (unsigned)((heads + hpb - 1) / hpb));

@@ -26,6 +26,8 @@ struct Rows {
 };
 
 constexpr int64_t kMaxHeads = 32767;            // of one tensor
+// a launch counts its threads in 32 bits, and the blocks here have 256
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 24) - 1;
 constexpr int64_t kMaxTokStride = (int64_t)1 << 24;   // elements: 64 rows' offsets are 32-bit
 
 // rows are loaded in 16-byte pieces, and strides do not point backwards

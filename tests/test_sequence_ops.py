@@ -192,3 +192,24 @@ def test_scales_whose_base_2_form_is_no_float_are_refused():
         ops.attn_window(x, x, x, torch.tensor([0, 4]), 3, scale=2.4e38)
     with pytest.raises(ValueError, match='scale'):
         ops.attn_window_step(x, x, x, n, c, c.clone(), 1, scale=2.9e38)
+
+
+def test_sizes_past_what_a_launch_can_count_are_refused():
+    """2^24 blocks of 256 threads are 2^32 threads, one more than a launch counts.  The sizes are refused before any launch, with the
+    status that other sizes which are not supported have."""
+    lib = _lib.lib()
+    window = dict(q=FAKE, qs=(16, 16), k=FAKE, ks=(16, 16), v=FAKE, vs=(16, 16), cu_q=FAKE, cu_k=FAKE, mask=0, n_seq=1, nq=1 << 30, nk=1 << 30,
+                  hq=1, hk=1, dim=16, dtype=0, window=3, sinks=0, scale=1.0, out=FAKE, ws=0, ws_bytes=0)
+    assert _call(lib, 'qcn_attn_window', '21qd3q', window) == UNSUPPORTED
+    assert _call(lib, 'qcn_attn_window', '21qd3q', window, hk=2, hq=4, dim=64, dtype=2) == UNSUPPORTED
+    assert _call(lib, 'qcn_attn_window', '21qd3q', window, nq=4, n_seq=1 << 24) == UNSUPPORTED
+    step = dict(q=FAKE, qs=(16, 16), k=FAKE, ks=(16, 16), v=FAKE, vs=(16, 16), lengths=FAKE, key_mask=0, batch=1 << 26, hq=1, hk=1, dim=16,
+                dtype=2, window=1, sinks=0, scale=1.0, kc=FAKE, vc=FAKE, mc=0, out=FAKE, ws=0, ws_bytes=0)
+    assert _call(lib, 'qcn_attn_window_step', '18qd6q', step) == UNSUPPORTED
+    assert _call(lib, 'qcn_attn_window_step', '18qd6q', step, batch=1 << 24, window=300) == UNSUPPORTED
+    append = dict(k=FAKE, ks=(16, 16), v=FAKE, vs=(16, 16), cu=FAKE, lengths=FAKE, key_mask=0, n_seq=1, n=1 << 28, hk=1, dim=16, dtype=0,
+                  window=3, sinks=0, kc=FAKE, vc=FAKE, mc=0)
+    assert _call(lib, 'qcn_window_cache_append', '19q', append) == UNSUPPORTED
+    rotary = dict(q=FAKE, qs=(8192, 256), hq=32, k=0, ks=(0, 0), hk=0, n=1 << 30, dim=256, dtype=0, pos=FAKE, pos_type=0, axes=1,
+                  sections=(8,) + (0,) * 7, freqs=FAKE, interleaved=0, inverse=0, q_out=FAKE, k_out=0)
+    assert _call(lib, 'qcn_rotary_embed', '27q', rotary) == UNSUPPORTED
