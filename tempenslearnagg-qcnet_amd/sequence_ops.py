@@ -132,9 +132,11 @@ def _window_workspace(index, code, n_seq, nq, nk, hq, hk, dim, window, sinks) ->
     return _on_device(index, _lib.lib().qcn_attn_window_workspace_bytes, args)
 
 
-def _scale(scale: Optional[float], dim: int) -> float:
+def _scale(scale: Optional[float], q: torch.Tensor) -> float:
     if scale is None:
-        return max(dim, 1) ** -0.5
+        if not isinstance(q, torch.Tensor):
+            raise TypeError('q must be a tensor')
+        return max(q.size(-1) if q.dim() else 1, 1) ** -0.5
     scale = float(scale)
     if not 0 <= scale <= _MAX_SCALE:                          # (NaN is neither)
         raise ValueError('scale must be 0 .. %g, got %r' % (_MAX_SCALE, scale))
@@ -218,8 +220,8 @@ def _rotary_embed(q, k, pos, freqs, sections, interleaved, inverse):
 # ------------------------------------------------------------------------------------------------
 # attention over ragged sequences
 # ------------------------------------------------------------------------------------------------
-def _check_kv(q, k, v) -> int:
-    """The type code of a matching set of rows, or the error."""
+def _check_kv(k, v) -> int:
+    """The type code of matching keys and values, or the error."""
     code = _dtype_code(k, 'k')
     dtype, index = k.dtype, k.get_device()
     ks = k.shape
@@ -232,12 +234,26 @@ def _check_kv(q, k, v) -> int:
         raise _lib.QcnError('head dim %d is not supported (a multiple of 8, 8 .. %d)' % (dim, MAX_HEAD_DIM))
     if hk < 1:
         raise ValueError('k has no heads')
-    if q is not None:
-        if not (isinstance(q, torch.Tensor) and q.dtype is dtype and q.get_device() == index and q.dim() == 3):
-            _rows(q, 'q', dtype, k.device)
-        if q.size(2) != dim or q.size(1) < 1 or q.size(1) % hk:
-            raise ValueError('q has shape %s: its dim must be %d and its heads a multiple of %d' % (tuple(q.shape), dim, hk))
     return code
+
+
+def _check_qkv(q, k, v) -> int:
+    code = _check_kv(k, v)
+    _, hk, dim = k.shape
+    if not (isinstance(q, torch.Tensor) and q.dtype is k.dtype and q.get_device() == k.get_device() and q.dim() == 3):
+        _rows(q, 'q', k.dtype, k.device)
+    if q.size(2) != dim or q.size(1) < 1 or q.size(1) % hk:
+        raise ValueError('q has shape %s: its dim must be %d and its heads a multiple of %d' % (tuple(q.shape), dim, hk))
+    return code
+
+
+def _mask_bytes(mask, name: str, index: int, device: torch.device, n: int):
+    """A mask of n as bytes in memory: bool as it is, anything else as ops.py's masks are taken."""
+    if _is(mask, torch.bool, index, (n,)):
+        return mask
+    if not isinstance(mask, torch.Tensor):
+        raise TypeError('%s must be a tensor' % name)
+    return _as_u8(mask, name, device, (n,))
 
 
 def attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, window: int, sinks: int = 0,
@@ -251,14 +267,14 @@ def attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     queries are its last positions).  ``key_mask`` bool [Nk]: false keys are seen by nobody, whatever k and v hold there.  A row
     that sees nothing is zero, and so are rows behind ``cu_q[-1]``.  ``scale`` defaults to D ** -0.5."""
     call = _attn_window if _plain(q, k, v, cu_q, cu_k, key_mask) else _op('attn_window')
-    return call(q, k, v, cu_q, int(window), int(sinks), cu_k, key_mask, _scale(scale, q.size(-1)))
+    return call(q, k, v, cu_q, int(window), int(sinks), cu_k, key_mask, _scale(scale, q))
 
 
 @_register('attn_window', '(Tensor q, Tensor k, Tensor v, Tensor cu_q, int window, int sinks, Tensor? cu_k, Tensor? key_mask, '
            'float scale) -> Tensor', lambda q, k, v, cu_q, window, sinks, cu_k, key_mask, scale: q.new_empty(q.shape),
            SEQUENCE_OP_NAMES)
 def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
-    code = _check_kv(q, k, v)
+    code = _check_qkv(q, k, v)
     index = k.get_device()
     nq, hq, dim = q.shape
     nk, hk, _ = k.shape
@@ -279,10 +295,9 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
         cu_k_ptr = cu_k.data_ptr()
     mask_ptr = 0
     if key_mask is not None:
-        if not _is(key_mask, torch.bool, index, (nk,)):
-            key_mask = _as_u8(key_mask, 'key_mask', k.device, (nk,))
+        key_mask = _mask_bytes(key_mask, 'key_mask', index, k.device, nk)
         mask_ptr = key_mask.data_ptr()
-    scale = _scale(scale, dim)
+    scale = _scale(scale, q)
     q, qs = _in_place(q)
     k, ks = _in_place(k)
     v, vs = _in_place(v)
@@ -351,7 +366,7 @@ def window_cache_append(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, leng
            'Tensor? key_mask, Tensor(c!)? mask_cache) -> ()',
            lambda k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, mask_cache: None, SEQUENCE_OP_NAMES)
 def _window_cache_append(k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, mask_cache):
-    code = _check_kv(None, k, v)
+    code = _check_kv(k, v)
     index = k.get_device()
     n, hk, dim = k.shape
     if not torch.is_tensor(cu) or cu.dim() != 1 or cu.numel() < 1:
@@ -362,8 +377,7 @@ def _window_cache_append(k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, m
     window, mask_cache_ptr = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch)
     mask_ptr = 0
     if key_mask is not None:
-        if not _is(key_mask, torch.bool, index, (n,)):
-            key_mask = _as_u8(key_mask, 'key_mask', k.device, (n,))
+        key_mask = _mask_bytes(key_mask, 'key_mask', index, k.device, n)
         mask_ptr = key_mask.data_ptr()
     k, ks = _in_place(k)
     v, vs = _in_place(v)
@@ -382,14 +396,14 @@ def attn_window_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     ``lengths`` is left as it is (see :func:`window_cache_append`).  A negative length marks a row that is not in use: its output
     is zero and its cache untouched.  ``key_mask`` bool [B]: whether the new token is visible, kept in ``mask_cache``."""
     call = _attn_window_step if _plain(q, k, v, lengths, k_cache, v_cache, key_mask, mask_cache) else _op('attn_window_step')
-    return call(q, k, v, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache, _scale(scale, q.size(-1)))
+    return call(q, k, v, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache, _scale(scale, q))
 
 
 @_register('attn_window_step', '(Tensor q, Tensor k, Tensor v, Tensor lengths, Tensor(a!) k_cache, Tensor(b!) v_cache, int sinks, '
            'Tensor? key_mask, Tensor(c!)? mask_cache, float scale) -> Tensor',
            lambda q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_cache, scale: q.new_empty(q.shape), SEQUENCE_OP_NAMES)
 def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_cache, scale):
-    code = _check_kv(q, k, v)
+    code = _check_qkv(q, k, v)
     index = k.get_device()
     batch, hq, dim = q.shape
     hk = k.size(1)
@@ -398,10 +412,9 @@ def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_
     window, mask_cache_ptr = _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch)
     mask_ptr = 0
     if key_mask is not None:
-        if not _is(key_mask, torch.bool, index, (batch,)):
-            key_mask = _as_u8(key_mask, 'key_mask', k.device, (batch,))
+        key_mask = _mask_bytes(key_mask, 'key_mask', index, k.device, batch)
         mask_ptr = key_mask.data_ptr()
-    scale = _scale(scale, dim)
+    scale = _scale(scale, q)
     q, qs = _in_place(q)
     k, ks = _in_place(k)
     v, vs = _in_place(v)

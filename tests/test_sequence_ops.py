@@ -213,3 +213,17 @@ def test_sizes_past_what_a_launch_can_count_are_refused():
     rotary = dict(q=FAKE, qs=(8192, 256), hq=32, k=0, ks=(0, 0), hk=0, n=1 << 30, dim=256, dtype=0, pos=FAKE, pos_type=0, axes=1,
                   sections=(8,) + (0,) * 7, freqs=FAKE, interleaved=0, inverse=0, q_out=FAKE, k_out=0)
     assert _call(lib, 'qcn_rotary_embed', '27q', rotary) == UNSUPPORTED
+
+
+def test_arguments_that_are_no_tensors_are_type_errors():
+    from tempenslearnagg_qcnet_amd import sequence_ops
+    x, n, c, cu = torch.zeros(4, 2, 16), torch.zeros(4, dtype=torch.int64), torch.zeros(4, 2, 6, 16), torch.tensor([0, 4])
+    for call in (lambda: ops.attn_window(None, x, x, cu, 3), lambda: ops.attn_window([1.0], x, x, cu, 3),
+                 lambda: ops.attn_window_step(None, x, x, n, c, c.clone(), 1), lambda: ops.attn_window(x, None, x, cu, 3, scale=1.0),
+                 lambda: ops.window_cache_append(None, x, cu, n, c, c.clone(), 1),
+                 lambda: ops.rotary_embed(None, None, torch.zeros(4, 1), torch.zeros(8), [8]),
+                 lambda: sequence_ops._mask_bytes([True] * 4, 'key_mask', 0, torch.device('cuda', 0), 4)):
+        with pytest.raises(TypeError, match='must be a tensor'):
+            call()
+    with pytest.raises(_lib.QcnError, match='no CPU fallback'):
+        ops.attn_window(torch.tensor(1.0), x, x, cu, 3)
