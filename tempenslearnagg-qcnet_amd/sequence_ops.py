@@ -27,7 +27,7 @@ SEQUENCE_OP_NAMES: List[str] = []
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}          # QCN_DTYPE_*
 _POS_TYPES = {torch.float32: 0, torch.int32: 1, torch.int64: 2}            # QCN_POS_*
 MAX_HEAD_DIM = 128
-_MOST = (1 << 62) - 1
+_MOST = (1 << 62) - 1      # windows and sinks above it mean the same, and operators take 64 bits
 _MOST_TOK = 1 << 24      # token stride in elements
 _MAX_SCALE = 2.35e38      # times log2(e) it is still a float32
 _NO_SECTIONS = (0,) * 8
@@ -128,7 +128,7 @@ def _step_workspace(index, batch, hq, hk, dim, window, sinks) -> int:
 
 @functools.lru_cache(maxsize=1024)
 def _window_workspace(index, code, n_seq, nq, nk, hq, hk, dim, window, sinks) -> int:
-    args = _WINDOW_ARGS(*[0] * 12, n_seq, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), 0.0, 0, 0, 0)
+    args = _WINDOW_ARGS(*[0] * 12, n_seq, nq, nk, hq, hk, dim, code, window, sinks, 0.0, 0, 0, 0)
     return _on_device(index, _lib.lib().qcn_attn_window_workspace_bytes, args)
 
 
@@ -267,7 +267,7 @@ def attn_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     queries are its last positions).  ``key_mask`` bool [Nk]: false keys are seen by nobody, whatever k and v hold there.  A row
     that sees nothing is zero, and so are rows behind ``cu_q[-1]``.  ``scale`` defaults to D ** -0.5."""
     call = _attn_window if _plain(q, k, v, cu_q, cu_k, key_mask) else _op('attn_window')
-    return call(q, k, v, cu_q, int(window), int(sinks), cu_k, key_mask, _scale(scale, q))
+    return call(q, k, v, cu_q, min(int(window), _MOST), min(int(sinks), _MOST), cu_k, key_mask, _scale(scale, q))
 
 
 @_register('attn_window', '(Tensor q, Tensor k, Tensor v, Tensor cu_q, int window, int sinks, Tensor? cu_k, Tensor? key_mask, '
@@ -304,7 +304,7 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
     out = _out_like(q)
     if nq:
         args = (q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu_q.data_ptr(), cu_k_ptr, mask_ptr,
-                n_cu - 1, nq, nk, hq, hk, dim, code, min(window, _MOST), min(sinks, _MOST), scale, out.data_ptr())
+                n_cu - 1, nq, nk, hq, hk, dim, code, window, sinks, scale, out.data_ptr())
         ws_ptr = ws_bytes = 0
         if code:                                            # 16-bit types: keys split over blocks when query tokens are few
             ws_bytes = _window_workspace(index, code, n_cu - 1, nq, nk, hq, hk, dim, window, sinks)

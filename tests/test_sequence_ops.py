@@ -227,3 +227,13 @@ def test_arguments_that_are_no_tensors_are_type_errors():
             call()
     with pytest.raises(_lib.QcnError, match='no CPU fallback'):
         ops.attn_window(torch.tensor(1.0), x, x, cu, 3)
+
+
+def test_windows_of_any_size_are_taken_by_the_operator_too(monkeypatch):
+    """A window past 64 bits is one that holds everything, whether the call goes through the dispatcher or past it."""
+    from tempenslearnagg_qcnet_amd import sequence_ops
+    x = torch.zeros(4, 2, 16)
+    for direct in (True, False):
+        monkeypatch.setattr(sequence_ops, '_plain', lambda *a: direct)
+        with pytest.raises(_lib.QcnError, match='no CPU fallback'):
+            ops.attn_window(x, x, x, torch.tensor([0, 4]), 1 << 70, 1 << 64)
