@@ -318,6 +318,11 @@ def _attn_window(q, k, v, cu_q, window, sinks, cu_k, key_mask, scale):
 # ------------------------------------------------------------------------------------------------
 # the bounded cache
 # ------------------------------------------------------------------------------------------------
+def _written(k_cache, v_cache, mask_cache) -> None:
+    """The caches have new contents: what autograd has saved of them is no longer what it was, and says so."""
+    torch._C._increment_version((k_cache, v_cache) if mask_cache is None else (k_cache, v_cache, mask_cache))
+
+
 def _check_cache(k, lengths, k_cache, v_cache, sinks, mask_cache, key_mask, batch):
     """(window, pointer of the mask cache) of a matching cache, or the error.  Caches are written in place: no copy stands in."""
     _, hk, dim = k.shape
@@ -385,6 +390,7 @@ def _window_cache_append(k, v, cu, lengths, k_cache, v_cache, sinks, key_mask, m
         _launch(index, 'qcn_window_cache_append', _APPEND_ARGS(
             k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], cu.data_ptr(), lengths.data_ptr(), mask_ptr, batch, n, hk, dim,
             code, window, sinks, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache_ptr))
+        _written(k_cache, v_cache, mask_cache)
 
 
 def attn_window_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: torch.Tensor, k_cache: torch.Tensor,
@@ -426,4 +432,5 @@ def _attn_window_step(q, k, v, lengths, k_cache, v_cache, sinks, key_mask, mask_
             q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], lengths.data_ptr(), mask_ptr, batch, hq,
             hk, dim, code, window, sinks, scale, k_cache.data_ptr(), v_cache.data_ptr(), mask_cache_ptr, out.data_ptr(),
             ws.data_ptr() if ws_bytes else 0, ws_bytes))
+        _written(k_cache, v_cache, mask_cache)
     return out

@@ -877,3 +877,25 @@ def test_the_largest_scale(dtype):
     _, _, _, lengths, kc, vc, _, _ = _step_case([30, 4], 4, 2, 64, 20, 1, False, dtype, seed=73)
     got = ops.attn_window_step(*_dev(q[:2], k[:2], v[:2], lengths, kc, vc), 1, scale=2.35e38)
     _check(got, ref.step(q[:2], k[:2], v[:2], lengths, kc, vc, 1), dtype, 64, vc)
+
+
+def test_writing_a_cache_shows_in_what_autograd_saved_of_it():
+    """A product of a cache with something trainable keeps the cache for its backward pass: appending or stepping in between is an error
+    there, as with torch's own operations in place, and not another gradient.  Inference tensors, which keep no count, are written too."""
+    def cache():
+        return tuple(torch.ones(2, 1, 6, 16, device=DEV) for _ in range(2)) + (torch.ones(2, 6, dtype=torch.bool, device=DEV),)
+
+    x, n, cu = torch.ones(2, 1, 16, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV), torch.tensor([0, 1, 2], device=DEV)
+    calls = (lambda kc, vc, mc: ops.window_cache_append(x, x, cu, n, kc, vc, 1, mask_cache=mc),
+             lambda kc, vc, mc: ops.attn_window_step(x, x, x, n, kc, vc, 1, mask_cache=mc))
+    for call in calls:
+        w = torch.ones(16, device=DEV, requires_grad=True)
+        kc, vc, mc = cache()
+        loss = (kc * w).sum() + (vc * w).sum()
+        before = [t._version for t in (kc, vc, mc)]
+        call(kc, vc, mc)
+        assert all(t._version > b for t, b in zip((kc, vc, mc), before))
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()
+        with torch.inference_mode():
+            call(*cache())
