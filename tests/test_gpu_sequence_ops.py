@@ -899,3 +899,55 @@ def test_writing_a_cache_shows_in_what_autograd_saved_of_it():
             loss.backward()
         with torch.inference_mode():
             call(*cache())
+
+
+@pytest.mark.parametrize('dtype', HALVES)
+@pytest.mark.parametrize('win,parts', [(1100, 2), (1700, 3), (2200, 4), (2700, 5), (3100, 6), (3600, 7), (4000, 8)])
+@pytest.mark.parametrize('dim', [24, 128])
+def test_window_split_into_every_number_of_parts(dim, win, parts, dtype):
+    from tempenslearnagg_qcnet_amd import sequence_ops
+    lens, extra, hq = [21, 6], [4000, 900], 3
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hq, dim, dtype, True, seed=51)
+    code = {torch.float16: 1, torch.bfloat16: 2}[dtype]
+    assert sequence_ops._window_workspace(0, code, 2, 27, k.size(0), hq, hq, dim, win, 2) == 27 * hq * parts * (dim + 2) * 4
+    got = ops.attn_window(*_dev(q, k, v, cu_q), win, 2, cu_k=cu_k.to(DEV), key_mask=mask.to(DEV))
+    _check(got, ref.window(q, k, v, cu_q, win, 2, cu_k, mask), dtype, dim, v)
+
+
+def test_two_threads_on_streams_of_their_own():
+    """Prompts and steps from two threads at once, each on its own stream with its own caches, are what one thread gives."""
+    import threading
+    hq, hk, dim, win, sinks, dtype = 8, 2, 64, 2200, 2, torch.bfloat16
+    q, k, v, cu_q, cu_k, mask = _case([20, 6], [2500, 1100], hq, hk, dim, dtype, True, seed=80)
+    dq, dk, dv, dcq, dck, dm = _dev(q, k, v, cu_q, cu_k, mask)
+    freqs, zero = torch.rand(dim // 2, generator=_gen(81)).to(DEV), torch.zeros(2, dtype=torch.int64, device=DEV)
+
+    def work(turns):
+        kc, vc = (torch.zeros(2, hk, win + sinks, dim, dtype=dtype, device=DEV) for _ in range(2))
+        mc = torch.zeros(2, win + sinks, dtype=torch.bool, device=DEV)
+        lengths = dck[1:] - dck[:-1]
+        ops.window_cache_append(dk, dv, dck, zero, kc, vc, sinks, key_mask=dm, mask_cache=mc)
+        outs = []
+        for i in range(turns):
+            outs.append(ops.attn_window(dq, dk, dv, dcq, win, sinks, cu_k=dck, key_mask=dm))
+            a, b = ops.rotary_embed(dq[i:i + 2], dk[i:i + 2], lengths.view(2, 1), freqs, [dim // 2])
+            outs.append(ops.attn_window_step(a, b, dv[i:i + 2], lengths, kc, vc, sinks, mask_cache=mc))
+            lengths = lengths + 1
+        return outs + [kc, vc, mc]
+
+    want, got = work(8), [None, None]
+    torch.cuda.synchronize()
+
+    def run(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got[i] = work(8)
+        stream.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g in got:
+        assert g is not None and len(g) == len(want) and all(torch.equal(x, y) for x, y in zip(g, want))

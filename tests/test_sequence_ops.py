@@ -237,3 +237,49 @@ def test_windows_of_any_size_are_taken_by_the_operator_too(monkeypatch):
         monkeypatch.setattr(sequence_ops, '_plain', lambda *a: direct)
         with pytest.raises(_lib.QcnError, match='no CPU fallback'):
             ops.attn_window(x, x, x, torch.tensor([0, 4]), 1 << 70, 1 << 64)
+
+
+def test_a_launch_for_a_device_that_is_not_current(monkeypatch):
+    """The launch happens with the tensors' device current and on that device's current stream, and so does the question for a
+    workspace; where it is current already, nothing is switched."""
+    from tempenslearnagg_qcnet_amd import sequence_ops
+    now, log = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            now.append(self.index)
+
+        def __exit__(self, *exc):
+            now.pop()
+
+    class Library:
+        def qcn_attn_window_step(self, args, stream):
+            log.append((now[-1], args, stream))
+            return 0
+
+        def qcn_attn_window_workspace_bytes(self, args):
+            log.append((now[-1], len(args)))
+            return 64
+
+        def qcn_status_string(self, status):
+            return b'refused'
+
+    library = Library()
+    monkeypatch.setattr(_lib, 'lib', lambda: library)
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: now[-1], raising=False)
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda index: 70 + index, raising=False)
+    monkeypatch.setattr(torch.cuda, 'device', Device)
+    sequence_ops._launch(0, 'qcn_attn_window_step', b'a')
+    sequence_ops._launch(3, 'qcn_attn_window_step', b'b')
+    assert log == [(0, b'a', 70), (3, b'b', 73)] and now == [0]
+    log.clear()
+    sequence_ops._window_workspace.cache_clear()
+    assert sequence_ops._window_workspace(2, 1, 1, 4, 4, 2, 2, 64, 9, 0) == 64 and log == [(2, 25 * 8)] and now == [0]
+    sequence_ops._window_workspace.cache_clear()
+    library.qcn_attn_window_step = lambda args, stream: INVALID
+    with pytest.raises(_lib.QcnError, match='refused'):
+        sequence_ops._launch(3, 'qcn_attn_window_step', b'c')
+    assert now == [0]
