@@ -491,14 +491,21 @@ int qcn_nms_select_f32(const float *traj, const float *conf, const float *gt, in
 
 /* ------------------------------------------------------------------------------------------------
  * Sequence operators: rotary positions, attention with a sliding window and sinks, and its bounded cache.  They have no
- * counterpart in the reference; they are the dense, edge-list-free form of its temporal attention
- * (modules/qcnet_agent_encoder.py:129-140: a causal band of time_span steps) for token sequences of any width.
+ * counterpart in the reference and none of its layers runs on them: a family of their own for token sequences of any width, beside
+ * its temporal attention (modules/qcnet_agent_encoder.py:129-140), which is a causal band over an edge list that leaves the own
+ * step out (1 .. time_span steps back) and adds a positional row per edge to k and v.  Here the band needs no edges, holds the own
+ * position (window = 10 is that and 9 before it), and positions are rotations of q and k.
  *
  * Row tensors are [tokens, heads, dim] with strides in ELEMENTS; the features of a head are contiguous and rows start on
- * 16-byte boundaries (rotary: on multiples of any access width, it adapts).  Strides are not negative.  dim: a multiple of 8, 8 .. 128 (rotary: even,
- * 2 .. 256).  Sizes that take 2^24 blocks or more (2^28 appended tokens, 2^30 rows of a key head, 2^26 cache rows times key heads) are
- * QCN_ERR_UNSUPPORTED.  Outputs are contiguous.  Boundaries `cu` are int64 [n_seq + 1], ascending, cu[0] = 0.  Accumulation, softmax
- * statistics and rotations are fp32, angles fp64; each output is rounded once.
+ * 16-byte boundaries (rotary: on multiples of any access width, it adapts).  Strides are not negative.  dim: a multiple of 8,
+ * 8 .. 128 (rotary: even, 2 .. 256).  Sizes that take 2^24 blocks or more (2^28 appended tokens, 2^30 rows of a key head, 2^26 cache
+ * rows times key heads) are QCN_ERR_UNSUPPORTED.  Outputs are contiguous.  Boundaries `cu` are int64 [n_seq + 1], ascending,
+ * cu[0] = 0.
+ *
+ * Scores, softmax statistics, sums and rotations are fp32, angles fp64, and each output is rounded once.  Softmax weights meet v in
+ * fp32 or, for 16-bit types, as the sum of two numbers of the type, but for one form: qcn_attn_window on 16-bit types with dim above
+ * 32, or above 16 and window + sinks above 17, rounds each weight to the type (and sums the rounded ones).  Its error against
+ * 64 bits is then 1.4 times what rounding the output alone makes.
  */
 #define QCN_DTYPE_F32 0
 #define QCN_DTYPE_F16 1
@@ -562,7 +569,8 @@ int qcn_attn_window(const qcn_attn_window_args *args, void *stream);
  * sinks + (p - sinks) % window; mask_cache uint8 [n_seq, sinks + window] (NULL: every token is visible).
  * append: sequence b brings cu[b + 1] - cu[b] tokens behind the lengths[b] (int64) it has; lengths is not changed (several
  * layers share it).  Tokens that fall out of the window within the call are not written; sequences with lengths[b] < 0 (or
- * above 2^62) and rows behind cu[n_seq] are left alone.  key_mask uint8 [n_tokens] (NULL: 1) goes into mask_cache. */
+ * above 2^62) and rows behind cu[n_seq] are left alone.  key_mask uint8 [n_tokens] (NULL: 1) goes into mask_cache.  k, v and key_mask
+ * may not lie in slots that the call writes (in other rows of the caches they may). */
 typedef struct {
     const void *k;
     int64_t k_strides[2];
@@ -580,8 +588,8 @@ int qcn_window_cache_append(const qcn_window_cache_append_args *args, void *stre
 /* One new token per sequence: k / v [batch, n_kv_heads, dim] go into the cache at position lengths[b], q [batch, n_q_heads,
  * dim] attends to what that position sees.  lengths[b] < 0 (or above 2^62): the row is not in use, its output is 0 and its cache
  * untouched.
- * lengths is not changed.  scale as above.  key_mask uint8 [batch]: whether the new token is visible.  The workspace's contents do not outlive
- * the call's work on its stream. */
+ * lengths is not changed.  scale as above.  key_mask uint8 [batch]: whether the new token is visible.  q, k, v and key_mask
+ * may not lie in the caches' written slots.  The workspace's contents do not outlive the call's work on its stream. */
 typedef struct {
     const void *q;
     int64_t q_strides[2];

@@ -152,9 +152,10 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 //
 // Weights meet 16-bit V in two products, rounded to its type and with what that left (16 bits of bfloat16, 22 of float16 together):
 // these rows wait for memory and for each other's results, not for the matrix units (bfloat16, one product and two: 1600 agents x 59 steps x
-// 8 heads of 16 33.7 and 36 us, 8 x 2000 steps of 16 62.5 and 63, float16 800 x 59 of 32 28.6 and 29.3).
+// 8 heads of 16 34.6 and 37 us, 8 x 2000 steps of 16 62.5 and 62.5, float16 800 x 59 of 32 28.9 and 29.4; one product of twice the
+// contraction for both was no faster).
 //
-// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48 us, 4.0 TB/s, bound by
+// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48.2 us, 4.0 TB/s, bound by
 // the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
 // 80 Tflop/s of the 154 that a library product reaches (8 x 2000 steps, 8 heads of 64 or 128, window 500: 183 and 371 us); the L1
 // cache is what bounds them (73 % of its cycles serve a request, against 57 % of the matrix units'): a load of 16 keys serves 16 rows.
@@ -174,7 +175,8 @@ template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 // OFF: byte offset inside one of the tensors; 32 bits where every tensor is below 4 GiB (a load then takes a scalar base).
 // Waves per SIMD asked for, against the compiler's own choice (8 x 2000 float32 steps x 8 heads, window 500; us): 16 features four
 // (76.5, own 85), 32 four (119.7, own 123.5), 64 four (183, own 196), 96 its own (390; three: 445), 128 two (371, own 388).  1600 x
-// 59 agent steps of 16 float32: 54.3 -> 51 us.  16-bit rows are faster with the compiler's three and no spills (34.0, four: 35.8).
+// 59 agent steps of 16 float32: 54.3 -> 51 us, and that kernel keeps two registers (12 bytes a lane) in scratch memory for it; the form
+// with 64-bit offsets 60 bytes.  16-bit rows are faster with the compiler's three and no spills (37, four: 43).
 template <class T, int DP> constexpr int direct_waves() { return sizeof(T) == 2 || DP == 96 ? 1 : DP <= 64 ? 4 : 2; }
 
 template <class T, int DP, class OFF>
@@ -581,9 +583,11 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // in flight while the matrix units work on this one, one barrier per tile.  v_mfma_f32_32x32x16: A = 32 keys (S^T) or 32 features
 // (O^T), B = 32 rows.  With the accumulator's row order, k-step t of key half-tile u contracts keys
 // 32 u + 16 t + {4 h .. 4 h + 3, 8 + 4 h ..}  in lane half h: V^T is fetched in that order by two transposing LDS reads, P^T is the
-// S^T registers rounded to 16 bits: a relative error of at most half a step of the type per weight (bfloat16 2^-9), below the
-// rounding of the output and averaged over the keys; the sum takes the rounded weights, so that they still add up to one.  A second
-// product with the remainders would cost half as much again of what bounds the kernel.
+// S^T registers rounded to 16 bits: a relative error of at most half a step of the type per weight (bfloat16 2^-8, float16 2^-11); the sum
+// takes the rounded weights, so that they add up to one.  The output is rounded to the same type, and its error against 64 bits is 1.4
+// times that of a form that keeps the weights (bfloat16 0.0023 against 0.00165, float16 0.00026 against 0.0002).  That is the price of one
+// product here: a second one with the remainders, as the direct form and the step have it, costs a quarter of the launch (one and two, us:
+// 16384 x 16 heads of 128, window 1024 177 and 222; the ragged prompts below 91 and 112; the chunks 110 and 144).
 //
 // LDS rows are swizzled in 16-byte pieces so that 16 neighbouring keys' pieces (K) and the 4 x 64 bytes of a transposing read
 // (V) cover all 64 banks; the copies write LDS in order and permute their source addresses.
@@ -591,12 +595,13 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // With few blocks (a short chunk of queries behind a long prefix) the key tiles are split over blocks as well and joined by a
 // second kernel.
 //
-// Bound by the matrix units and the vector instructions around them, which two or three waves per SIMD do not fully overlap
-// (timed with parts left out, 16384 x 16 heads of 128, window 1024: all 177 us, no products 109, no LDS reads 151, no exponentials
-// 167, no copies 175).  Measured: that case 160 us, 840 Tflop/s of the 1130 that a large library product reaches; 24 ragged
-// prompts up to 2500 x 12 heads of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10
-// tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32
-// heads of 128 behind 7000 keys each, window 4096, in three parts: 107 us with the join, 670 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
+// Bound by the matrix units and the vector instructions around them, which two or three waves per SIMD do not fully overlap (an
+// earlier state of the kernel, 177 us for 16384 x 16 heads of 128 and window 1024, timed with parts left out: no products 109, no
+// LDS reads 151, no exponentials 167, no copies 175).  Measured on a card at work (its first dozen launches after a pause take a tenth
+// longer): that case 160 us a call, 833 Tflop/s of the 1130 that a large library product reaches; 24 ragged prompts up to 2500 x 12 heads
+// of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10 tiles where one row's window is 8, and
+// 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32 heads of 128 behind 7000 keys each, window 4096, in three
+// parts: 105 us with the join, 680 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);

@@ -1,16 +1,19 @@
 """Token-sequence operators over the C ABI: rotary positions over several axes, attention with a sliding window and a few first
 tokens that stay visible, and its bounded cache with the single-token form.
 
-They are the dense form of what the encoders do with edge lists: the temporal attention of an agent is a causal band of
-``time_span`` steps (modules/qcnet_agent_encoder.py:129-140) whose positions enter through a 512-byte row per edge; here the
-band is a window over a ragged token sequence, positions are rotations of q and k, and a new time step costs one token
-(:func:`attn_window_step`) instead of a frame.  Forward only, like every operator of this package; the gradient of a rotation is
-the rotation with ``inverse=True``.
+They are a family of their own for token sequences; the models' layers do not run on them.  The temporal attention of an agent
+(modules/qcnet_agent_encoder.py:129-140) is a causal band over an edge list: 1 .. ``time_span`` steps back, the own step left out, with
+a 512-byte positional row per edge added to k and v.  Here the band is a window over a ragged sequence that holds the own position
+(``window=10``: that and the 9 before it), positions are rotations of q and k, and a new step costs one token
+(:func:`attn_window_step`).  Forward only, like every operator of this package; the gradient of a rotation is the rotation with
+``inverse=True``.
 
 Row tensors are ``[tokens, heads, dim]`` in float32, float16 or bfloat16 and may be views (of a fused projection, for one): rows
-whose features are contiguous and 16-byte aligned are read in place, anything else is copied first.  Sums and softmax statistics
-are float32 and every output is rounded once.  All of them launch on torch's current stream of the tensors' device, allocate
-their outputs with torch, never synchronise, and can be captured into graphs.
+whose features are contiguous and 16-byte aligned are read in place, anything else is copied first.  Scores, sums and softmax
+statistics are float32 and every output is rounded once.  Softmax weights meet v unrounded, but for :func:`attn_window` in 16-bit types
+with heads above 32 features (above 16 if window + sinks is above 17): the matrix units take them rounded to the type there, and
+the error against 64 bits is 1.4 times that of rounding the output alone.  All of them launch on torch's current stream of the
+tensors' device, allocate their outputs with torch, never synchronise, and can be captured into graphs.
 """
 import functools
 import struct
@@ -362,7 +365,8 @@ def window_cache_append(k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, leng
 
     Position p lies in slot p (p < sinks) or sinks + (p - sinks) % window.  ``lengths`` is left as it is, so that the layers of a
     model share it: advance it once per call of the model.  Sequences with a negative length and rows behind ``cu[-1]`` are left
-    alone.  ``mask_cache`` bool [B, sinks + window] takes ``key_mask`` [N] (true where that is None)."""
+    alone.  ``mask_cache`` bool [B, sinks + window] takes ``key_mask`` [N] (true where that is None).  k and v may be views of other
+    rows of the caches, but not of slots that the call writes."""
     call = _window_cache_append if _plain(k, v, cu, lengths, k_cache, v_cache, key_mask, mask_cache) else _op('window_cache_append')
     call(k, v, cu, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache)
 
@@ -400,7 +404,8 @@ def attn_window_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     [B, Hq, D] attends to what that position sees (:func:`attn_window`'s rule, out of the cache); returns [B, Hq, D].
 
     ``lengths`` is left as it is (see :func:`window_cache_append`).  A negative length marks a row that is not in use: its output
-    is zero and its cache untouched.  ``key_mask`` bool [B]: whether the new token is visible, kept in ``mask_cache``."""
+    is zero and its cache untouched.  ``key_mask`` bool [B]: whether the new token is visible, kept in ``mask_cache``.  q, k
+    and v may not lie in slots that the call writes."""
     call = _attn_window_step if _plain(q, k, v, lengths, k_cache, v_cache, key_mask, mask_cache) else _op('attn_window_step')
     return call(q, k, v, lengths, k_cache, v_cache, int(sinks), key_mask, mask_cache, _scale(scale, q))
 

@@ -951,3 +951,19 @@ def test_two_threads_on_streams_of_their_own():
         t.join()
     for g in got:
         assert g is not None and len(g) == len(want) and all(torch.equal(x, y) for x, y in zip(g, want))
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_a_cache_row_is_taken_over_by_another(dtype):
+    """The tokens of one row, as a view of the cache, appended to another row of the same cache; both then go on by themselves."""
+    hk, hq, dim, win, sinks, n = 2, 4, 64, 30, 2, 25
+    q, k, v, lengths, kc, vc, _, _ = _step_case([n, 0, 9], hq, hk, dim, win, sinks, False, dtype, seed=90)
+    dk, dv = kc.to(DEV), vc.to(DEV)
+    ops.window_cache_append(dk[0, :, :n].transpose(0, 1), dv[0, :, :n].transpose(0, 1), torch.tensor([0, 0, n, n], device=DEV),
+                            torch.tensor([n, 0, 9], device=DEV), dk, dv, sinks)
+    kc[1, :, :n], vc[1, :, :n] = kc[0, :, :n], vc[0, :, :n]
+    assert torch.equal(dk.cpu(), kc) and torch.equal(dv.cpu(), vc)
+    lengths[1] = n
+    got = ops.attn_window_step(*_dev(q, k, v, lengths), dk, dv, sinks)
+    _check(got, ref.step(q, k, v, lengths, kc, vc, sinks), dtype, dim, vc)
+    assert torch.equal(dk.cpu(), kc) and torch.equal(dv.cpu(), vc)
