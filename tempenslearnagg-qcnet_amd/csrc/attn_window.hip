@@ -10,7 +10,10 @@
 //   direct  16 rows per wave, operands straight from memory, no barrier: float32, and 16-bit rows of up to 16 features (up to 32
 //           where the window is short)
 //   tile    128 rows per block, 64-key tiles through LDS: wider 16-bit rows
-// Both keep one running maximum and sum per row, in float32, and go over the keys once.
+// Both keep one running maximum and sum per row, in float32, and go over the keys once; a second time only where a value is not
+// finite (one that some rows of a wave see and others do not reaches the others as 0 * inf).  Formed again row by row and key by key, as
+// they were before, such rows made a call hundreds of times as long (16384 x 16 heads of 128, window 1024, one infinite value in the
+// first token: 101 ms, now 0.59; none: 0.17).
 #include "sequence.hip.h"
 
 #include <type_traits>
@@ -27,33 +30,9 @@ struct Args {
     int64_t n_seq, nq, nk;
     int hq, hk, group, dim;
     int64_t window, sinks;
-    float scale, c2;      // c2: scale in base 2
+    float c2;             // scale in base 2
     void *out;            // [nq, hq, dim] contiguous
 };
-
-// One wave, one row, key by key: the form that is right for every input.
-template <class T>
-__device__ __forceinline__ void row_by_wave(const Args &a, int64_t k_beg, int64_t p, int64_t row, int head, int lane)
-{
-    const T *q = reinterpret_cast<const T *>(a.q) + row * a.qr.tok + head * a.qr.head;
-    const T *k = reinterpret_cast<const T *>(a.k) + k_beg * a.kr.tok + (head / a.group) * a.kr.head;
-    const T *v = reinterpret_cast<const T *>(a.v) + k_beg * a.vr.tok + (head / a.group) * a.vr.head;
-    const bool has0 = lane < a.dim, has1 = lane + 64 < a.dim;
-    const float q0 = has0 ? to_f32(q[lane]) : 0.f, q1 = has1 ? to_f32(q[lane + 64]) : 0.f;
-    WaveRow r;
-    const int64_t start = p - a.window + 1 > 0 ? p - a.window + 1 : 0;
-    const int64_t ns = a.sinks < start ? a.sinks : start;
-    for (int64_t i = 0; i < ns + (p + 1 - start); ++i) {
-        const int64_t j = i < ns ? i : start + (i - ns);
-        if (a.key_mask && !a.key_mask[k_beg + j]) continue;
-        const T *kj = k + j * a.kr.tok, *vj = v + j * a.vr.tok;
-        const float dot = (has0 ? q0 * to_f32(kj[lane]) : 0.f) + (has1 ? q1 * to_f32(kj[lane + 64]) : 0.f);
-        r.add(wave_sum(dot) * a.scale, has0 ? to_f32(vj[lane]) : 0.f, has1 ? to_f32(vj[lane + 64]) : 0.f);
-    }
-    T *o = reinterpret_cast<T *>(a.out) + (row * a.hq + head) * (int64_t)a.dim;
-    if (has0) o[lane] = from_f32<T>(r.result(0));
-    if (has1) o[lane + 64] = from_f32<T>(r.result(1));
-}
 
 // Rows behind the last sequence (and of sequences that see nothing): zero.
 template <class T>
@@ -175,8 +154,8 @@ template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 // OFF: byte offset inside one of the tensors; 32 bits where every tensor is below 4 GiB (a load then takes a scalar base).
 // Waves per SIMD asked for, against the compiler's own choice (8 x 2000 float32 steps x 8 heads, window 500; us): 16 features four
 // (76.5, own 85), 32 four (119.7, own 123.5), 64 four (183, own 196), 96 its own (390; three: 445), 128 two (371, own 388).  1600 x
-// 59 agent steps of 16 float32: 54.3 -> 51 us, and that kernel keeps two registers (12 bytes a lane) in scratch memory for it; the form
-// with 64-bit offsets 60 bytes.  16-bit rows are faster with the compiler's three and no spills (37, four: 43).
+// 59 agent steps of 16 float32: 54.3 -> 51 us, and that kernel keeps five registers (24 bytes a lane) in scratch memory for it; the form
+// with 64-bit offsets 80 bytes.  16-bit rows are faster with the compiler's three and no spills (37, four: 43).
 template <class T, int DP> constexpr int direct_waves() { return sizeof(T) == 2 || DP == 96 ? 1 : DP <= 64 ? 4 : 2; }
 
 template <class T, int DP, class OFF>
@@ -374,10 +353,11 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
     };
     // LDS of the wave's own: its accesses are done in order; only the compiler is to keep them apart
     const auto in_order = [&]() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); };
-    // o / l; a bit for each row that did not come out finite.  A value that is not finite, of a key that some rows of the tile see
-    // and others do not, reaches the others as 0 * inf: such rows are formed again key by key.
+    // o / l; whether a row of the wave came out not finite though its weights are numbers: the wave has loaded a value that is not
+    // finite, and a row that does not see its key has it as 0 * inf, and a row that does, perhaps, as (a weight too small for a float) * inf
     const auto divide = [&](float l, f32x4 (&o)[L::NT]) {
-        const float inv = inverse_sum(quarters_sum(l));
+        l = quarters_sum(l);
+        const float inv = inverse_sum(l);
         bool bad = false;
 #pragma unroll
         for (int i = 0; i < L::NT; ++i)
@@ -386,14 +366,7 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                 o[i][r] *= inv;
                 bad |= !(fabsf(o[i][r]) < INFINITY);
             }
-        const uint64_t b = __ballot(bad && n <= last);
-        return (unsigned)((b | (b >> 16) | (b >> 32) | (b >> 48)) & 0xffffu);
-    };
-    const auto again = [&](int kvh, unsigned rows) {
-        for (; rows; rows &= rows - 1) {
-            const int r = 16 * wave + __builtin_ctz(rows), token = t.token(r, a.group);
-            row_by_wave<T>(a, t.k_beg, token + t.shift, t.q_beg + token, kvh * a.group + t.sub(r, a.group), lane);
-        }
+        return __ballot(bad && l == l) != 0;
     };
     // the lane's 4 VW neighbouring features per sb, four at a time, to to(feature)
     const auto write = [&](const f32x4 (&o)[L::NT], auto to) {
@@ -414,16 +387,119 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
         }
     };
     const auto finish = [&](int kvh, float l, f32x4 (&o)[L::NT]) {
-        const unsigned bad = divide(l, o);
-        if (n <= last && !((bad >> n) & 1)) {
+        const bool bad = divide(l, o);
+        if (n <= last) {
             char *out = ob + (int64_t)kvh * a.group * a.dim * ES;
             write(o, [&](int d) { return out + (OFF)(o_off + (OFF)(d * ES)); });
         }
-        again(kvh, bad);
+        return bad;
     };
     const auto clear = [&](f32x4 (&o)[L::NT]) {
 #pragma unroll
         for (int i = 0; i < L::NT; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    };
+
+    const auto turn_v = [&](const Place &x, const Rows16 &rows) {   // narrow heads: V rows to LDS, masked ones as zeros
+        if constexpr (L::NARROW) {
+            T *mine = turn + wave * L::WAVE_ELEMS;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int c = 0; c < DP / 16; ++c) {
+                    P4 y = rows.v[u][c];
+                    if (mask) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y.e[e] = keep(y.e[e], x.seen[u][0]);
+                    }
+                    *reinterpret_cast<P4 *>(mine + (16 * u + n) * L::V_STRIDE + 16 * c + 4 * g) = y;
+                }
+            in_order();
+        }
+    };
+    // A head whose values are not all finite, again (a bit per head, from the 65th on shared): once over the keys for maximum and sum, once
+    // more with weights that add up to one.  V is taken in two parts: what is finite of it, and the codes of the rest against what each
+    // row sees, so that the rest reaches the rows that see it and no other.  Three to four times the head's first pass.
+    uint64_t again = 0;
+    const auto note = [&](int kvh, bool bad) { again |= bad ? 1ull << ((kvh - h0) & 63) : 0; };
+    const auto redo = [&](int kvh) {
+        f32x4 s[NU], o[L::NT];
+        const Query q = load_q(kvh);
+        float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+        for (int step = 0; step < chunks; ++step) {
+            const Place x = locate(step * L::CHUNK);
+            const float mn = fmaxf(m, scores(x, load(x, kvh), q, s));
+            l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn)) + softmax(s, mn);
+            m = mn;
+        }
+        l = quarters_sum(l);
+        // (float16: weights keep to the scale of the largest, as small ones would lose bits, and no sum of them overflows)
+        if (!std::is_same_v<T, _Float16> && l > 0.f && l < INFINITY) m += __builtin_amdgcn_logf(l);
+        clear(o);
+        float sum = 0.f;
+#pragma unroll 1
+        for (int step = 0; step < chunks; ++step) {
+            const Place x = locate(step * L::CHUNK);
+            const Rows16 rows = load(x, kvh);
+            scores(x, rows, q, s);
+            sum += softmax(s, m);
+            turn_v(x, rows);
+            const T *turned = turn + wave * L::WAVE_ELEMS;
+#pragma unroll
+            for (int sb = 0; sb < L::NSB; ++sb) {
+                f32x4 count[L::VW];
+#pragma unroll
+                for (int e = 0; e < L::VW; ++e) count[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    PV v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if constexpr (L::NARROW) v[r] = *reinterpret_cast<const PV *>(turned + (16 * u + 4 * g + r) * L::V_STRIDE + sb * L::SB + L::VW * n);
+                        else v[r] = value(x, kvh, u, sb, r);
+                    }
+#pragma unroll
+                    for (int e = 0; e < L::VW; ++e) {
+                        f32x4 &to = o[sb * L::VW + e];
+                        using V4 = T __attribute__((ext_vector_type(4)));
+                        V4 va, code, hi, lo, one;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            // (keys that are masked or behind the range are seen by no row)
+                            const float c = value_code(to_f32(v[r].e[e]));
+                            va[r] = c == 0.f ? v[r].e[e] : (T)0.f;
+                            code[r] = (T)c;
+                            hi[r] = from_f32<T>(s[u][r]);
+                            lo[r] = from_f32<T>(s[u][r] - to_f32(hi[r]));
+                            one[r] = (T)(x.sees[u][r] ? 1.f : 0.f);
+                        }
+                        if constexpr (F32) {
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                to = __builtin_amdgcn_mfma_f32_16x16x4f32(va[r], s[u][r], to, 0, 0, 0);
+                                count[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(code[r], one[r], count[e], 0, 0, 0);
+                            }
+                        } else {
+                            to = Mat<T>::mul16(va, hi, to);
+                            to = Mat<T>::mul16(va, lo, to);
+                            count[e] = Mat<T>::mul16(code, one, count[e]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < L::VW; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[sb * L::VW + e][r] += counted_sum(count[e][r]);
+            }
+            if constexpr (L::NARROW) in_order();
+        }
+        finish(kvh, sum, o);
+    };
+    const auto redo_noted = [&]() {
+        if (!again) return;
+        __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): behind the stores of the first pass
+        for (int kvh = h0; kvh < h1; ++kvh)
+            if ((again >> ((kvh - h0) & 63)) & 1) redo(kvh);
     };
 
     if constexpr (L::NARROW) {
@@ -500,7 +576,6 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                 }
                 in_order();
                 if (first + HP < h1) request(first + HP);
-                unsigned bad[HP] = {};
 #pragma unroll
                 for (int i = 0; i < HP; ++i) {
                     const int kvh = first + i;
@@ -511,7 +586,7 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                     const float m = scores(x, rows[i], q[i], s);
                     const float l = softmax(s, m);
                     accumulate(x, kvh, s, o, own + 16 * L::V_STRIDE);
-                    bad[i] = divide(l, o);
+                    note(kvh, divide(l, o));
                     // rows go out as they came in, through the place of q
                     in_order();
                     write(o, [&](int f) { return mine + i * L::HEAD_ELEMS + n * L::V_STRIDE + f; });
@@ -525,13 +600,8 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                                 *reinterpret_cast<const u32x4 *>(to + (lr + 8 * i) * L::V_STRIDE);
                 }
                 in_order();
-#pragma unroll
-                for (int i = 0; i < HP; ++i)
-                    if (bad[i]) {
-                        __builtin_amdgcn_s_waitcnt(0x0F70);    // vmcnt(0): behind the stores above
-                        again(first + i, bad[i]);
-                    }
             }
+            redo_noted();
             return;
         }
     }
@@ -554,26 +624,13 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                 m = mn;
             }
             l += softmax(s, m);
-            T *mine = turn + wave * L::WAVE_ELEMS;
-            if constexpr (L::NARROW) {
-#pragma unroll
-                for (int u = 0; u < NU; ++u)
-#pragma unroll
-                    for (int c = 0; c < DP / 16; ++c) {
-                        P4 y = rows.v[u][c];
-                        if (mask) {
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) y.e[e] = keep(y.e[e], x.seen[u][0]);
-                        }
-                        *reinterpret_cast<P4 *>(mine + (16 * u + n) * L::V_STRIDE + 16 * c + 4 * g) = y;
-                    }
-                in_order();
-            }
-            accumulate(x, kvh, s, o, mine);
+            turn_v(x, rows);
+            accumulate(x, kvh, s, o, turn + wave * L::WAVE_ELEMS);
             if constexpr (L::NARROW) in_order();
         }
-        finish(kvh, l, o);
+        note(kvh, finish(kvh, l, o));
     }
+    redo_noted();
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -601,7 +658,8 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // longer): that case 160 us a call, 833 Tflop/s of the 1130 that a large library product reaches; 24 ragged prompts up to 2500 x 12 heads
 // of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10 tiles where one row's window is 8, and
 // 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32 heads of 128 behind 7000 keys each, window 4096, in three
-// parts: 105 us with the join, 680 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us).
+// parts: 105 us with the join, 680 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us); at dim 32 they have to be asked for, as the
+// second pass would take 135 registers of the 115 that do (800 x 59 x 8 heads, window 30: 52 us, three waves 58).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);
@@ -639,7 +697,7 @@ __device__ __forceinline__ uint32_t lds_address(const void *p)
 }
 
 template <class T, int DP>
-__global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_t n_tiles, int splits, float *part_o, float *part_ml)
+__global__ __launch_bounds__(256, DP == 32 ? 4 : 2) void attn_window_tile_kernel(Args a, int64_t n_tiles, int splits, float *part_o, float *part_ml)
 {
     constexpr int LS = DP == 96 ? 128 : DP;                    // elements of an LDS row
     constexpr int PIECES = LS / 8, PER = LS / 32, NK = DP / 16, ND = DP / 32, TILE = kKeys * LS;
@@ -872,6 +930,8 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
             }
         __builtin_amdgcn_sched_barrier(0);
     };
+    __shared__ int any_redo;                                   // set at the end, many barriers later (a wave without steps sets nothing)
+    if (tid == 0) any_redo = 0;
     if (s0 < s1) {
         load(s0, 0, std::false_type{});
         load(s0, 0, std::true_type{});
@@ -881,61 +941,137 @@ __global__ __launch_bounds__(256, 2) void attn_window_tile_kernel(Args a, int64_
         }
     }
     l = halves_sum(l + l2);
-    if (splits > 1) {
-        // joined by attn_window_join_kernel: this part's maximum, sum and numerators
-        const int64_t at = out_row * splits + split;
-        if (real && h == 0) { part_ml[2 * at] = m; part_ml[2 * at + 1] = l; }
-        if (real && m != -INFINITY) {
+    T *out = reinterpret_cast<T *>(a.out) + out_row * a.dim;
+    const auto emit = [&]() {
+        if (splits > 1) {
+            // joined by attn_window_join_kernel: this part's maximum, sum and numerators
+            const int64_t at = out_row * splits + split;
+            if (real && h == 0) { part_ml[2 * at] = m; part_ml[2 * at + 1] = l; }
+            if (real && m != -INFINITY) {
 #pragma unroll
-            for (int i = 0; i < ND; ++i)
+                for (int i = 0; i < ND; ++i)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int d = 32 * i + 8 * x + 4 * h;
-                    if (d < a.dim) *reinterpret_cast<f32x4 *>(part_o + at * a.dim + d) = f32x4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]};
-                }
+                    for (int x = 0; x < 4; ++x) {
+                        const int d = 32 * i + 8 * x + 4 * h;
+                        if (d < a.dim) *reinterpret_cast<f32x4 *>(part_o + at * a.dim + d) = f32x4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]};
+                    }
+            }
+            return;
         }
-        return;
-    }
-    const float inv = inverse_sum(l);
+        const float inv = inverse_sum(l);
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {                      // 16 features: halves hold {0-3, 8-11} and {4-7, 12-15}
+                unsigned w[2][2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const int r = 8 * x + 4 * y + 2 * z;
+                        Pack<T, 2> two = {{from_f32<T>(o[i][r] * inv), from_f32<T>(o[i][r + 1] * inv)}};
+                        w[y][z] = __builtin_bit_cast(unsigned, two);
+                    }
+                const auto w0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
+                const auto w1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
+                const int d = 32 * i + 16 * x + 8 * h;         // after the exchange a lane holds 8 neighbouring features
+                if (real && d < a.dim) *reinterpret_cast<u32x4 *>(out + d) = u32x4{w0[0], w1[0], w0[1], w1[1]};
+            }
+    };
+    // A value that is not finite, of a key that some rows of the wave see and others do not, reaches the others as 0 * inf.  A row whose
+    // weights are not numbers either (l) is NaN by itself; where a row ends before DP its last scores are products with the copied
+    // start of a key, and only the second pass says.
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            o[i][r] *= inv;
-            bad |= !(fabsf(o[i][r]) < INFINITY);
-        }
-    unsigned repair;
-    {
-        const uint64_t b = __ballot(bad && real);
-        repair = (unsigned)(b | (b >> 32));
-    }
-    T *out = reinterpret_cast<T *>(a.out) + out_row * a.dim;
-    const bool keep = real && !((repair >> n) & 1);
+        for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[i][r]) < INFINITY);
+    const bool redo = __ballot(bad && (l == l || a.dim < DP)) != 0;
+    if (redo) any_redo = 1;
+    else emit();
+    __syncthreads();
+    if (!any_redo) return;
+
+    // The second pass over the keys, for such waves: the maximum is known, and so is the scale that makes the weights add up to one.  V is
+    // taken in two parts: what is finite of it, and the codes of the rest against what each row sees.  A simple loop: the block's
+    // time with it is three to five times that of the first pass alone.
+    if (!std::is_same_v<T, _Float16> && l > 0.f && l < INFINITY) m += __builtin_amdgcn_logf(l);
+    l = 0.f;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {                          // 16 features: halves hold {0-3, 8-11} and {4-7, 12-15}
-            unsigned w[2][2];
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+    for (int step = s0; step < s1; ++step) {
+        __syncthreads();                                       // the last tiles have been read
+        load(step, 0, std::false_type{});
+        load(step, 0, std::true_type{});
+        const uint64_t seen = seen_keys(step * kKeys);
+        copies_landed();
+        T *lk = buffer(0, 0), *lv = buffer(0, 1), *lc = buffer(1, 1);
+#pragma unroll 1
+        for (int i = 0; i < PER; ++i) {
+            const int x = (PER * wave + i) * 64 + lane, row = x / PIECES;
+            V8 v = *reinterpret_cast<const V8 *>(lv + 8 * x), code;
 #pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    const int r = 8 * x + 4 * y + 2 * z;
-                    Pack<T, 2> two = {{from_f32<T>(o[i][r]), from_f32<T>(o[i][r + 1])}};
-                    w[y][z] = __builtin_bit_cast(unsigned, two);
-                }
-            const auto w0 = __builtin_amdgcn_permlane32_swap(w[0][0], w[1][0], false, false);
-            const auto w1 = __builtin_amdgcn_permlane32_swap(w[0][1], w[1][1], false, false);
-            const int d = 32 * i + 16 * x + 8 * h;             // after the exchange a lane holds 8 neighbouring features
-            if (keep && d < a.dim) *reinterpret_cast<u32x4 *>(out + d) = u32x4{w0[0], w1[0], w0[1], w1[1]};
+            for (int e = 0; e < 8; ++e) {
+                const float c = (seen >> row) & 1 ? value_code(to_f32(v[e])) : 0.f;
+                v[e] = (seen >> row) & 1 && c == 0.f ? v[e] : (T)0.f;
+                code[e] = (T)c;
+            }
+            *reinterpret_cast<V8 *>(lv + 8 * x) = v;
+            *reinterpret_cast<V8 *>(lc + 8 * x) = code;
+            if (8 * k_piece<LS>(row, x % PIECES) >= a.dim) *reinterpret_cast<u32x4 *>(lk + 8 * x) = u32x4{0, 0, 0, 0};
         }
-    // A value that is not finite, of a key that some rows of the tile see and others do not, reaches the others as 0 * inf.
-    // Rows that came out not finite are formed again key by key.
-    for (; repair; repair &= repair - 1) {
-        const int r = wave * 32 + __builtin_ctz(repair), token = t.token(r, a.group);
-        row_by_wave<T>(a, t.k_beg, token + t.shift, t.q_beg + token, kvh * a.group + t.sub(r, a.group), lane);
+        __syncthreads();
+        if (!redo || !(step < es || (step >= ea && step < eb))) continue;
+        f32x16 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NK; ++c) {
+                const int kr = 32 * u + n;
+                s[u] = Mat<T>::mul32(*reinterpret_cast<const V8 *>(&lk[kr * LS + 8 * k_piece<LS>(kr, 2 * c + h)]), qf[c], s[u]);
+            }
+        }
+        const uint64_t vis = sees.bits(step * kKeys) & seen;
+        V8 weight[4], one[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned w = (unsigned)(vis >> (32 * (k >> 1))) >> (4 * h);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = 8 * (k & 1) + i, bit = (r & 3) + 8 * (r >> 2);
+                weight[k][i] = from_f32<T>(__builtin_amdgcn_exp2f(fmaf(seen_or_inf(w, bit, s[k >> 1][r]), c2, -base)));
+                one[k][i] = (T)(float)((w >> bit) & 1);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l = Mat<T>::add_pair(weight[k], i, l);
+        }
+        const int i16 = lane & 15;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) {
+            f32x16 count;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) count[r] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int vr = 16 * k + 4 * h + (i16 >> 2), d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+                const int at = vr * LS + 8 * v_piece<LS>(vr, d >> 3) + (d & 7), at8 = (vr + 8) * LS + 8 * v_piece<LS>(vr + 8, d >> 3) + (d & 7);
+                const uint2 x = lds_read_transposed(lv + at), y = lds_read_transposed(lv + at8);
+                const uint2 cx = lds_read_transposed(lc + at), cy = lds_read_transposed(lc + at8);
+                o[dt] = Mat<T>::mul32(__builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y}), weight[k], o[dt]);
+                count = Mat<T>::mul32(__builtin_bit_cast(V8, u32x4{cx.x, cx.y, cy.x, cy.y}), one[k], count);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[dt][r] += counted_sum(count[r]);
+        }
     }
+    l = halves_sum(l);
+    if (redo) emit();
 }
 
 // Joins the parts of a row, all requested before the first is used: half a wave per (token, query head) and 16 bytes of a part per
@@ -969,46 +1105,32 @@ __global__ __launch_bounds__(256) void attn_window_join_kernel(Args a, int split
         ov[s] = *reinterpret_cast<const Vec *>(part_o + at * a.dim + (has ? d : 0));
         top = fmaxf(top, ml[s].x);
     }
-    float sum = 0.f;
+    // a part that saw nothing has no numerators; its sum is 0, or NaN where every score was
+    float f[PARTS], sum = 0.f;
+#pragma unroll
+    for (int s = 0; s < PARTS; ++s) {
+        f[s] = ml[s].x != -INFINITY ? __builtin_amdgcn_exp2f(ml[s].x - top) : 0.f;
+        sum = fmaf(f[s], ml[s].y, sum);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     Vec x = {};
 #pragma unroll
     for (int s = 0; s < PARTS; ++s) {
-        const bool saw = ml[s].x != -INFINITY;                 // a part that saw nothing has no numerators; its sum is 0, or NaN
-        const float f = saw ? __builtin_amdgcn_exp2f(ml[s].x - top) : 0.f;   // where every score was
-        sum = fmaf(f, ml[s].y, sum);
+        const bool saw = ml[s].x != -INFINITY;
+        const float w = f[s] * inv;                            // (weights first: numerators may be as large as a float is)
 #pragma unroll
-        for (int e = 0; e < VE; ++e) x[e] = saw ? fmaf(f, ov[s][e], x[e]) : x[e];
+        for (int e = 0; e < VE; ++e) {
+            const float v = ov[s][e];
+            // an infinity that the row sees is one however small its part's share
+            x[e] = saw ? (fabsf(v) < INFINITY ? fmaf(w, v, x[e]) : x[e] + v) : x[e];
+        }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < VE; ++e) {
-        x[e] *= inv;
-        bad |= !(fabsf(x[e]) < INFINITY);
-    }
-    const uint64_t again = __ballot(bad && has && real);       // see the end of the tile kernel
-    const auto of_row = [&](int r) { return LANES == 64 ? again : (uint64_t)(unsigned)(again >> (LANES * r)); };
-    if (has && real && !of_row(lane / LANES)) {
+    if (sum != sum) x = sum;                                   // a score that is no number, in a part that has no numerators
+    if (has && real) {
         Pack<T, VE> y;
 #pragma unroll
         for (int e = 0; e < VE; ++e) y.e[e] = from_f32<T>(x[e]);
         *reinterpret_cast<Pack<T, VE> *>(reinterpret_cast<T *>(a.out) + row * a.dim + d) = y;
-    }
-    for (int half = 0; half < ROWS; ++half) {
-        if (!of_row(half)) continue;
-        const int64_t token = (row0 + half) / a.hq;
-        const int head = (int)((row0 + half) % a.hq);
-        int64_t lo = 0, hi = a.n_seq;                          // last sequence that starts at or before token
-        while (lo + 1 < hi) {
-            const int64_t mid = (lo + hi) / 2;
-            if (clamp64(a.cu_q[mid], 0, a.nq) <= token) lo = mid;
-            else hi = mid;
-        }
-        int64_t q_beg, q_end, k_beg, k_end;
-        seq_range(a.cu_q, lo, a.nq, q_beg, q_end);
-        seq_range(a.cu_k, lo, a.nk, k_beg, k_end);
-        if (token >= q_beg && token < q_end)
-            row_by_wave<T>(a, k_beg, token - q_beg + (k_end - k_beg) - (q_end - q_beg), token, head, lane);
     }
 }
 
@@ -1131,7 +1253,7 @@ extern "C" int qcn_attn_window(const qcn_attn_window_args *args, void *stream)
     const int64_t window = x.window < most ? x.window : most, sinks = x.sinks < most ? x.sinks : most;
     const Args a = {x.q, x.k, x.v, {x.q_strides[0], x.q_strides[1]}, {x.k_strides[0], x.k_strides[1]}, {x.v_strides[0], x.v_strides[1]},
                     x.cu_q, x.cu_k, x.key_mask, x.n_seq, x.n_q_tokens, x.n_k_tokens, (int)x.n_q_heads, (int)x.n_kv_heads,
-                    (int)(x.n_q_heads / x.n_kv_heads), (int)x.dim, window, sinks, (float)x.scale,
+                    (int)(x.n_q_heads / x.n_kv_heads), (int)x.dim, window, sinks,
                     // an unseen key's score is -inf and has to stay so: scale 0 becomes one that no score outgrows
                     fmaxf((float)x.scale * kLog2e, 1e-37f), x.out};
     hipStream_t s = qcn_stream(stream);

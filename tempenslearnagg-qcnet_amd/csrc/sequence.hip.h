@@ -116,22 +116,17 @@ __device__ __forceinline__ float wave_sum(float v)
     return v;
 }
 
-// Streaming softmax of one row held by a whole wave: lane owns features lane and lane + 64.  -inf scores of an empty
-// prefix are kept out of the exponent, so a row that sees nothing ends with l = 0.
-struct WaveRow {
-    float m = -INFINITY, l = 0.f, acc[2] = {0.f, 0.f};
-    __device__ __forceinline__ void add(float score, float v0, float v1)
-    {
-        const float mn = fmaxf(m, score);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float alpha = expf(m - base), p = expf(score - base);
-        l = fmaf(l, alpha, p);
-        acc[0] = fmaf(p, v0, acc[0] * alpha);
-        acc[1] = fmaf(p, v1, acc[1] * alpha);
-        m = mn;
-    }
-    __device__ __forceinline__ float result(int i) const { return l == 0.f ? 0.f : acc[i] / l; }
-};
+// Values that are not finite, as numbers that a product can count: +inf 1, -inf 128, NaN both.  The products of the codes of up to
+// 127 keys with 1 (a row sees the key) or 0 say what the row's sum holds of each.
+__device__ __forceinline__ float value_code(float v)
+{
+    return fabsf(v) < INFINITY ? 0.f : (v > 0.f ? 1.f : (v < 0.f ? 128.f : 129.f));
+}
+__device__ __forceinline__ float counted_sum(float c)   // +inf, -inf, NaN (of both) or 0
+{
+    const float minus = floorf(c * (1.f / 128.f));
+    return (c > 128.f * minus ? INFINITY : 0.f) + (minus > 0.f ? -INFINITY : 0.f);
+}
 
 // ---------------------------------------------------------------------------------------------------------------------
 // matrix operands

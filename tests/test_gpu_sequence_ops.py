@@ -967,3 +967,109 @@ def test_a_cache_row_is_taken_over_by_another(dtype):
     got = ops.attn_window_step(*_dev(q, k, v, lengths), dk, dv, sinks)
     _check(got, ref.step(q, k, v, lengths, kc, vc, sinks), dtype, dim, vc)
     assert torch.equal(dk.cpu(), kc) and torch.equal(dv.cpu(), vc)
+
+
+# ------------------------------------------------------------------------------------------------
+# values that are not finite
+# ------------------------------------------------------------------------------------------------
+FORMS = [
+    # lens, extra keys, hq, hk, dim, window, sinks: every form of the window attention, and rows that end inside its width
+    ([59, 1, 0, 16], None, 8, 8, 16, 10, 1), ([150, 70], None, 4, 2, 16, 90, 2), ([70, 40], None, 6, 2, 24, 10, 3),
+    ([150, 70], None, 4, 2, 32, 60, 1), ([150, 70], None, 4, 2, 40, 60, 1), ([150, 300], None, 4, 2, 64, 100, 2),
+    ([130, 31], None, 4, 1, 80, 50, 1), ([130], None, 3, 3, 96, 40, 0), ([150, 70], None, 4, 1, 128, 60, 2),
+    ([20, 6], [2500, 1100], 2, 1, 64, 2200, 2), ([9], [4000], 3, 1, 72, 3600, 0),
+]
+
+
+def _same_kind(got, want, tol):
+    """NaN where it is NaN, an infinity of the same sign where it is one, near where it is finite."""
+    assert bool((got.isnan() == want.isnan()).all()), (got.isnan() != want.isnan()).nonzero()[:4]
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf]) and bool((got.isinf() == inf).all())
+    fine = torch.isfinite(want)
+    assert bool(((got - want).abs() <= tol)[fine].all()), float(((got - want).abs() / tol)[fine].max())
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('form', range(len(FORMS)))
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(form, dtype):
+    """Single features of some keys are NaN or infinite, masked keys are NaN throughout: each element of each row is what the sum over
+    the keys that the row sees makes it, in float64."""
+    lens, extra, hq, hk, dim, win, sinks = FORMS[form]
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hk, dim, dtype, True, seed=100 + form)
+    g = _gen(101 + form)
+    fine = float(v.double().abs().max())
+    tol = ref.tolerance(dtype, dim, *ref.window(q, k, v, cu_q, win, sinks, cu_k, mask), fine)
+    vv = v.clone()
+    for fill in (float('nan'), float('inf'), -float('inf')):
+        hit = torch.rand(v.size(0), hk, 1, generator=g) < 0.04
+        vv[(hit & (torch.rand(v.shape, generator=g) < 0.2))] = fill
+    vv[0, 0, dim - 1] = float('inf')
+    k, vv = k.clone(), vv.clone()
+    k[~mask], vv[~mask] = float('nan'), float('nan')
+    want = ref.window(q, torch.where(mask[:, None, None], k, torch.zeros_like(k)), vv, cu_q, win, sinks, cu_k, mask)[0]
+    got = ops.attn_window(*_dev(q, k, vv, cu_q), win, sinks, cu_k=None if extra is None else cu_k.to(DEV), key_mask=mask.to(DEV))
+    _same_kind(got.cpu().double(), want, tol)
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('form', range(len(FORMS)))
+def test_a_score_of_minus_infinity_counts_for_nothing(form, dtype):
+    """A key whose first feature is -inf, against queries whose first is 1: its score is -inf and its weight 0, also where a row ends inside
+    the width that the kernel works on.  Beside it, a value of another key is infinite, so that the rows are formed a second time."""
+    lens, extra, hq, hk, dim, win, sinks = FORMS[form]
+    q, k, v, cu_q, cu_k, mask = _case(lens, extra, hq, hk, dim, dtype, True, seed=120 + form)
+    at = int(cu_q[1] if extra is None else cu_k[1]) - 2
+    mask[at - 1:at + 1] = True
+    q, k, vv = q.clone(), k.clone(), v.clone()
+    q[..., 0] = 1
+    k[at, :, 0] = -float('inf')
+    vv[at - 1, :, dim // 2] = float('inf')
+    rest = mask.clone()
+    rest[at] = False
+    kk = k.clone()
+    kk[at] = 0
+    tol = ref.tolerance(dtype, dim, *ref.window(q, kk, v, cu_q, win, sinks, cu_k, rest), float(v.double().abs().max()))
+    for values in (v, vv):
+        want = ref.window(q, kk, values, cu_q, win, sinks, cu_k, rest)[0]
+        got = ops.attn_window(*_dev(q, k, values, cu_q), win, sinks, cu_k=None if extra is None else cu_k.to(DEV), key_mask=mask.to(DEV))
+        _same_kind(got.cpu().double(), want, tol)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('form', range(len(FORMS)))
+def test_means_of_values_near_the_largest_float(form, dtype):
+    """Values of 1e38 to 3e38: their sums are no floats, their means are."""
+    lens, extra, hq, hk, dim, win, sinks = FORMS[form]
+    q, k, v, cu_q, cu_k, _ = _case(lens, extra, hq, hk, dim, dtype, False, seed=140 + form)
+    v = ((torch.rand(v.shape, generator=_gen(141)) + 0.5) * 2e38).to(dtype)
+    r = ref.window(q, k, v, cu_q, win, sinks, cu_k)
+    got = ops.attn_window(*_dev(q, k, v, cu_q), win, sinks, cu_k=None if extra is None else cu_k.to(DEV)).cpu().double()
+    assert bool(((got - r[0]).abs() <= ref.tolerance(dtype, dim, *r, float(v.double().abs().max()))).all())
+
+
+@pytest.mark.parametrize('lens,extra,hq,hk,dim,win,dtype', [
+    ([4096], None, 8, 2, 128, 1024, torch.bfloat16), ([4096], None, 8, 8, 32, 1024, torch.float16), ([200, 333], [3000, 3000], 8, 2, 64, 3000, torch.bfloat16),
+    ([700] * 4, None, 4, 4, 64, 500, torch.float32), ([700] * 4, None, 8, 8, 16, 500, torch.float32)])
+def test_a_value_that_is_not_finite_does_not_cost_hundreds_of_calls(lens, extra, hq, hk, dim, win, dtype):
+    """An infinite value that every row sees, queries that are NaN, values that are NaN throughout: a second pass over the keys at most, three
+    to five times the call (a bound of 30 leaves room for a busy card)."""
+    q, k, v, cu_q, cu_k, _ = _case(lens, extra, hq, hk, dim, dtype, False, seed=160)
+    q, k, v, cu_q, cu_k = _dev(q, k, v, cu_q, cu_k)
+    sink, gone = v.clone(), torch.full_like(v, float('nan'))
+    sink[(cu_q if extra is None else cu_k)[:-1]] = float('inf')
+
+    def time(q, v):
+        times = []
+        for _ in range(7):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            ops.attn_window(q, k, v, cu_q, win, 1, cu_k=cu_k)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return sorted(times)[3]
+
+    plain = time(q, v)
+    for args in ((q, sink), (torch.full_like(q, float('nan')), v), (q, gone)):
+        assert time(*args) < 30 * plain
