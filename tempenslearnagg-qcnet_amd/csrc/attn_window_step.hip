@@ -88,8 +88,10 @@ struct StepArgs {
 // The new token is read from the inputs, never from its slot, which another block of this launch is writing.
 //
 // Weights meet 16-bit V in two products: rounded to its type, and with what that rounding left (16 bits of bfloat16, 22 of float16
-// together), so the output's rounding is the only one to 16 bits.  The kernel waits for memory, and the second product hardly shows: 64 x 8
-// key heads x 4100 slots 168.5 us against 168.2 with one product, one request 17.5 (17.6), 1600 agents x 51 slots in bfloat16 19.1 (18.4).
+// together), so the output's rounding is the only one to 16 bits.  The kernel waits for memory, and that hardly shows where it has much to
+// read (us, one product and two, with the look for values that are not finite that the second needs): 64 x 8 key heads x 4100 slots 170 and
+// 171, one request 19.9 and 20.4, 256 x 4 heads of 64 x 1004 slots 47.8 and 48.5, 64 x 8 x 240 slots 25.1 and 26.6, 1600 agents x 8 x 51
+// slots in bfloat16 19.2 and 20.2.
 // Measured: that step (64 requests x 32 heads of 128 in bfloat16) 168 us, 984 MB at 5.9 TB/s; one request 9.8 + 4.1
 // us (two launches, three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21 us, 4 TB/s.
 template <class T, int DP> struct Step {
@@ -280,6 +282,54 @@ __device__ __forceinline__ void attend_slots(const StepArgs &a, const Part &t, i
         }
         if constexpr (L::TURN) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+    if constexpr (!L::F32) {
+        // An infinite value has met two parts of a weight, of which one may be 0 or below.  All heads of the task see the same slots, so
+        // the values alone say what becomes of such a feature: they are gone over again, without keys and weights, 32 slots at a time.
+        f32x4 any = o[0];                                  // not finite if an element is not (an overflow costs a look)
+#pragma unroll
+        for (int i = 1; i < DP / 16; ++i) any += o[i];
+        const float sum = (any[0] + any[1]) + (any[2] + any[3]);
+        if (__ballot(!(fabsf(sum) < INFINITY) && l == l)) {
+            using V8 = typename Mat<T>::V8;
+            V8 one;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) one[i] = (T)1.f;
+            f32x4 held[DP / 16];                           // 0, or what is not finite among a feature's values
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) held[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int64_t j0 = t.c0 + 32 * wave; j0 < t.c1; j0 += 32 * waves) {
+#pragma unroll 1
+                for (int x = lane; x < 32 * L::PIECES; x += 64) {
+                    const int r = x / L::PIECES, c = x % L::PIECES;
+                    const int64_t slot = j0 + r;
+                    u32x4 v = {0, 0, 0, 0};
+                    if (slot < t.c1 && (slot == t.slot ? new_seen : (!mask || mask[slot] != 0)))
+                        v = piece(slot == t.slot ? vn : vc + slot * a.dim, c * L::PIECE);
+                    *reinterpret_cast<u32x4 *>(lds + r * L::V_ROW + v_piece<DP>(r, c) * 16) = v;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                const int i16 = lane & 15, r = 4 * g + (i16 >> 2);
+#pragma unroll
+                for (int dt = 0; dt < DP / 16; ++dt) {
+                    const int c = 2 * dt + ((i16 >> 1) & 1), byte = 8 * (i16 & 1);
+                    const uint2 x = lds_read_transposed(lds + r * L::V_ROW + v_piece<DP>(r, c) * 16 + byte);
+                    const uint2 y = lds_read_transposed(lds + (r + 16) * L::V_ROW + v_piece<DP>(r + 16, c) * 16 + byte);
+                    V8 code = __builtin_bit_cast(V8, u32x4{x.x, x.y, y.x, y.y});
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) code[i] = (T)value_code(to_f32(code[i]));
+                    const f32x4 count = Mat<T>::mul16(code, one, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) held[dt][i] += counted_sum(count[i]);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][r] = held[i][r] == 0.f ? o[i][r] : held[i][r];
+        }
+    }
     l = quarters_sum(l);
 }
 
@@ -359,7 +409,9 @@ __global__ __launch_bounds__(256, WAVES == 1 && DP <= 16 ? 6 : 1) void attn_wind
             for (int w = 0; w < 4; ++w) {
                 const float mw = ml[w][hd][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - top);
                 sum = fmaf(f, ml[w][hd][1], sum);
-                if (mw != -INFINITY) acc = fmaf(f, reinterpret_cast<float *>(lds + w * L::WAVE_BYTES)[hd * L::O_STRIDE + d], acc);
+                const float x = reinterpret_cast<float *>(lds + w * L::WAVE_BYTES)[hd * L::O_STRIDE + d];
+                // an infinity is one however small its wave's share
+                if (mw != -INFINITY) acc = fabsf(x) < INFINITY ? fmaf(f, x, acc) : acc + x;
             }
             const int64_t row = t.b * a.hq + t.head0 + hd;
             if (splits == 1) {
@@ -419,8 +471,8 @@ __global__ __launch_bounds__(256) void attn_window_step_join_kernel(StepArgs a, 
             const int s = s0 + 4 * i;
             const float g = __shfl(f, s < splits ? s : 0), mg = __shfl(own.x, s < splits ? s : 0);
             if (s < splits && mg != -INFINITY) {
-                x = fmaf(g, v[i].x, x);
-                y = fmaf(g, v[i].y, y);
+                x = fabsf(v[i].x) < INFINITY ? fmaf(g, v[i].x, x) : x + v[i].x;
+                y = fabsf(v[i].y) < INFINITY ? fmaf(g, v[i].y, y) : y + v[i].y;
             }
         }
     }

@@ -1073,3 +1073,24 @@ def test_a_value_that_is_not_finite_does_not_cost_hundreds_of_calls(lens, extra,
     plain = time(q, v)
     for args in ((q, sink), (torch.full_like(q, float('nan')), v), (q, gone)):
         assert time(*args) < 30 * plain
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('case', range(len(STEPS)))
+def test_step_values_that_are_not_finite(case, dtype):
+    """Single features of some slots and of the new token are NaN or infinite: infinities of one sign stay what they are, both signs or a NaN
+    among a feature's seen values make NaN, and the other features stay near."""
+    ages, hq, hk, dim, win, sinks, masked = STEPS[case]
+    q, k, v, lengths, kc, vc, km, mc = _step_case(ages, hq, hk, dim, win, sinks, masked, dtype, seed=170)
+    clone = lambda t: None if t is None else t.clone()
+    r = ref.step(q, k, v, lengths, kc.clone(), vc.clone(), sinks, km, clone(mc))
+    tol = ref.tolerance(dtype, dim, *r, float(vc.double().abs().max()))
+    g = _gen(171 + case)
+    for fill in (float('nan'), float('inf'), -float('inf')):
+        vc[(torch.rand(vc.shape, generator=g) < 1.2 / vc.size(2))] = fill
+        v[(torch.rand(v.shape, generator=g) < 0.1)] = fill
+    got = ops.attn_window_step(*_dev(q, k, v, lengths, kc, vc), sinks, key_mask=None if km is None else km.to(DEV),
+                               mask_cache=None if mc is None else mc.to(DEV))
+    want = ref.step(q, k, v, lengths, kc, vc, sinks, km, mc)[0]
+    assert bool(want.isinf().any()) and bool(torch.isfinite(want).any())
+    _same_kind(got.cpu().double(), want, tol)
