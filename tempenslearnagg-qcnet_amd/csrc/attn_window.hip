@@ -131,8 +131,8 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 //
 // Weights meet 16-bit V in two products, rounded to its type and with what that left (16 bits of bfloat16, 22 of float16 together):
 // these rows wait for memory and for each other's results, not for the matrix units (bfloat16, one product and two: 1600 agents x 59 steps x
-// 8 heads of 16 34.6 and 37 us, 8 x 2000 steps of 16 62.5 and 62.5, float16 800 x 59 of 32 28.9 and 29.4; one product of twice the
-// contraction for both was no faster).
+// 8 heads of 16 33.9 and 35.4 us, 8 x 2000 steps of 16 62 and 61, float16 800 x 59 of 32 28.8 and 28.5, the second with the pass below for
+// values that are not finite; one product of twice the contraction for both was no faster).
 //
 // Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48.2 us, 4.0 TB/s, bound by
 // the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
@@ -152,36 +152,26 @@ template <class T, int DP> struct Direct {
 template <class T, int N> struct alignas(sizeof(T) * N) Pack { T e[N]; };
 
 // OFF: byte offset inside one of the tensors; 32 bits where every tensor is below 4 GiB (a load then takes a scalar base).
-// Waves per SIMD asked for, against the compiler's own choice (8 x 2000 float32 steps x 8 heads, window 500; us): 16 features four
-// (76.5, own 85), 32 four (119.7, own 123.5), 64 four (183, own 196), 96 its own (390; three: 445), 128 two (371, own 388).  1600 x
-// 59 agent steps of 16 float32: 54.3 -> 51 us, and that kernel keeps five registers (24 bytes a lane) in scratch memory for it; the form
-// with 64-bit offsets 80 bytes.  16-bit rows are faster with the compiler's three and no spills (37, four: 43).
+// Waves per SIMD asked for, against the compiler's own choice, measured before there was a second pass (8 x 2000 float32 steps x 8 heads,
+// window 500; us): 16 features four (76.5, own 85), 32 four (119.7, own 123.5), 64 four (183, own 196), 96 its own (390; three: 445), 128
+// two (371, own 388); today 70, 119, 182, 369 and 370.  1600 x 59 agent steps of 16 float32: 54.3 -> 51 us; 123 registers, and the form with
+// 64-bit offsets keeps eight (36 bytes a lane) in scratch memory.  16-bit rows are faster with the compiler's three (35, four with spills: 43).
 template <class T, int DP> constexpr int direct_waves() { return sizeof(T) == 2 || DP == 96 ? 1 : DP <= 64 ? 4 : 2; }
 
-template <class T, int DP, class OFF>
-__global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_direct_kernel(Args a, int64_t n_tiles, int heads_per_wave, int head_groups)
+// The 16 rows of a wave over its key heads.  Returns which heads hold values that are not finite (a bit per head, from the 65th on
+// shared); AGAIN: the second pass of those.
+template <class T, int DP, class OFF, bool AGAIN>
+__device__ __forceinline__ uint64_t direct_rows(const Args &a, const Tile &t, int wave, int lane, int h0, int h1, T *turn, uint64_t again)
 {
     using L = Direct<T, DP>;
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int NU = L::NU;
-    __shared__ __attribute__((aligned(16))) T turn[4 * L::WAVE_ELEMS];
-    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
-    const int64_t tile = item / (unsigned)head_groups;
-    const int h0 = (int)(item % (unsigned)head_groups) * heads_per_wave, h1 = h0 + heads_per_wave < a.hk ? h0 + heads_per_wave : a.hk;
-    const Tile t = find_tile(a, tile, n_tiles, 6, lane);
+    const int n = lane & 15, g = lane >> 4;
     const int64_t row0 = t.row0 + 16 * wave;
-    if (t.row0 < 0 || row0 >= t.rows) return;
     const int last = (int)((t.rows - 1 - row0) < 15 ? (t.rows - 1 - row0) : 15);
     const int r_own = 16 * wave + (n < last ? n : last);   // lanes past the end repeat the last row and do not store
     const int64_t qi = t.token(r_own, a.group);
     const int sub = t.sub(r_own, a.group);                 // query head inside the group
-    if (t.behind) {
-        if (n <= last)
-            for (int kvh = h0; kvh < h1; ++kvh) zero_row<T>(a, t.q_beg + qi, kvh * a.group + sub, g, 4);
-        return;
-    }
     const int p = (int)qi + t.shift;
     const int p0 = t.token(16 * wave, a.group) + t.shift, p1 = t.token(16 * wave + last, a.group) + t.shift;
     const Keys keys = key_range(a, p0, p1);
@@ -416,91 +406,89 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
             in_order();
         }
     };
-    // A head whose values are not all finite, again (a bit per head, from the 65th on shared): once over the keys for maximum and sum, once
-    // more with weights that add up to one.  V is taken in two parts: what is finite of it, and the codes of the rest against what each
-    // row sees, so that the rest reaches the rows that see it and no other.  Three to four times the head's first pass.
-    uint64_t again = 0;
-    const auto note = [&](int kvh, bool bad) { again |= bad ? 1ull << ((kvh - h0) & 63) : 0; };
-    const auto redo = [&](int kvh) {
-        f32x4 s[NU], o[L::NT];
-        const Query q = load_q(kvh);
-        float m = -INFINITY, l = 0.f;
+    if constexpr (AGAIN) {
+        // Heads whose values are not all finite: once over the keys for maximum and sum, once more with weights that add up to one.  V is
+        // taken in two parts: what is finite of it, and the codes of the rest against what each row sees, so that the rest reaches the
+        // rows that see it and no other.  Three to four times a head's first pass.
+        __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): behind the stores of the first pass
+        for (int kvh = h0; kvh < h1; ++kvh) {
+            if (!((again >> ((kvh - h0) & 63)) & 1)) continue;
+            f32x4 s[NU], o[L::NT];
+            const Query q = load_q(kvh);
+            float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-        for (int step = 0; step < chunks; ++step) {
-            const Place x = locate(step * L::CHUNK);
-            const float mn = fmaxf(m, scores(x, load(x, kvh), q, s));
-            l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn)) + softmax(s, mn);
-            m = mn;
-        }
-        l = quarters_sum(l);
-        // (float16: weights keep to the scale of the largest, as small ones would lose bits, and no sum of them overflows)
-        if (!std::is_same_v<T, _Float16> && l > 0.f && l < INFINITY) m += __builtin_amdgcn_logf(l);
-        clear(o);
-        float sum = 0.f;
+            for (int step = 0; step < chunks; ++step) {
+                const Place x = locate(step * L::CHUNK);
+                const float mn = fmaxf(m, scores(x, load(x, kvh), q, s));
+                l = l * (m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mn)) + softmax(s, mn);
+                m = mn;
+            }
+            l = quarters_sum(l);
+            // (float16: weights keep to the scale of the largest, as small ones would lose bits, and no sum of them overflows)
+            if (!std::is_same_v<T, _Float16> && l > 0.f && l < INFINITY) m += __builtin_amdgcn_logf(l);
+            clear(o);
+            float sum = 0.f;
 #pragma unroll 1
-        for (int step = 0; step < chunks; ++step) {
-            const Place x = locate(step * L::CHUNK);
-            const Rows16 rows = load(x, kvh);
-            scores(x, rows, q, s);
-            sum += softmax(s, m);
-            turn_v(x, rows);
-            const T *turned = turn + wave * L::WAVE_ELEMS;
+            for (int step = 0; step < chunks; ++step) {
+                const Place x = locate(step * L::CHUNK);
+                const Rows16 rows = load(x, kvh);
+                scores(x, rows, q, s);
+                sum += softmax(s, m);
+                turn_v(x, rows);
+                const T *turned = turn + wave * L::WAVE_ELEMS;
 #pragma unroll
-            for (int sb = 0; sb < L::NSB; ++sb) {
-                f32x4 count[L::VW];
+                for (int sb = 0; sb < L::NSB; ++sb) {
+                    f32x4 count[L::VW];
 #pragma unroll
-                for (int e = 0; e < L::VW; ++e) count[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int e = 0; e < L::VW; ++e) count[e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int u = 0; u < NU; ++u) {
-                    PV v[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        if constexpr (L::NARROW) v[r] = *reinterpret_cast<const PV *>(turned + (16 * u + 4 * g + r) * L::V_STRIDE + sb * L::SB + L::VW * n);
-                        else v[r] = value(x, kvh, u, sb, r);
-                    }
-#pragma unroll
-                    for (int e = 0; e < L::VW; ++e) {
-                        f32x4 &to = o[sb * L::VW + e];
-                        using V4 = T __attribute__((ext_vector_type(4)));
-                        V4 va, code, hi, lo, one;
+                    for (int u = 0; u < NU; ++u) {
+                        PV v[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            // (keys that are masked or behind the range are seen by no row)
-                            const float c = value_code(to_f32(v[r].e[e]));
-                            va[r] = c == 0.f ? v[r].e[e] : (T)0.f;
-                            code[r] = (T)c;
-                            hi[r] = from_f32<T>(s[u][r]);
-                            lo[r] = from_f32<T>(s[u][r] - to_f32(hi[r]));
-                            one[r] = (T)(x.sees[u][r] ? 1.f : 0.f);
+                            if constexpr (L::NARROW) v[r] = *reinterpret_cast<const PV *>(turned + (16 * u + 4 * g + r) * L::V_STRIDE + sb * L::SB + L::VW * n);
+                            else v[r] = value(x, kvh, u, sb, r);
                         }
-                        if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < L::VW; ++e) {
+                            f32x4 &to = o[sb * L::VW + e];
+                            using V4 = T __attribute__((ext_vector_type(4)));
+                            V4 va, code, hi, lo, one;
 #pragma unroll
                             for (int r = 0; r < 4; ++r) {
-                                to = __builtin_amdgcn_mfma_f32_16x16x4f32(va[r], s[u][r], to, 0, 0, 0);
-                                count[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(code[r], one[r], count[e], 0, 0, 0);
+                                // (keys that are masked or behind the range are seen by no row)
+                                const float c = value_code(to_f32(v[r].e[e]));
+                                va[r] = c == 0.f ? v[r].e[e] : (T)0.f;
+                                code[r] = (T)c;
+                                hi[r] = from_f32<T>(s[u][r]);
+                                lo[r] = from_f32<T>(s[u][r] - to_f32(hi[r]));
+                                one[r] = (T)(x.sees[u][r] ? 1.f : 0.f);
                             }
-                        } else {
-                            to = Mat<T>::mul16(va, hi, to);
-                            to = Mat<T>::mul16(va, lo, to);
-                            count[e] = Mat<T>::mul16(code, one, count[e]);
+                            if constexpr (F32) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) {
+                                    to = __builtin_amdgcn_mfma_f32_16x16x4f32(va[r], s[u][r], to, 0, 0, 0);
+                                    count[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(code[r], one[r], count[e], 0, 0, 0);
+                                }
+                            } else {
+                                to = Mat<T>::mul16(va, hi, to);
+                                to = Mat<T>::mul16(va, lo, to);
+                                count[e] = Mat<T>::mul16(code, one, count[e]);
+                            }
                         }
                     }
+#pragma unroll
+                    for (int e = 0; e < L::VW; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[sb * L::VW + e][r] += counted_sum(count[e][r]);
                 }
-#pragma unroll
-                for (int e = 0; e < L::VW; ++e)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[sb * L::VW + e][r] += counted_sum(count[e][r]);
+                if constexpr (L::NARROW) in_order();
             }
-            if constexpr (L::NARROW) in_order();
+            finish(kvh, sum, o);
         }
-        finish(kvh, sum, o);
-    };
-    const auto redo_noted = [&]() {
-        if (!again) return;
-        __builtin_amdgcn_s_waitcnt(0x0F70);                // vmcnt(0): behind the stores of the first pass
-        for (int kvh = h0; kvh < h1; ++kvh)
-            if ((again >> ((kvh - h0) & 63)) & 1) redo(kvh);
-    };
+        return 0;
+    }
+    const auto note = [&](int kvh, bool bad) { again |= bad ? 1ull << ((kvh - h0) & 63) : 0; };
 
     if constexpr (L::NARROW) {
         if (chunks == 1) {
@@ -601,8 +589,7 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
                 }
                 in_order();
             }
-            redo_noted();
-            return;
+            return again;
         }
     }
     for (int kvh = h0; kvh < h1; ++kvh) {
@@ -630,7 +617,33 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
         }
         note(kvh, finish(kvh, l, o));
     }
-    redo_noted();
+    return again;
+}
+
+template <class T, int DP, class OFF>
+__global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_direct_kernel(Args a, int64_t n_tiles, int heads_per_wave, int head_groups)
+{
+    using L = Direct<T, DP>;
+    __shared__ __attribute__((aligned(16))) T turn[4 * L::WAVE_ELEMS];
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned item = qcn_xcd_remap(blockIdx.x, gridDim.x);
+    const int64_t tile = item / (unsigned)head_groups;
+    const int h0 = (int)(item % (unsigned)head_groups) * heads_per_wave, h1 = h0 + heads_per_wave < a.hk ? h0 + heads_per_wave : a.hk;
+    const Tile t = find_tile(a, tile, n_tiles, 6, lane);
+    const int64_t row0 = t.row0 + 16 * wave;
+    if (t.row0 < 0 || row0 >= t.rows) return;
+    if (t.behind) {
+        const int n = lane & 15, r = 16 * wave + n;
+        if (row0 + n < t.rows)
+            for (int kvh = h0; kvh < h1; ++kvh) zero_row<T>(a, t.q_beg + t.token(r, a.group), kvh * a.group + t.sub(r, a.group), lane >> 4, 4);
+        return;
+    }
+    const uint64_t again = direct_rows<T, DP, OFF, false>(a, t, wave, lane, h0, h1, turn, 0);
+    if (again) {
+        asm("" : "+v"(lane));   // what the second pass needs of each lane is found again, not kept in registers through the first
+        direct_rows<T, DP, OFF, true>(a, t, wave, lane, h0, h1, turn, again);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -981,12 +994,14 @@ __global__ __launch_bounds__(256, DP == 32 ? 4 : 2) void attn_window_tile_kernel
     // A value that is not finite, of a key that some rows of the wave see and others do not, reaches the others as 0 * inf.  A row whose
     // weights are not numbers either (l) is NaN by itself; where a row ends before DP its last scores are products with the copied
     // start of a key, and only the second pass says.
-    bool bad = false;
+    f32x16 any = o[0];                                         // not finite if an element is not (an overflow costs a second pass)
 #pragma unroll
-    for (int i = 0; i < ND; ++i)
+    for (int i = 1; i < ND; ++i) any += o[i];
+    f32x4 four = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) bad |= !(fabsf(o[i][r]) < INFINITY);
-    const bool redo = __ballot(bad && (l == l || a.dim < DP)) != 0;
+    for (int r = 0; r < 16; ++r) four[r & 3] += any[r];
+    const float sum = (four[0] + four[1]) + (four[2] + four[3]);
+    const bool redo = __ballot(!(fabsf(sum) < INFINITY) && (l == l || a.dim < DP)) != 0;
     if (redo) any_redo = 1;
     else emit();
     __syncthreads();
