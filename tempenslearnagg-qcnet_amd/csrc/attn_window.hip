@@ -13,7 +13,7 @@
 // Both keep one running maximum and sum per row, in float32, and go over the keys once; a second time only where a value is not
 // finite (one that some rows of a wave see and others do not reaches the others as 0 * inf).  Formed again row by row and key by key, as
 // they were before, such rows made a call hundreds of times as long (16384 x 16 heads of 128, window 1024, one infinite value in the
-// first token: 101 ms, now 0.59; none: 0.17).
+// first token: 101 ms, now 0.59; none: 0.16).
 #include "sequence.hip.h"
 
 #include <type_traits>
@@ -134,7 +134,7 @@ __device__ __forceinline__ float seen_or_inf(unsigned bits, int bit, float x)
 // 8 heads of 16 33.9 and 35.4 us, 8 x 2000 steps of 16 62 and 61, float16 800 x 59 of 32 28.8 and 28.5, the second with the pass below for
 // values that are not finite; one product of twice the contraction for both was no faster).
 //
-// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 48.2 us, 4.0 TB/s, bound by
+// Measured: 1600 agents x 59 steps x 8 heads of 16 in float32, window 10 + 1 (193 MB read and written): 47.4 us, 4.1 TB/s, bound by
 // the latency of three dependent looks (boundaries, rows, LDS) at three to four waves per SIMD.  Wide float32 rows over long windows:
 // 80 Tflop/s of the 154 that a library product reaches (8 x 2000 steps, 8 heads of 64 or 128, window 500: 183 and 371 us); the L1
 // cache is what bounds them (73 % of its cycles serve a request, against 57 % of the matrix units'): a load of 16 keys serves 16 rows.
@@ -668,11 +668,12 @@ __global__ __launch_bounds__(256, (direct_waves<T, DP>())) void attn_window_dire
 // Bound by the matrix units and the vector instructions around them, which two or three waves per SIMD do not fully overlap (an
 // earlier state of the kernel, 177 us for 16384 x 16 heads of 128 and window 1024, timed with parts left out: no products 109, no
 // LDS reads 151, no exponentials 167, no copies 175).  Measured on a card at work (its first dozen launches after a pause take a tenth
-// longer): that case 160 us a call, 833 Tflop/s of the 1130 that a large library product reaches; 24 ragged prompts up to 2500 x 12 heads
-// of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10 tiles where one row's window is 8, and
-// 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32 heads of 128 behind 7000 keys each, window 4096, in three
-// parts: 105 us with the join, 680 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93 us); at dim 32 they have to be asked for, as the
-// second pass would take 135 registers of the 115 that do (800 x 59 x 8 heads, window 30: 52 us, three waves 58).
+// longer): that case 156 to 167 us a call on different cards, 800 to 857 Tflop/s of the 1130 that a large library product reaches; 24
+// ragged prompts up to 2500 x 12 heads of 64, window 512, float16: 87 us, 450 Tflop/s counting visible pairs only (32 rows see 9 or 10
+// tiles where one row's window is 8, and 2800 blocks are 3.7 rounds of the card); chunks of 200 to 333 queries x 32 heads of 128 behind
+// 7000 keys each, window 4096, in three parts: 105 us with the join, 680 Tflop/s.  Four waves per SIMD at dim 64 spill (103 against 93
+// us); at dim 32 they have to be asked for, as the second pass would take 135 registers of the 115 that do (800 x 59 x 8 heads, window
+// 30: 52 us, three waves 58).
 template <int LS> __device__ __forceinline__ int k_piece(int row, int piece)
 {
     return piece ^ (LS == 128 ? row & 15 : LS == 64 ? (row >> 1) & 7 : (row >> 2) & 3);

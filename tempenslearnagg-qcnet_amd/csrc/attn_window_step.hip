@@ -92,8 +92,8 @@ struct StepArgs {
 // read (us, one product and two, with the look for values that are not finite that the second needs): 64 x 8 key heads x 4100 slots 170 and
 // 171, one request 19.9 and 20.4, 256 x 4 heads of 64 x 1004 slots 47.8 and 48.5, 64 x 8 x 240 slots 25.1 and 26.6, 1600 agents x 8 x 51
 // slots in bfloat16 19.2 and 20.2.
-// Measured: that step (64 requests x 32 heads of 128 in bfloat16) 168 us, 984 MB at 5.9 TB/s; one request 9.8 + 4.1
-// us (two launches, three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21 us, 4 TB/s.
+// Measured: that step (64 requests x 32 heads of 128 in bfloat16) 169.7 us, 984 MB at 5.8 TB/s; one request 10.4 + 4.7 us (two launches,
+// three memory latencies each); 1600 agents x 8 heads of 16 x 51 slots in float32 21.9 us, 3.6 TB/s.
 template <class T, int DP> struct Step {
     static constexpr bool F32 = sizeof(T) == 4;
     static constexpr int NU = DP <= 32 ? 4 : 2, CHUNK = 16 * NU;                        // slots of a chunk: narrow heads take 64
